@@ -302,6 +302,86 @@ int w4a16_attention_decode_f16(const void* qkv, void* k_cache, void* v_cache, vo
                                float softmax_scale, uint32_t* status, uint32_t flags, w4a16_stream_t stream);
 
 /*
+ * Rotary positions and an 8-bit key/value cache (no counterpart in the reference, which leaves both to HuggingFace).
+ *
+ * The cache of one attention layer holds, for every sequence and key/value head, blocks of 32 tokens:
+ *   a full block     8-bit codes, with one FP32 scale for its keys and one for its values:
+ *                      scale = max |x| / 127 over the block's 32 * head_dim numbers
+ *                      code  = round_half_even(127 * x / max |x|), value = code * scale
+ *   the newest block, while it is being filled: the numbers as they came (16 bits).
+ * So what it holds depends on the tokens alone, not on how many came at a time, and each number is rounded once.  A block with an
+ * infinity or NaN gets the scale NaN and reads back as NaN.  The number of tokens held is the caller's to keep (device words, so
+ * that a captured graph serves every step); it may be set back, as after refused drafts, to as far as the beginning of the block
+ * before the newest one that was reached.
+ *
+ * Sizes: head_dim 64 or 128, any max_len >= 1.  `type` says what the numbers outside of the codes are.  Every device word that
+ * names a length, start or count outside its range makes the kernel leave that sequence alone (its outputs are zeros), and sets bit 0
+ * of *status; bit 1 says that a bounded wait ran out, and that outputs are incomplete.
+ */
+enum { W4A16_TYPE_F16 = 0, W4A16_TYPE_BF16 = 1 };
+
+typedef struct w4a16_kv8_cache {
+    void* k_codes;                /* [batch * kv_heads][max_len / 32][32 * head_dim], in an order of the library's own */
+    void* v_codes;
+    float* k_scales;              /* [batch * kv_heads][max_len / 32]                              */
+    float* v_scales;
+    void* k_tail;                 /* [batch * kv_heads][2][32][head_dim]                           */
+    void* v_tail;
+    uint32_t* status;
+    int32_t batch, kv_heads, max_len, head_dim;
+    int32_t type;                 /* W4A16_TYPE_*                                                  */
+} w4a16_kv8_cache;
+
+/* 16-bit numbers [batch][tokens][heads][head_dim]: strides in numbers, the last dimension contiguous. */
+typedef struct w4a16_rows {
+    const void* data;
+    int64_t batch_stride, token_stride, head_stride;
+} w4a16_rows;
+
+/* Pair j of a head at position p is turned by p * inv_freq[j], the angle formed in FP64: (a, b) -> (a cos - b sin, b cos + a sin) with
+ * cos and sin times `scale`, in FP32, rounded once.  Pairs are (2j, 2j + 1) if `interleaved`, else (j, j + rotary_dim / 2); numbers
+ * from rotary_dim on stay as they are.  rotary_dim: even, 2 .. head_dim. */
+typedef struct w4a16_rotary_spec {
+    const float* inv_freq;        /* [rotary_dim / 2]                                              */
+    int32_t rotary_dim;
+    int32_t interleaved;
+    float scale;
+} w4a16_rotary_spec;
+
+/* Bytes of device memory (256-byte aligned, zero-filled before its first use) that a cache takes (0: sizes out of range), and the parts
+ * of it.  Host code only. */
+size_t w4a16_kv8_cache_bytes(int64_t batch, int64_t kv_heads, int64_t max_len, int64_t head_dim);
+int w4a16_kv8_cache_describe(void* memory, size_t bytes, int64_t batch, int64_t kv_heads, int64_t max_len, int64_t head_dim,
+                             int32_t type, w4a16_kv8_cache* cache);
+
+/* out = x with its heads turned; positions int64 [batch * tokens].  head_dim: even, up to 256.  out->data may be x->data with the same
+ * strides (in place); otherwise the two must not overlap. */
+int w4a16_rotary(const w4a16_rotary_spec* spec, const w4a16_rows* x, const w4a16_rows* out, int64_t batch, int64_t tokens,
+                 int32_t heads, int32_t head_dim, const int64_t* positions, int32_t type, uint32_t flags, w4a16_stream_t stream);
+
+/* Writes counts[b] (NULL: all) of the `tokens` new keys and values of each sequence at positions start[b], start[b] + 1, ...
+ * With `rotary` the keys are turned on the way (position = place in the cache), and the queries q (may be NULL), all `tokens` of
+ * them, from q to q_out: the bits of a w4a16_rotary call in front. */
+int w4a16_kv8_append(const w4a16_kv8_cache* cache, const w4a16_rows* k, const w4a16_rows* v, int64_t tokens, const int64_t* start,
+                     const int64_t* counts, const w4a16_rotary_spec* rotary, const w4a16_rows* q, const w4a16_rows* q_out,
+                     int32_t q_heads, uint32_t flags, w4a16_stream_t stream);
+
+/* The values held at positions first[b] (NULL: 0) .. first[b] + tokens - 1 of sequences of lengths[b] tokens, zeros behind the
+ * last: k_out, v_out [batch][tokens][kv_heads][head_dim] of the cache's type. */
+int w4a16_kv8_read(const w4a16_kv8_cache* cache, const int64_t* lengths, const int64_t* first, int64_t tokens, void* k_out,
+                   void* v_out, uint32_t flags, w4a16_stream_t stream);
+
+/* out [batch][tokens][q_heads][head_dim] = attention of the newest tokens over the cache: lengths[b] counts them too, query i of
+ * counts[b] (NULL: all `tokens`) stands at position lengths[b] - counts[b] + i and sees the positions up to its own.  Rows behind a
+ * sequence's last query, and rows that see nothing, are zeros.  q_heads is a multiple of kv_heads.  The workspace (16-byte aligned)
+ * must hold w4a16_kv8_attention_workspace_bytes(); its contents do not matter, before or after; calls that may overlap need one
+ * each. */
+size_t w4a16_kv8_attention_workspace_bytes(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t tokens);
+int w4a16_kv8_attention(const w4a16_kv8_cache* cache, const w4a16_rows* q, void* out, int32_t q_heads, int64_t tokens,
+                        const int64_t* lengths, const int64_t* counts, float softmax_scale, void* workspace,
+                        size_t workspace_bytes, uint32_t flags, w4a16_stream_t stream);
+
+/*
  * One whole decode step (batch 1) of a LLaMA-architecture model as ONE cooperative kernel launch: resident
  * CTAs walk a prebuilt list of operations (per block: fused q/k/v with add + RMSNorm inside, attention, o_proj,
  * fused gate/up with add + RMSNorm inside, down_proj with SiLU * up inside; then lm_head with the final norm and

@@ -5,6 +5,7 @@ from .cuda import (check_device_status, cuda_extension_available, dequantize_cud
                    quantize_and_pack_cuda)
 from .fusion import FusedQuantizedLinear, FusedSlice, fuse_parallel_linears
 from .integration import load_packed_state_dict, replace_linear_layers
+from .kv_cache import QuantizedKVCache, apply_rotary
 from .linear import Int4Linear, QuantizedLinear
 from .quantization import pack_int4, quantize_and_pack_weights, quantize_groupwise, unpack_int4
 
@@ -25,6 +26,8 @@ __all__ = [
     "fuse_parallel_linears",
     "FusedQuantizedLinear",
     "FusedSlice",
+    "QuantizedKVCache",
+    "apply_rotary",
     "linear_cuda",
     "dequantize_cuda",
     "quantize_and_pack_cuda",

@@ -28,7 +28,8 @@ CORE_LIB = PKG / "libw4a16_b200.so"
 CHECKED_LIB = PKG / "libw4a16_b200_checked.so"
 TORCH_LIB = PKG / "_C.so"
 
-CUDA_SOURCES = ["capi.cu", "linear_mma.cu", "linear_mma_groups.cu", "linear_generic.cu", "dequantize.cu", "linear_static_scratch.cu", "linear_gemm.cu", "linear_gemm_pair.cu", "quantize.cu", "decode_ops.cu", "decode_persistent.cu"]
+CUDA_SOURCES = ["capi.cu", "linear_mma.cu", "linear_mma_groups.cu", "linear_generic.cu", "dequantize.cu", "linear_static_scratch.cu", "linear_gemm.cu", "linear_gemm_pair.cu", "quantize.cu", "decode_ops.cu", "decode_persistent.cu",
+                "kv_cache.cu", "kv_attention.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++20", "-lineinfo",
@@ -120,7 +121,7 @@ def build_torch_shim(force: bool = False) -> pathlib.Path:
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         "-DTORCH_EXTENSION_NAME=_C",
         *includes, "-I", str(INCLUDE),
-        str(CSRC / "int4_linear.cpp"), str(CSRC / "linear_module.cpp"), "-o", str(TORCH_LIB),
+        str(CSRC / "int4_linear.cpp"), str(CSRC / "linear_module.cpp"), str(CSRC / "kv_module.cpp"), "-o", str(TORCH_LIB),
         f"-L{torch_lib_dir}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
         f"-L{PKG}", "-l:libw4a16_b200.so",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib_dir}",

@@ -89,6 +89,28 @@ class DecodePlanInfo(ctypes.Structure):
                 ("grid", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("smem_bytes", ctypes.c_uint32)]
 
 
+class KV8Cache(ctypes.Structure):
+    """``w4a16_kv8_cache``."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail", "status")] + [
+        (name, ctypes.c_int32) for name in ("batch", "kv_heads", "max_len", "head_dim", "type")]
+
+
+class Rows(ctypes.Structure):
+    """``w4a16_rows``."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class RotarySpec(ctypes.Structure):
+    """``w4a16_rotary_spec``."""
+
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int64
 
@@ -123,6 +145,25 @@ C_API = {
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_float,
          ctypes.c_float, _P, ctypes.c_uint32, _P],
+    ),
+    "w4a16_kv8_cache_bytes": (ctypes.c_size_t, [_I, _I, _I, _I]),
+    "w4a16_kv8_cache_describe": (ctypes.c_int, [_P, ctypes.c_size_t, _I, _I, _I, _I, ctypes.c_int32, ctypes.POINTER(KV8Cache)]),
+    "w4a16_rotary": (
+        ctypes.c_int,
+        [ctypes.POINTER(RotarySpec), ctypes.POINTER(Rows), ctypes.POINTER(Rows), _I, _I, ctypes.c_int32, ctypes.c_int32, _P,
+         ctypes.c_int32, ctypes.c_uint32, _P],
+    ),
+    "w4a16_kv8_append": (
+        ctypes.c_int,
+        [ctypes.POINTER(KV8Cache), ctypes.POINTER(Rows), ctypes.POINTER(Rows), _I, _P, _P, ctypes.POINTER(RotarySpec),
+         ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.c_int32, ctypes.c_uint32, _P],
+    ),
+    "w4a16_kv8_read": (ctypes.c_int, [ctypes.POINTER(KV8Cache), _P, _P, _I, _P, _P, ctypes.c_uint32, _P]),
+    "w4a16_kv8_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(KV8Cache), ctypes.c_int32, _I]),
+    "w4a16_kv8_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(KV8Cache), ctypes.POINTER(Rows), _P, ctypes.c_int32, _I, _P, _P, ctypes.c_float, _P, ctypes.c_size_t,
+         ctypes.c_uint32, _P],
     ),
     "w4a16_decode_plan_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecodeModel)]),
     "w4a16_decode_plan_build": (ctypes.c_int, [ctypes.POINTER(DecodeModel), _P, ctypes.c_size_t, _P, _P,

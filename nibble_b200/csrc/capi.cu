@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "kernels.h"
+#include "kv_cache.cuh"
 
 namespace w4a16 {
 std::atomic<uint64_t> g_launch_count{0};
@@ -455,6 +456,137 @@ int w4a16_attention_decode_f16(const void* qkv, void* k_cache, void* v_cache, vo
                                           reinterpret_cast<const long long*>(position), inv_freq, q_heads, kv_heads, head_dim,
                                           max_len, rope_scale, softmax_scale, status,
                                           (flags & W4A16_FLAG_PROGRAMMATIC_LAUNCH) != 0, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ------------------------------------------------------------------ rotary positions and the 8-bit cache
+
+static bool fits_cache(int64_t batch, int64_t kv_heads, int64_t max_len, int64_t head_dim) {
+    if (batch <= 0 || kv_heads <= 0 || max_len <= 0 || (head_dim != 64 && head_dim != 128)) return false;
+    return batch <= INT32_MAX && kv_heads <= INT32_MAX / batch && max_len <= INT32_MAX - 64 &&
+           batch * kv_heads <= INT32_MAX / (max_len / w4a16::kKvBlock + 1);
+}
+
+static int check_cache(const w4a16_kv8_cache* cache) {
+    if (cache == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (!fits_cache(cache->batch, cache->kv_heads, cache->max_len, cache->head_dim)) return W4A16_ERR_BAD_SHAPE;
+    if (cache->type != W4A16_TYPE_F16 && cache->type != W4A16_TYPE_BF16) return W4A16_ERR_BAD_CONFIG;
+    const void* parts[] = {cache->k_codes, cache->v_codes, cache->k_scales, cache->v_scales, cache->k_tail, cache->v_tail, cache->status};
+    for (const void* part : parts) {
+        if (part == nullptr) return W4A16_ERR_NULL_POINTER;
+        if (!aligned16(part)) return W4A16_ERR_MISALIGNED;
+    }
+    return W4A16_OK;
+}
+
+static int check_rows(const w4a16_rows* rows) {
+    if (rows == nullptr || rows->data == nullptr) return W4A16_ERR_NULL_POINTER;
+    return reinterpret_cast<uintptr_t>(rows->data) % 2 == 0 ? W4A16_OK : W4A16_ERR_MISALIGNED;
+}
+
+static int check_spec(const w4a16_rotary_spec* spec, int64_t head_dim) {
+    if (spec == nullptr || spec->inv_freq == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (spec->rotary_dim < 2 || spec->rotary_dim % 2 != 0 || spec->rotary_dim > head_dim) return W4A16_ERR_BAD_SHAPE;
+    return reinterpret_cast<uintptr_t>(spec->inv_freq) % 4 == 0 ? W4A16_OK : W4A16_ERR_MISALIGNED;
+}
+
+static bool programmatic(uint32_t flags) { return (flags & W4A16_FLAG_PROGRAMMATIC_LAUNCH) != 0; }
+
+size_t w4a16_kv8_cache_bytes(int64_t batch, int64_t kv_heads, int64_t max_len, int64_t head_dim) {
+    if (!fits_cache(batch, kv_heads, max_len, head_dim)) return 0;
+    w4a16_kv8_cache unused;
+    return w4a16::kv_cache_layout(nullptr, batch, kv_heads, max_len, head_dim, &unused);
+}
+
+int w4a16_kv8_cache_describe(void* memory, size_t bytes, int64_t batch, int64_t kv_heads, int64_t max_len, int64_t head_dim, int32_t type,
+                             w4a16_kv8_cache* cache) {
+    if (memory == nullptr || cache == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (!fits_cache(batch, kv_heads, max_len, head_dim)) return W4A16_ERR_BAD_SHAPE;
+    if (type != W4A16_TYPE_F16 && type != W4A16_TYPE_BF16) return W4A16_ERR_BAD_CONFIG;
+    if (reinterpret_cast<uintptr_t>(memory) % 256 != 0) return W4A16_ERR_MISALIGNED;
+    if (bytes < w4a16_kv8_cache_bytes(batch, kv_heads, max_len, head_dim)) return W4A16_ERR_WORKSPACE;
+    w4a16::kv_cache_layout(memory, batch, kv_heads, max_len, head_dim, cache);
+    cache->type = type;
+    return W4A16_OK;
+}
+
+int w4a16_rotary(const w4a16_rotary_spec* spec, const w4a16_rows* x, const w4a16_rows* out, int64_t batch, int64_t tokens,
+                 int32_t heads, int32_t head_dim, const int64_t* positions, int32_t type, uint32_t flags, w4a16_stream_t stream) {
+    if (batch < 0 || tokens < 0 || heads < 0 || head_dim < 2 || head_dim % 2 != 0 || head_dim > 256) return W4A16_ERR_BAD_SHAPE;
+    if (type != W4A16_TYPE_F16 && type != W4A16_TYPE_BF16) return W4A16_ERR_BAD_CONFIG;
+    if (batch == 0 || tokens == 0 || heads == 0) return W4A16_OK;
+    for (const int status : {check_spec(spec, head_dim), check_rows(x), check_rows(out)}) {
+        if (status != W4A16_OK) return status;
+    }
+    if (positions == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (x->data == out->data && (x->batch_stride != out->batch_stride || x->token_stride != out->token_stride ||
+                                 x->head_stride != out->head_stride)) {
+        return W4A16_ERR_BAD_CONFIG;
+    }
+    return w4a16::launch_rotary(*spec, *x, *out, batch, tokens, heads, head_dim, reinterpret_cast<const long long*>(positions),
+                                type == W4A16_TYPE_BF16, programmatic(flags), reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_kv8_append(const w4a16_kv8_cache* cache, const w4a16_rows* k, const w4a16_rows* v, int64_t tokens, const int64_t* start,
+                     const int64_t* counts, const w4a16_rotary_spec* rotary, const w4a16_rows* q, const w4a16_rows* q_out, int32_t q_heads,
+                     uint32_t flags, w4a16_stream_t stream) {
+    if (const int status = check_cache(cache); status != W4A16_OK) return status;
+    if (tokens < 0) return W4A16_ERR_BAD_SHAPE;
+    if (tokens == 0) return W4A16_OK;
+    for (const int status : {check_rows(k), check_rows(v)}) {
+        if (status != W4A16_OK) return status;
+    }
+    if (start == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (rotary != nullptr) {
+        if (const int status = check_spec(rotary, cache->head_dim); status != W4A16_OK) return status;
+    }
+    if (q != nullptr) {
+        if (rotary == nullptr) return W4A16_ERR_BAD_CONFIG;
+        if (q_heads <= 0) return W4A16_ERR_BAD_SHAPE;
+        for (const int status : {check_rows(q), check_rows(q_out)}) {
+            if (status != W4A16_OK) return status;
+        }
+        if (q->data == q_out->data && (q->batch_stride != q_out->batch_stride || q->token_stride != q_out->token_stride ||
+                                       q->head_stride != q_out->head_stride)) {
+            return W4A16_ERR_BAD_CONFIG;
+        }
+    }
+    return w4a16::launch_kv_append(*cache, *k, *v, tokens, reinterpret_cast<const long long*>(start),
+                                   reinterpret_cast<const long long*>(counts), rotary, q, q_out, q_heads, programmatic(flags),
+                                   reinterpret_cast<cudaStream_t>(stream));
+}
+
+int w4a16_kv8_read(const w4a16_kv8_cache* cache, const int64_t* lengths, const int64_t* first, int64_t tokens, void* k_out, void* v_out,
+                   uint32_t flags, w4a16_stream_t stream) {
+    if (const int status = check_cache(cache); status != W4A16_OK) return status;
+    if (tokens < 0) return W4A16_ERR_BAD_SHAPE;
+    if (tokens == 0) return W4A16_OK;
+    if (lengths == nullptr || k_out == nullptr || v_out == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (!aligned16(k_out) || !aligned16(v_out)) return W4A16_ERR_MISALIGNED;
+    return w4a16::launch_kv_read(*cache, reinterpret_cast<const long long*>(lengths), reinterpret_cast<const long long*>(first), tokens,
+                                 k_out, v_out, programmatic(flags), reinterpret_cast<cudaStream_t>(stream));
+}
+
+static bool fits_queries(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t tokens) {
+    return q_heads > 0 && q_heads % cache->kv_heads == 0 && tokens >= 0 && tokens <= INT32_MAX / 64 / q_heads;
+}
+
+size_t w4a16_kv8_attention_workspace_bytes(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t tokens) {
+    if (check_cache(cache) != W4A16_OK || !fits_queries(cache, q_heads, tokens) || tokens == 0) return 0;
+    return w4a16::kv_attention_workspace_bytes(*cache, q_heads, tokens);
+}
+
+int w4a16_kv8_attention(const w4a16_kv8_cache* cache, const w4a16_rows* q, void* out, int32_t q_heads, int64_t tokens,
+                        const int64_t* lengths, const int64_t* counts, float softmax_scale, void* workspace, size_t workspace_bytes,
+                        uint32_t flags, w4a16_stream_t stream) {
+    if (const int status = check_cache(cache); status != W4A16_OK) return status;
+    if (!fits_queries(cache, q_heads, tokens)) return W4A16_ERR_BAD_SHAPE;
+    if (tokens == 0) return W4A16_OK;
+    if (const int status = check_rows(q); status != W4A16_OK) return status;
+    if (out == nullptr || lengths == nullptr) return W4A16_ERR_NULL_POINTER;
+    if (!aligned16(out) || !aligned16(workspace)) return W4A16_ERR_MISALIGNED;
+    return w4a16::launch_kv_attention(*cache, *q, out, q_heads, tokens, reinterpret_cast<const long long*>(lengths),
+                                      reinterpret_cast<const long long*>(counts), softmax_scale, workspace, workspace_bytes,
+                                      programmatic(flags), reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
