@@ -2,8 +2,9 @@
 //
 // Query i of `count` stands at position length - count + i and sees the positions up to its own:
 //     out = sum_t p_t v_t / sum_t p_t,   p_t = exp(softmax_scale * q . k_t - max)
-// The queries of all heads that share a key/value head are rows of one problem (row = i * group + head in group), 16 of them a
-// tile of mma.sync m16n8k16.  Codes enter the products as exact FP16 integers, made of bytes by OR-ing them into 1024.0 (one LOP3 for
+// The queries of all heads that share a key/value head are rows of one problem (row = i * group + head in group).  They are the
+// eight columns of mma.sync m16n8k16, and keys and (transposed) values its sixteen rows: one token of a model with eight query heads
+// for each key/value head fills a tile.  (With the queries as the sixteen rows half of every tile was empty: 48.)  Codes enter the products as exact FP16 integers, made of bytes by OR-ing them into 1024.0 (one LOP3 for
 // two, then 1152 is subtracted); the key's scale multiplies the FP32 score, the value's goes into the probability before that is
 // rounded to FP16, both relative to the block at which the accumulator was last rescaled.  FP16 has its eleven bits for
 // probabilities down to 2^-24 of the largest (they are held times 2^10), so a weight is off by 2^-12 of itself at most on average
@@ -16,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <limits.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -32,6 +35,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMinRun = 2 * kWarps;             // blocks that are worth a CTA
+constexpr int kUnitCost = 4;                    // what starting and ending a sequence, head and tile costs, in blocks
 constexpr float kNone = -1.0e30f;               // the maximum of nothing
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;            // probabilities are held in FP16 times this: 2^10,
@@ -45,44 +49,91 @@ struct AttentionParams {
     bool q_wide;                                 // rows can be read 16 bytes at a time
     char* out;                                   // [batch][tokens][q heads][D]
     int tokens, q_heads, group;
-    int row_tiles;                               // of 16 * MT rows: as many as `tokens` queries make
+    int tile_rows, row_tiles;                    // rows of a CTA, and as many tiles as `tokens` queries make
     const long long* lengths;
     const long long* counts;                     // null: all `tokens` of every sequence
     float scale;                                 // softmax scale * log2 e
     float* parts;                                // workspace: see part_of()
     int grid;                                    // CTAs of the first kernel
-    bool split;                                  // whether runs may cut a sequence and head
 };
 
 struct Sequence {
-    int length, count, blocks, row_tiles;        // row_tiles: of this sequence's queries, 0 when there is nothing to do
+    int length, count, blocks, row_tiles;        // full blocks; tiles of this sequence's queries
+    bool sound;
 };
 
-__device__ __forceinline__ Sequence sequence_of(const AttentionParams& p, int b, int tile_rows) {
-    Sequence s{0, 0, 0, 0};
+__device__ __forceinline__ Sequence sequence_of(const AttentionParams& p, int b) {
+    Sequence s{0, 0, 0, 0, false};
     const long long length = p.lengths[b], count = p.counts == nullptr ? p.tokens : p.counts[b];
     if (length < 0 || length > p.cache.max_len || count < 0 || count > p.tokens) return s;
     s.length = static_cast<int>(length);
     s.count = static_cast<int>(count);
-    s.blocks = (s.length + kKvBlock - 1) / kKvBlock;
-    s.row_tiles = s.blocks > 0 ? (s.count * p.group + tile_rows - 1) / tile_rows : 0;
+    s.blocks = s.length / kKvBlock;
+    s.row_tiles = (s.count * p.group + p.tile_rows - 1) / p.tile_rows;
+    s.sound = true;
     return s;
 }
 
-__device__ __forceinline__ long long work_of(const AttentionParams& p, const Sequence& s) {
-    return static_cast<long long>(s.blocks) * s.row_tiles * p.cache.kv_heads;
+// Work of a sequence's heads and tiles, in blocks: each starts and ends at the cost of some.  (All of it is less than 2^31: the
+// launcher sees to that.)
+__device__ __forceinline__ int work_of(const AttentionParams& p, const Sequence& s) {
+    return s.blocks == 0 ? 0 : (s.blocks + kUnitCost) * s.row_tiles * p.cache.kv_heads;
 }
 
-// The part of (sequence, head, tile) that a CTA's run holds: its first segment or its last.
-__device__ __forceinline__ float* part_of(const AttentionParams& p, int cta, bool first, int tile_rows, int d) {
-    return p.parts + (static_cast<size_t>(cta) * 2 + (first ? 0 : 1)) * tile_rows * (d + 2);
+// What a run has of a sequence, head and tile: for each row D sums, their maximum and the sum of the weights.  Along the runs either
+// the tile or the run goes up from one piece to the next, so their sum names the piece.
+__device__ __forceinline__ float* part_of(const AttentionParams& p, int b, int head, int tile, int run, int d) {
+    const size_t piece = (static_cast<size_t>(b) * p.cache.kv_heads + head) * p.row_tiles + tile + run;
+    return p.parts + piece * p.tile_rows * (d + 2);
 }
 
-// All blocks of all sequences, and CTAs that share them.
-__device__ __forceinline__ int active_ctas(const AttentionParams& p, long long total) {
-    return static_cast<int>(max(1ll, min(static_cast<long long>(p.grid), total / kMinRun)));
+// All work in equal runs: the first `longer` are one block longer than the others.
+struct Runs {
+    int active, length, longer;
+    __device__ __forceinline__ Runs(const AttentionParams& p, int total)
+        : active(max(1, min(p.grid, total / kMinRun))), length(total / active), longer(total - active * length) {}
+    __device__ __forceinline__ int begin(int cta) const { return cta * length + min(cta, longer); }
+    __device__ __forceinline__ int of(int block) const {
+        const int in_longer = longer * (length + 1);
+        return block < in_longer ? block / (length + 1) : longer + (block - in_longer) / length;
+    }
+};
+
+// A piece of one sequence, head and tile: full blocks [begin, stop).
+struct Segment {
+    int b, length, count, head, tile, begin, stop;
+};
+
+// Where the next segment of a run up to `end` is looked for: sequence b, the work before it, and the run's next piece of work.
+struct Place {
+    int b, base, position;
+};
+
+__device__ __forceinline__ bool next_segment(const AttentionParams& p, int end, Place& at, Segment& seg) {
+    while (at.position < end && at.b < p.cache.batch) {
+        const Sequence s = sequence_of(p, at.b);
+        const int work = work_of(p, s);
+        if (at.position >= at.base + work) {
+            at.base += work;
+            ++at.b;
+            continue;
+        }
+        const int cost = s.blocks + kUnitCost;
+        const int unit = (at.position - at.base) / cost, from = at.position - at.base - unit * cost;
+        const int to = min(cost, from + end - at.position);
+        at.position += to - from;
+        seg.begin = max(0, from - kUnitCost);
+        seg.stop = max(0, to - kUnitCost);
+        if (seg.begin == seg.stop) continue;
+        seg.length = s.length;
+        seg.count = s.count;
+        seg.head = unit / s.row_tiles;
+        seg.tile = unit - seg.head * s.row_tiles;
+        seg.b = at.b;
+        return true;
+    }
+    return false;
 }
-__device__ __forceinline__ long long run_begin(long long total, int active, int cta) { return total * cta / active; }
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -113,6 +164,13 @@ __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigne
                  : "memory");
 }
 
+// A matrix of 8 x 8 16-bit numbers, two of a row in each lane, transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t pair) {
+    uint32_t out;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(out) : "r"(pair));
+    return out;
+}
+
 // A power of two that brings `top` to between 2^9 and 2^10 (1 for zero), and its inverse.
 __device__ __forceinline__ float power_for(float top, float& inverse) {
     const int exponent = top > 0.0f ? max(-100, min(100, 9 - ilogbf(top))) : 0;
@@ -125,580 +183,584 @@ __device__ __forceinline__ float finite_magnitude(float x) {
     return m <= 3.4028235e38f ? m : 0.0f;
 }
 
-// A team of MT warps shares a ring; each has a 16-row tile of its own, and the kWarps / MT teams take the blocks in turn.
-template <typename T, int D, int MT>
+// A team of MT warps shares a ring; each has 8 * NT rows of its own, and the kWarps / MT teams take the blocks in turn.
+template <typename T, int D, int NT, int MT>
 struct AttentionShape {
     static constexpr int kTeams = kWarps / MT;
-    static constexpr int kTileRows = 16 * MT;
-    static constexpr int kBlockBytes = kKvBlock * D;                   // of keys, and of values
-    static constexpr int kStages = 2 * MT * (128 / D);                 // blocks of a ring: 64 KB for a CTA, two of which fit an SM
-    static constexpr size_t kRingBytes = static_cast<size_t>(kTeams) * kStages * 2 * kBlockBytes;
-    static constexpr size_t kMergeBytes = static_cast<size_t>(kTeams) * kTileRows * (D + 2) * sizeof(float);
-    static constexpr size_t kSharedBytes = kRingBytes + (kTeams > 1 ? kMergeBytes : 0);
+    static constexpr int kTileRows = 8 * NT * MT;
+    static constexpr int kSlotBytes = kKvBlock * D;                    // a block's keys, or its values
+    static constexpr int kSlots = (NT == 1 ? 3 : MT == 1 ? 4 : 8) * (128 / D);
+    static constexpr int kResident = NT == 1 ? 3 : 2;                  // CTAs that fit an SM
+    static constexpr size_t kRingBytes = static_cast<size_t>(kTeams) * kSlots * kSlotBytes;
+    static constexpr size_t kSharedBytes = kRingBytes + static_cast<size_t>(kTeams) * kTileRows * (D + 2) * sizeof(float);
+    static_assert(kResident * (kSharedBytes + 2048) <= 227 * 1024);
 };
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kThreads, 2)
+// What one thread of a team asks for next.  It runs ahead of the team by the ring's slots, across the ends of segments.
+struct Feed {
+    Place at;
+    int left;                          // slots of this segment that have not been asked for
+    const uint8_t *keys, *values;      // the team's next block
+    unsigned fill;
+};
+
+template <typename T, int D, int NT, int MT>
+__global__ void __launch_bounds__(kThreads, AttentionShape<T, D, NT, MT>::kResident)
 kv_attention_kernel(const AttentionParams p) {
-    using Shape = AttentionShape<T, D, MT>;
-    constexpr int kTeams = Shape::kTeams, kStages = Shape::kStages, kTileRows = Shape::kTileRows, kSteps = D / 16, kTiles = D / 8;
+    using Shape = AttentionShape<T, D, NT, MT>;
+    constexpr int kTeams = Shape::kTeams, kSlots = Shape::kSlots, kTileRows = Shape::kTileRows, kSteps = D / 16;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(128) uint8_t shared[];
-    __shared__ __align__(8) unsigned long long bars[kTeams][kStages][2];      // full, empty
-    __shared__ long long plan[2];                                              // all blocks; blocks before this CTA's sequence
-    __shared__ int plan_b;
-    pdl_release_downstream();
+    __shared__ __align__(8) unsigned long long bars[kTeams][kSlots][2];        // full; empty, where several warps share a ring
+    __shared__ Feed feeds[kTeams];
+    __shared__ int plan[3];                    // all work; this CTA's sequence; work before it
     pdl_wait_for_upstream();
+    pdl_release_downstream();                  // (behind the wait: what the next kernel reads of ours before its own wait is there)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int team = warp / MT, member = warp % MT;
     const int g = lane >> 2, c = lane & 3;
-    uint8_t* const ring = shared + static_cast<size_t>(team) * kStages * 2 * Shape::kBlockBytes;
+    uint8_t* const ring = shared + static_cast<size_t>(team) * kSlots * Shape::kSlotBytes;
     float* const merge = reinterpret_cast<float*>(shared + Shape::kRingBytes);
-    if (lane == 0 && member == 0) {
-        for (int s = 0; s < kStages; ++s) {
+    const bool feeder = lane == 0 && member == 0;
+    if (feeder) {
+        for (int s = 0; s < kSlots; ++s) {
             mbar_init(smem_u32(&bars[team][s][0]), 1);
             mbar_init(smem_u32(&bars[team][s][1]), MT);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // rows of queries that are not there
-    for (long long at = blockIdx.x; at < static_cast<long long>(p.cache.batch) * p.tokens; at += gridDim.x) {
-        const int b = static_cast<int>(at / p.tokens), i = static_cast<int>(at % p.tokens);
-        const Sequence s = sequence_of(p, b, kTileRows);
-        if (i < s.count && s.blocks > 0) continue;
-        const long long length = p.lengths[b], count = p.counts == nullptr ? p.tokens : p.counts[b];
-        if (tid == 0 && (length < 0 || length > p.cache.max_len || count < 0 || count > p.tokens)) {
-            atomicOr(p.cache.status, kKvBadLength);
-        }
-        uint4* to = reinterpret_cast<uint4*>(p.out + at * p.q_heads * D * 2);
-        for (int e = tid; e < p.q_heads * D / 8; e += kThreads) to[e] = make_uint4(0u, 0u, 0u, 0u);
-    }
     // this CTA's run: where it begins
-    if (warp == 0) {
-        long long total = 0;
-        for (int b = lane; b < p.cache.batch; b += 32) total += work_of(p, sequence_of(p, b, kTileRows));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        long long mine = -1;
+    if (p.cache.batch > 1 && warp == 0) {
+        const int first_work = lane < p.cache.batch ? work_of(p, sequence_of(p, lane)) : 0;
+        int total = first_work;
+        for (int b = lane + 32; b < p.cache.batch; b += 32) total += work_of(p, sequence_of(p, b));
+        total = __reduce_add_sync(0xffffffffu, total);
+        int mine = -1;
         if (total > 0) {
-            if (p.split) {
-                const int active = active_ctas(p, total);
-                if (static_cast<int>(blockIdx.x) < active) mine = run_begin(total, active, blockIdx.x);
-            }
+            const Runs runs(p, total);
+            if (static_cast<int>(blockIdx.x) < runs.active) mine = runs.begin(blockIdx.x);
         }
-        if (p.split && mine >= 0) {
-            long long before = 0;
-            for (int base = 0; base < p.cache.batch; base += 32) {
-                const long long work = base + lane < p.cache.batch ? work_of(p, sequence_of(p, base + lane, kTileRows)) : 0;
-                long long upto = work;
+        int before = 0;
+        for (int base = 0; mine >= 0 && base < p.cache.batch; base += 32) {
+            const int work = base == 0 ? first_work : base + lane < p.cache.batch ? work_of(p, sequence_of(p, base + lane)) : 0;
+            int upto = work;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += other;
-                }
-                const unsigned past = __ballot_sync(0xffffffffu, before + upto > mine);
-                if (past != 0) {
-                    const int at = __ffs(past) - 1;
-                    if (lane == at) {
-                        plan[1] = before + upto - work;
-                        plan_b = base + at;
-                    }
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, upto, 31);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += other;
             }
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > mine);
+            if (past != 0) {
+                const int at = __ffs(past) - 1;
+                if (lane == at) {
+                    plan[1] = base + at;
+                    plan[2] = before + upto - work;
+                }
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (lane == 0) plan[0] = p.split && mine < 0 ? 0 : total;
+        if (lane == 0) plan[0] = total;
     }
     __syncthreads();
-    const long long total = plan[0];
+    const int total = p.cache.batch > 1 ? plan[0] : work_of(p, sequence_of(p, 0));
     if (total == 0) return;
-    int b;
-    long long base, position, end;             // blocks before sequence b; this run's next block and end
-    if (p.split) {
-        const int active = active_ctas(p, total);
-        b = plan_b;
-        base = plan[1];
-        position = run_begin(total, active, blockIdx.x);
-        end = run_begin(total, active, blockIdx.x + 1);
-    } else {                                     // a whole sequence, head and tile for each CTA
-        const int per_sequence = p.cache.kv_heads * p.row_tiles;
-        b = blockIdx.x / per_sequence;
-        const Sequence s = sequence_of(p, b, kTileRows);
-        const int unit = blockIdx.x % per_sequence;
-        if (unit >= p.cache.kv_heads * s.row_tiles) return;
-        base = 0;
-        position = static_cast<long long>(unit) * s.blocks;
-        end = position + s.blocks;
+    const Runs runs(p, total);
+    if (static_cast<int>(blockIdx.x) >= runs.active) return;
+    Place at{0, 0, runs.begin(blockIdx.x)};
+    if (p.cache.batch > 1) {
+        at.b = plan[1];
+        at.base = plan[2];
     }
-    unsigned fill = 0, take = 0;                 // blocks that this team's ring was asked for, and that it has used
+    const int end = runs.begin(blockIdx.x + 1);
+
     bool healthy = true;
-    bool first_segment = true;
-    while (position < end) {
-        Sequence s = sequence_of(p, b, kTileRows);
-        while (b + 1 < p.cache.batch && position >= base + work_of(p, s)) {
-            base += work_of(p, s);
-            ++b;
-            s = sequence_of(p, b, kTileRows);
+    Feed& feed = feeds[team];
+    // Asks for what the team needs next, if there is anything left: by the feeder, into the slot that has just become free.
+    auto ask = [&]() {
+        while (feed.left == 0) {
+            Segment seg;
+            if (!next_segment(p, end, feed.at, seg)) return;
+            const size_t from = ((static_cast<size_t>(seg.b) * p.cache.kv_heads + seg.head) * p.cache.blocks + seg.begin + team) * Shape::kSlotBytes;
+            feed.left = 2 * max(0, (seg.stop - seg.begin - team + kTeams - 1) / kTeams);
+            feed.keys = p.cache.k_codes + from;
+            feed.values = p.cache.v_codes + from;
         }
-        const long long local = position - base;
-        const int unit = static_cast<int>(local / s.blocks), begin = static_cast<int>(local % s.blocks);
-        const int stop = static_cast<int>(min(static_cast<long long>(s.blocks), begin + (end - position)));
-        const int head = unit / s.row_tiles, tile = unit % s.row_tiles;
-        const int full = min(stop, s.length / kKvBlock);                     // blocks [begin, full) are codes, [full, stop) the tail
-        const size_t pair = static_cast<size_t>(b) * p.cache.kv_heads + head;
-        const uint8_t* k_codes = p.cache.k_codes + pair * p.cache.blocks * Shape::kBlockBytes;
-        const uint8_t* v_codes = p.cache.v_codes + pair * p.cache.blocks * Shape::kBlockBytes;
+        const unsigned slot = feed.fill % kSlots;
+        if (MT > 1 && feed.fill >= kSlots &&
+            !mbar_wait(smem_u32(&bars[team][slot][1]), (feed.fill / kSlots - 1) & 1, kKvGaveUp, p.cache.status)) {
+            healthy = false;
+            return;
+        }
+        const uint8_t*& next = feed.left & 1 ? feed.values : feed.keys;
+        const unsigned full_bar = smem_u32(&bars[team][slot][0]);
+        mbar_arrive_expect_tx(full_bar, Shape::kSlotBytes);
+        bulk_load(smem_u32(ring + slot * Shape::kSlotBytes), next, Shape::kSlotBytes, full_bar);
+        next += kTeams * Shape::kSlotBytes;
+        --feed.left;
+        ++feed.fill;
+    };
+    if (feeder) {
+        feed.at = at;
+        feed.left = 0;
+        feed.fill = 0;
+        for (int i = 0; i < kSlots; ++i) ask();
+    }
+    unsigned take = 0;                           // slots that this warp has used
+    // A slot, once it has been filled; null if that did not happen.
+    auto arrived = [&](unsigned number) -> const uint8_t* {
+        const unsigned slot = number % kSlots;
+        healthy = mbar_wait(smem_u32(&bars[team][slot][0]), (number / kSlots) & 1, kKvGaveUp, p.cache.status) && healthy;
+        healthy = __all_sync(0xffffffffu, healthy);
+        return healthy ? ring + slot * Shape::kSlotBytes : nullptr;
+    };
+    auto release = [&]() {
+        // (the slot was read through the generic proxy and is refilled through the async one: each lane orders its own reads)
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            if (MT > 1) mbar_arrive(smem_u32(&bars[team][take % kSlots][1]));
+            if (member == 0) ask();
+        }
+        ++take;
+    };
+    bool first_segment = true;
+    Segment seg;
+    while (next_segment(p, end, at, seg)) {
+        const int first_block = seg.begin + team;
+        const size_t pair = static_cast<size_t>(seg.b) * p.cache.kv_heads + seg.head;
         const float* k_scales = p.cache.k_scales + pair * p.cache.blocks;
         const float* v_scales = p.cache.v_scales + pair * p.cache.blocks;
-
-        auto request = [&](int block) {           // by one thread of the team
-            const unsigned slot = fill % kStages;
-            const unsigned full_bar = smem_u32(&bars[team][slot][0]);
-            if (fill >= kStages && !mbar_wait(smem_u32(&bars[team][slot][1]), (fill / kStages - 1) & 1, kKvGaveUp, p.cache.status)) {
-                healthy = false;
-            }
-            if (healthy) {
-                const unsigned to = smem_u32(ring + slot * 2 * Shape::kBlockBytes);
-                mbar_arrive_expect_tx(full_bar, 2 * Shape::kBlockBytes);
-                bulk_load(to, k_codes + static_cast<size_t>(block) * Shape::kBlockBytes, Shape::kBlockBytes, full_bar);
-                bulk_load(to + Shape::kBlockBytes, v_codes + static_cast<size_t>(block) * Shape::kBlockBytes, Shape::kBlockBytes, full_bar);
-            }
+        const int coded = max(0, (seg.stop - first_block + kTeams - 1) / kTeams);
+        float k_scale_set, v_scale_set;            // lane l: of this team's block number l since the last set
+        auto load_scales = [&](int block) {
+            const int mine = block + lane * kTeams;
+            k_scale_set = mine < seg.stop ? k_scales[mine] : 0.0f;
+            v_scale_set = mine < seg.stop ? v_scales[mine] : 0.0f;
         };
-        const int first_block = begin + team;
-        int asked = first_block;                  // next block to request
-        for (int i = 0; i < kStages && asked < full; ++i, asked += kTeams) {
-            if (lane == 0 && member == 0) request(asked);
-            ++fill;
-        }
+        load_scales(first_block);
 
-        // queries as the first operand: rows g and g + 8 of this warp's tile, dims in the order of the codes' bytes
-        const int row_lo = tile * kTileRows + member * 16 + g, row_hi = row_lo + 8;
-        const int rows = s.count * p.group;
-        uint32_t q[kSteps][4];
-        float q_scale[2] = {p.scale, p.scale};
-        int place[2];                              // position of the row's query; -1: no such row
-        {
-            uint32_t raw[2][D / 8];                // [row][64-dim run * 8 + word]: sixteen dims of each run
-            float top[2] = {0.0f, 0.0f};
+        // queries as the second operand: row g of each of this warp's 8-row tiles, dims in the order of the codes' bytes
+        const int rows = seg.count * p.group;
+        const int first_row = seg.tile * kTileRows + member * 8 * NT;
+        uint32_t q[NT][kSteps][2];
+        float q_scale[NT][2];                      // of rows 2c and 2c + 1
+        int place[NT][2];                          // their queries' positions
+        int lowest = INT_MAX;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = r == 0 ? row_lo : row_hi;
-                place[r] = row < rows ? s.length - s.count + row / p.group : -1;
-                const T* from = reinterpret_cast<const T*>(p.q) + b * p.q_batch + (row / p.group) * p.q_token +
-                                (head * p.group + row % p.group) * p.q_head;
+        for (int n = 0; n < NT; ++n) {
+            const int row = first_row + n * 8 + g;
+            const bool there = row < rows;
+            const T* from = reinterpret_cast<const T*>(p.q) + seg.b * p.q_batch + (row / p.group) * p.q_token +
+                            (seg.head * p.group + row % p.group) * p.q_head + c * 16;
+            uint32_t raw[D / 8];                   // sixteen dims of each run of 64
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-#pragma unroll
-                    for (int w = 0; w < 8; w += 4) {
-                        uint4 four = make_uint4(0u, 0u, 0u, 0u);
-                        if (row < rows && p.q_wide) {
-                            four = *reinterpret_cast<const uint4*>(from + j * 64 + c * 16 + w * 2);
-                        } else if (row < rows) {
-                            const uint16_t* h = reinterpret_cast<const uint16_t*>(from + j * 64 + c * 16 + w * 2);
-                            four = make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
-                                              h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
-                        }
-                        raw[r][j * 8 + w] = four.x;
-                        raw[r][j * 8 + w + 1] = four.y;
-                        raw[r][j * 8 + w + 2] = four.z;
-                        raw[r][j * 8 + w + 3] = four.w;
-                    }
-#pragma unroll
-                    for (int w = 0; w < 8; ++w) {
-                        const float2 f = widen2<T>(raw[r][j * 8 + w]);
-                        top[r] = fmaxf(top[r], fmaxf(finite_magnitude(f.x), finite_magnitude(f.y)));
-                    }
+            for (int i = 0; i < D / 8; i += 4) {
+                const T* at = from + i / 8 * 64 + i % 8 * 2;
+                uint4 four = make_uint4(0u, 0u, 0u, 0u);
+                if (there && p.q_wide) {
+                    four = *reinterpret_cast<const uint4*>(at);
+                } else if (there) {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(at);
+                    four = make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
+                                      h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
                 }
-                // BF16 queries become FP16 by a power of two of their row's own: every number that is not 2^-24 below the
-                // row's largest keeps all its bits.  FP16 ones are taken as they are.
-                float by = 1.0f;
-                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    float back;
-                    by = power_for(top[r], back);
-                    q_scale[r] *= back;
+                raw[i] = four.x;
+                raw[i + 1] = four.y;
+                raw[i + 2] = four.z;
+                raw[i + 3] = four.w;
+            }
+            float back = 1.0f;
+            if constexpr (kBf16) {
+                // BF16 queries become FP16 by a power of two of their row's own: a number keeps all its bits unless it is 2^-23
+                // of the row's largest or less.  FP16 ones are taken as they are.
+                float largest = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float2 f = widen2<T>(raw[i]);
+                    largest = fmaxf(largest, fmaxf(finite_magnitude(f.x), finite_magnitude(f.y)));
                 }
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                const float by = power_for(largest, back);
 #pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const float2 lo = widen2<T>(raw[r][j * 8 + 2 * w]), hi = widen2<T>(raw[r][j * 8 + 2 * w + 1]);
-                        q[j * 4 + w][r] = pack_half(lo.x * by, hi.x * by);
-                        q[j * 4 + w][2 + r] = pack_half(lo.y * by, hi.y * by);
-                    }
+                for (int i = 0; i < D / 8; ++i) {
+                    const float2 f = widen2<T>(raw[i]);
+                    raw[i] = pack_half(f.x * by, f.y * by);
                 }
             }
-        }
-        float acc[kTiles][4];
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-        float top[2] = {kNone, kNone}, sum[2] = {0.0f, 0.0f};      // the sum of this lane's columns
-        float unit_scale = 1.0e-30f;                              // of the accumulator: values are acc * unit_scale / kHeadroom
-
-        // Scores of a block in place of which come the probabilities, as operands of the second product; tokens of lane c:
-        // 16 * group + 4 c + 2 e + parity.
-        auto probabilities = [&](float (&score)[4][4], int block, float k_scale, float v_scale, uint32_t (&prob)[2][4]) {
-            const float by[2] = {k_scale * q_scale[0], k_scale * q_scale[1]};
-            const int token = block * kKvBlock;
-            float next[2] = {kNone, kNone};
+            for (int i = 0; i < kSteps; ++i) {
+                q[n][i][0] = prmt(raw[2 * i], raw[2 * i + 1], 0x5410);
+                q[n][i][1] = prmt(raw[2 * i], raw[2 * i + 1], 0x7632);
+            }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const bool all = token + kKvBlock - 1 <= place[r];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = score[t][2 * r + e];
-                        x = all || token + (t >> 1) * 16 + 4 * c + 2 * e + (t & 1) <= place[r] ? x * by[r] : -INFINITY;
-                        next[r] = fmaxf(next[r], x);
-                    }
-                }
-                next[r] = fmaxf(next[r], __shfl_xor_sync(0xffffffffu, next[r], 1));
-                next[r] = fmaxf(next[r], __shfl_xor_sync(0xffffffffu, next[r], 2));
+                q_scale[n][r] = p.scale * __shfl_sync(0xffffffffu, back, (2 * c + r) * 4);
+                const int of = first_row + n * 8 + 2 * c + r;
+                place[n][r] = of < rows ? seg.length - seg.count + of / p.group : INT_MAX;      // (rows that are not there: anything goes)
+                lowest = min(lowest, place[n][r]);
             }
-            const bool new_unit = v_scale > kMaxRatio * unit_scale;
-            const bool lag = next[0] > top[0] + kMaxLag || next[1] > top[1] + kMaxLag;
-            if (new_unit || __any_sync(0xffffffffu, lag)) {
-                float shrink[2];
-                const float unit_change = new_unit ? unit_scale / v_scale : 1.0f;
-                if (new_unit) unit_scale = v_scale;
+        }
+        lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 1));
+        lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 2));
+
+        float acc[NT][kSteps][4];                  // dims 16 j + g and + 8, rows 2c and 2c + 1
+        float top[NT][2], sum[NT][2];              // the sum is of this lane's tokens
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.0f;
+            top[n][0] = top[n][1] = kNone;
+            sum[n][0] = sum[n][1] = 0.0f;
+        }
+        float unit_scale = 1.0e-30f;               // of the accumulators: values are acc * unit_scale / kHeadroom
+        float per_scale = kHeadroom / 1.0e-30f;    // kHeadroom / unit_scale
+
+        // Scores of a block, [group of 16 tokens][token 2g: rows 2c, 2c + 1; token 2g + 1: the same], and the probabilities that come
+        // of them, as operands of the second product: row g, tokens 4c, 4c + 2 and 4c + 1, 4c + 3 of each group.
+        uint32_t prob[NT][2][2];
+        auto probabilities = [&](float (&score)[NT][2][4], int block, float k_scale, float v_scale) {
+            const bool masked = (block + 1) * kKvBlock - 1 > lowest;
+            bool lag = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float now = fmaxf(top[r], next[r]);
-                    shrink[r] = exp2_fast(top[r] - now);
-                    top[r] = now;
-                    sum[r] *= shrink[r];
-                    shrink[r] *= unit_change;
-                }
+                    const float by = k_scale * q_scale[n][r];
 #pragma unroll
-                for (int j = 0; j < kTiles; ++j) {
-                    acc[j][0] *= shrink[0];
-                    acc[j][1] *= shrink[0];
-                    acc[j][2] *= shrink[1];
-                    acc[j][3] *= shrink[1];
+                    for (int t = 0; t < 4; ++t) {
+                        float& x = score[n][t >> 1][(t & 1) * 2 + r];
+                        x *= by;
+                        if (masked && block * kKvBlock + (t >> 1) * 16 + 2 * g + (t & 1) > place[n][r]) x = -INFINITY;
+                        lag = lag || x > top[n][r] + kMaxLag;
+                    }
                 }
             }
-            const float weight = v_scale / unit_scale * kHeadroom;
+            const bool new_unit = v_scale > kMaxRatio * unit_scale;
+            if (__any_sync(0xffffffffu, lag || new_unit)) {
+                const float unit_change = new_unit ? unit_scale / v_scale : 1.0f;
+                if (new_unit) {
+                    unit_scale = v_scale;
+                    per_scale = kHeadroom / v_scale;
+                }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+                for (int n = 0; n < NT; ++n) {
+                    float shrink[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float now = fmaxf(fmaxf(score[n][0][r], score[n][0][2 + r]), fmaxf(score[n][1][r], score[n][1][2 + r]));
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+                        now = fmaxf(now, top[n][r]);
+                        shrink[r] = exp2_fast(top[n][r] - now);
+                        top[n][r] = now;
+                        sum[n][r] *= shrink[r];
+                        shrink[r] *= unit_change;
+                    }
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j) {
+                        acc[n][j][0] *= shrink[0];
+                        acc[n][j][1] *= shrink[1];
+                        acc[n][j][2] *= shrink[0];
+                        acc[n][j][3] *= shrink[1];
+                    }
+                }
+            }
+            const float weight = v_scale * per_scale;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     float w[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float x = score[t][2 * r + e];
-                        const float pr = exp2_fast(x - top[r]);
-                        sum[r] += pr;
-                        w[e] = x == -INFINITY ? 0.0f : pr * weight;      // (a masked token's scale may be NaN)
+                    for (int r = 0; r < 2; ++r) {
+                        const float x = score[n][t >> 1][(t & 1) * 2 + r];
+                        const float e = exp2_fast(x - top[n][r]);
+                        sum[n][r] += e;
+                        w[r] = e * weight;
+                        if (masked && x == -INFINITY) w[r] = 0.0f;           // (the block's scale may be NaN)
                     }
-                    prob[t >> 1][(t & 1) * 2 + r] = pack_half(w[0], w[1]);
+                    prob[n][t >> 1][t & 1] = transpose8x8(pack_half(w[0], w[1]));
                 }
             }
         };
 
-        float k_scale_set = 0.0f, v_scale_set = 0.0f;              // lane l: of this team's block number l since the last set
-        int count = 0;
-        for (int block = first_block; block < full; block += kTeams, ++count) {
-            if ((count & 31) == 0) {
-                const int mine = block + lane * kTeams;
-                k_scale_set = mine < full ? k_scales[mine] : 0.0f;
-                v_scale_set = mine < full ? v_scales[mine] : 0.0f;
-            }
-            const float k_scale = __shfl_sync(0xffffffffu, k_scale_set, count & 31);
-            const float v_scale = __shfl_sync(0xffffffffu, v_scale_set, count & 31);
-            const unsigned slot = take % kStages;
-            healthy = mbar_wait(smem_u32(&bars[team][slot][0]), (take / kStages) & 1, kKvGaveUp, p.cache.status) && healthy;
-            healthy = __all_sync(0xffffffffu, healthy);
-            if (!healthy) break;
-            const uint8_t* keys = ring + slot * 2 * Shape::kBlockBytes;
-            const uint8_t* values = keys + Shape::kBlockBytes;
-            float score[4][4];
+        for (int i = 0; i < coded; ++i) {
+            const int block = first_block + i * kTeams;
+            if ((i & 31) == 0 && i > 0) load_scales(block);
+            const uint8_t* keys = arrived(take);
+            if (keys == nullptr) break;
+            float score[NT][2][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.0f;
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) score[n][0][t] = score[n][1][t] = 0.0f;
+            }
 #pragma unroll
             for (int j = 0; j < D / 64; ++j) {
-                uint32_t words[4][4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const uint4 codes = *reinterpret_cast<const uint4*>(keys + (t * (D / 64) + j) * 512 + lane * 16);
-                    words[t][0] = codes.x; words[t][1] = codes.y; words[t][2] = codes.z; words[t][3] = codes.w;
-                }
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        uint32_t even, odd;
-                        codes_to_half(words[t][w], even, odd);
-                        mma16816(score[t], q[j * 4 + w], even, odd);
-                    }
-                }
-            }
-            uint32_t prob[2][4];
-            probabilities(score, block, k_scale, v_scale, prob);
-#pragma unroll
-            for (int j = 0; j < kTiles / 2; ++j) {
-                const uint4 codes = *reinterpret_cast<const uint4*>(values + j * 512 + lane * 16);
-                const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {                       // words: [half of the sixteen dims][token group]
-                    uint32_t even, odd;
-                    codes_to_half(words[w], even, odd);
-                    mma16816(acc[2 * j + w / 2], prob[w % 2], even, odd);
-                }
-            }
-            // (the slot was read through the generic proxy and is refilled through the async one: each lane orders its own reads)
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars[team][slot][1]));
-            ++take;
-            if (asked < full) {
-                if (lane == 0 && member == 0) request(asked);
-                ++fill;
-                asked += kTeams;
-            }
-        }
-
-        // the block that is being filled, by the team whose turn it is
-        if (stop > full && healthy && (full - begin) % kTeams == team) {
-            const int token = full * kKvBlock;
-            const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + (pair * 2 + (full & 1)) * kKvBlock * D;
-            const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (full & 1)) * kKvBlock * D;
-            const int held = s.length - token;
-            // both in FP16 by one power of two each, which takes the scales' place
-            float k_top = 0.0f, v_top = 0.0f;
-            bool odd_values = false;                               // an infinity or NaN among the values
-            for (int i = lane * 2; i < held * D; i += 64) {
-                const float2 kf = widen2<T>(*reinterpret_cast<const uint32_t*>(k_tail + i));
-                const float2 vf = widen2<T>(*reinterpret_cast<const uint32_t*>(v_tail + i));
-                k_top = fmaxf(k_top, fmaxf(finite_magnitude(kf.x), finite_magnitude(kf.y)));
-                v_top = fmaxf(v_top, fmaxf(finite_magnitude(vf.x), finite_magnitude(vf.y)));
-                odd_values = odd_values || !(fabsf(vf.x) <= 3.4028235e38f) || !(fabsf(vf.y) <= 3.4028235e38f);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                k_top = fmaxf(k_top, __shfl_xor_sync(0xffffffffu, k_top, o));
-                v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
-            }
-            odd_values = __any_sync(0xffffffffu, odd_values);
-            float k_back, v_back;
-            const float k_by = power_for(k_top, k_back), v_by = power_for(v_top, v_back);
-            float score[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.0f;
-                const int at = (t >> 1) * 16 + 2 * g + (t & 1);
-#pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        float2 lo = make_float2(0.0f, 0.0f), hi = lo;
-                        if (at < held) {
-                            const uint2 two = *reinterpret_cast<const uint2*>(k_tail + at * D + j * 64 + c * 16 + w * 4);
-                            lo = widen2<T>(two.x);
-                            hi = widen2<T>(two.y);
-                        }
-                        mma16816(score[t], q[j * 4 + w], pack_half(lo.x * k_by, hi.x * k_by), pack_half(lo.y * k_by, hi.y * k_by));
-                    }
-                }
-            }
-            uint32_t prob[2][4];
-            probabilities(score, full, k_back, v_back, prob);
-#pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    float v[4];
+                    const uint4 even_token = *reinterpret_cast<const uint4*>(keys + ((half * 2) * (D / 64) + j) * 512 + lane * 16);
+                    const uint4 odd_token = *reinterpret_cast<const uint4*>(keys + ((half * 2 + 1) * (D / 64) + j) * 512 + lane * 16);
+                    const uint32_t even_words[4] = {even_token.x, even_token.y, even_token.z, even_token.w};
+                    const uint32_t odd_words[4] = {odd_token.x, odd_token.y, odd_token.z, odd_token.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = half * 16 + 4 * c + e;
-                        v[e] = at < held ? widen<T>(v_tail[at * D + j * 8 + g]) : 0.0f;
-                        // (a probability of zero times an infinity would be NaN in rows that do not see the token: added below)
-                        v[e] = fabsf(v[e]) <= 3.4028235e38f ? v[e] * v_by : 0.0f;
-                    }
-                    mma16816(acc[j], prob[half], pack_half(v[0], v[2]), pack_half(v[1], v[3]));
-                }
-            }
-            if (odd_values) {
-                for (int t = 0; t < held; ++t) {
-                    for (int j = 0; j < kTiles; ++j) {
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t a[4];
+                        codes_to_half(even_words[w], a[0], a[2]);
+                        codes_to_half(odd_words[w], a[1], a[3]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v = widen<T>(v_tail[t * D + j * 8 + c * 2 + (e & 1)]);
-                            if (!(fabsf(v) <= 3.4028235e38f) && token + t <= place[e >> 1]) acc[j][e] += v;
-                        }
+                        for (int n = 0; n < NT; ++n) mma16816(score[n][half], a, q[n][j * 4 + w][0], q[n][j * 4 + w][1]);
                     }
                 }
             }
+            release();
+            probabilities(score, block, __shfl_sync(0xffffffffu, k_scale_set, i & 31), __shfl_sync(0xffffffffu, v_scale_set, i & 31));
+            const uint8_t* values = arrived(take);
+            if (values == nullptr) break;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const uint4 codes = *reinterpret_cast<const uint4*>(values + j * 512 + lane * 16);
+                const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};     // [half of the sixteen dims][token group]
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t a[4];
+                    codes_to_half(words[half], a[0], a[2]);
+                    codes_to_half(words[2 + half], a[1], a[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma16816(acc[n][j], a, prob[n][half][0], prob[n][half][1]);
+                }
+            }
+            release();
         }
+
         if (!healthy) break;
 
-        // rows of this run: sums of a row's four lanes, then the teams'
+        // rows of this segment: a row's sums, then the teams' results
         const float to_value = unit_scale / kHeadroom;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-        }
-        const bool whole = begin == 0 && stop == s.blocks;
-        float* part = whole ? nullptr : part_of(p, blockIdx.x, first_segment, kTileRows, D);
-        const int tile_rows = min(kTileRows, rows - tile * kTileRows);
-        auto row_out = [&](int row) {              // of the tile
-            const int at = tile * kTileRows + row;
-            return reinterpret_cast<T*>(p.out) +
-                   ((static_cast<size_t>(b) * p.tokens + at / p.group) * p.q_heads + head * p.group + at % p.group) * D;
-        };
-        if constexpr (kTeams == 1) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int row = member * 16 + g + 8 * r;
-                if (row >= tile_rows) continue;
-                if (whole) {
-                    const float by = sum[r] > 0.0f ? to_value / sum[r] : sum[r] == 0.0f ? 0.0f : sum[r];
-                    uint32_t* to = reinterpret_cast<uint32_t*>(row_out(row));
 #pragma unroll
-                    for (int j = 0; j < kTiles; ++j) to[j * 4 + c] = narrow2<T>(acc[j][2 * r] * by, acc[j][2 * r + 1] * by);
-                } else {
-                    float* to = part + row * (D + 2);
-#pragma unroll
-                    for (int j = 0; j < kTiles; ++j) {
-                        *reinterpret_cast<float2*>(to + j * 8 + c * 2) = make_float2(acc[j][2 * r] * to_value, acc[j][2 * r + 1] * to_value);
-                    }
-                    if (c == 0) *reinterpret_cast<float2*>(to + D) = make_float2(top[r], sum[r]);
-                }
-            }
-        } else {
-            __syncthreads();                        // an earlier segment's rows have been read
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = member * 16 + g + 8 * r;
-                if (row >= tile_rows) continue;
-                float* to = merge + (team * kTileRows + row) * (D + 2);
-#pragma unroll
-                for (int j = 0; j < kTiles; ++j) {
-                    *reinterpret_cast<float2*>(to + j * 8 + c * 2) = make_float2(acc[j][2 * r] * to_value, acc[j][2 * r + 1] * to_value);
-                }
-                if (c == 0) *reinterpret_cast<float2*>(to + D) = make_float2(top[r], sum[r]);
-            }
-            __syncthreads();
-            for (int at = tid; at < tile_rows * (D / 2); at += kThreads) {
-                const int row = at / (D / 2), d = at % (D / 2) * 2;
-                const float* from = merge + row * (D + 2);
-                float best = kNone;
-#pragma unroll
-                for (int t = 0; t < kTeams; ++t) best = fmaxf(best, from[t * kTileRows * (D + 2) + D]);
-                float all = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll
-                for (int t = 0; t < kTeams; ++t) {
-                    const float* of = from + t * kTileRows * (D + 2);
-                    const float w = exp2_fast(of[D] - best);
-                    const float2 v = *reinterpret_cast<const float2*>(of + d);
-                    all += w * of[D + 1];
-                    x += w * v.x;
-                    y += w * v.y;
-                }
-                if (whole) {
-                    const float by = all > 0.0f ? 1.0f / all : all;
-                    *reinterpret_cast<uint32_t*>(row_out(row) + d) = narrow2<T>(x * by, y * by);
-                } else {
-                    float* to = part + row * (D + 2);
-                    *reinterpret_cast<float2*>(to + d) = make_float2(x, y);
-                    if (d == 0) *reinterpret_cast<float2*>(to + D) = make_float2(best, all);
-                }
+                for (int o = 4; o < 32; o <<= 1) sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], o);
             }
         }
-        position += stop - begin;
+        if (!first_segment) __syncthreads();        // the segment before has been read
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float* to = merge + (team * kTileRows + member * 8 * NT + n * 8 + 2 * c + r) * (D + 2);
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) {
+                    to[j * 16 + g] = acc[n][j][r] * to_value;
+                    to[j * 16 + 8 + g] = acc[n][j][2 + r] * to_value;
+                }
+                if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(top[n][r], sum[n][r]);
+            }
+        }
+        __syncthreads();
+        float* part = part_of(p, seg.b, seg.head, seg.tile, blockIdx.x, D);
+        const int tile_rows = min(kTileRows, rows - seg.tile * kTileRows);
+        for (int at = tid; at < tile_rows * (D / 2); at += kThreads) {
+            const int row = at / (D / 2), d = at % (D / 2) * 2;
+            const float* from = merge + row * (D + 2);
+            float best = kNone;
+#pragma unroll
+            for (int t = 0; t < kTeams; ++t) best = fmaxf(best, from[t * kTileRows * (D + 2) + D]);
+            float all = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int t = 0; t < kTeams; ++t) {
+                const float* of = from + t * kTileRows * (D + 2);
+                const float w = exp2_fast(of[D] - best);
+                const float2 v = *reinterpret_cast<const float2*>(of + d);
+                all += w * of[D + 1];
+                x += w * v.x;
+                y += w * v.y;
+            }
+            float* to = part + row * (D + 2);
+            *reinterpret_cast<float2*>(to + d) = make_float2(x, y);
+            if (d == 0) *reinterpret_cast<float2*>(to + D) = make_float2(best, all);
+        }
         first_segment = false;
     }
-    if (!healthy) {                                 // wait, within limits, for copies that are still on their way
-        if (lane == 0 && member == 0) {
-            for (unsigned s = take; s < fill; ++s) mbar_wait(smem_u32(&bars[team][s % kStages][0]), (s / kStages) & 1, kKvGaveUp, p.cache.status);
+    if (!healthy && feeder) {                       // wait, within limits, for copies that are still on their way
+        for (unsigned s = take; s < feed.fill; ++s) {
+            mbar_wait(smem_u32(&bars[team][s % kSlots][0]), (s / kSlots) & 1, kKvGaveUp, p.cache.status);
         }
     }
 }
 
-// Adds up the parts of the sequences and heads that several runs share; one CTA for each row of each tile.
-template <typename T, int D>
+// Rows of the output: the parts that the runs have of each, in order, and the block that is being filled, whose 16-bit numbers are
+// multiplied in FP32 as they are.  A CTA has `rows` rows of one sequence and key/value head, ROW_WARPS warps for each at a time.  What
+// needs no part is done before the kernel in front has ended; that one lets this one start only when all before it has.
+template <typename T, int D, int ROW_WARPS>
 __global__ void __launch_bounds__(kThreads)
-kv_combine_kernel(const AttentionParams p, int tile_rows) {
-    __shared__ float sums[kWarps][D], tops[kWarps], weights[kWarps];
-    __shared__ long long plan[2];                    // all blocks; blocks before this sequence
+kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
+    constexpr int kRows = kWarps / ROW_WARPS;            // at a time
+    constexpr int kDims = D / 32;                        // of a lane
+    constexpr int kStride = D + 8;                       // of a token's numbers in shared memory
+    __shared__ __align__(16) T keys[kKvBlock * kStride];
+    __shared__ __align__(16) T values[kKvBlock * D];
+    __shared__ __align__(16) float queries[kRows][D];
+    __shared__ float sums[kWarps][D];
+    __shared__ int plan[2];                              // all work; work before this sequence
+    if (p.grid == 0) pdl_wait_for_upstream();            // there is no kernel of ours in front
     pdl_release_downstream();
-    pdl_wait_for_upstream();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rows_at_most = p.tokens * p.group;
-    const int row = blockIdx.x % rows_at_most;
-    const int pair = blockIdx.x / rows_at_most, b = pair / p.cache.kv_heads, head = pair % p.cache.kv_heads;
-    const Sequence s = sequence_of(p, b, tile_rows);
-    if (row >= s.count * p.group || s.blocks == 0) return;
+    const int row_ctas = (p.tokens * p.group + rows_per_cta - 1) / rows_per_cta;
+    const int pair = blockIdx.x / row_ctas, b = pair / p.cache.kv_heads, head = pair % p.cache.kv_heads;
+    const int first_row = blockIdx.x % row_ctas * rows_per_cta;
+    const int last_row = min(first_row + rows_per_cta, p.tokens * p.group);
+    const Sequence s = sequence_of(p, b);
+    const int held = s.length - s.blocks * kKvBlock;
+    {
+        const size_t from = (static_cast<size_t>(pair) * 2 + (s.blocks & 1)) * kKvBlock * D * sizeof(T);
+        const uint4* k_tail = reinterpret_cast<const uint4*>(p.cache.k_tail + from);
+        const uint4* v_tail = reinterpret_cast<const uint4*>(p.cache.v_tail + from);
+#pragma unroll 4
+        for (int i = tid; i < held * D / 8; i += kThreads) {
+            *reinterpret_cast<uint4*>(keys + i / (D / 8) * kStride + i % (D / 8) * 8) = k_tail[i];
+            reinterpret_cast<uint4*>(values)[i] = v_tail[i];
+        }
+    }
     if (warp == 0) {
-        long long total = 0, before = 0;
+        int total = 0, before = 0;
         for (int i = lane; i < p.cache.batch; i += 32) {
-            const long long work = work_of(p, sequence_of(p, i, tile_rows));
+            const int work = work_of(p, i == b ? s : sequence_of(p, i));
             total += work;
             if (i < b) before += work;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            total += __shfl_xor_sync(0xffffffffu, total, o);
-            before += __shfl_xor_sync(0xffffffffu, before, o);
-        }
+        total = __reduce_add_sync(0xffffffffu, total);
+        before = __reduce_add_sync(0xffffffffu, before);
         if (lane == 0) {
             plan[0] = total;
             plan[1] = before;
+            if (!s.sound) atomicOr(p.cache.status, kKvBadLength);
         }
     }
-    __syncthreads();
-    const long long total = plan[0];
-    const int active = active_ctas(p, total);
-    const int tile = row / tile_rows;
-    const long long begin = plan[1] + (static_cast<long long>(head) * s.row_tiles + tile) * s.blocks, end = begin + s.blocks;
-    // the runs that hold its first and its last block: the last whose begin is not behind it
-    auto run_of = [&](long long block) {
-        int at = static_cast<int>(block * active / total);
-        while (at + 1 < active && run_begin(total, active, at + 1) <= block) ++at;
-        while (at > 0 && run_begin(total, active, at) > block) --at;
-        return at;
-    };
-    const int first = run_of(begin), last = run_of(end - 1);
-    if (first == last) return;                       // one run has it all, and has written the result
-    const int in_tile = row % tile_rows;
-    float best = kNone, weight = 0.0f, acc[D / 32];
+    bool waited = false;
+    for (int base = first_row; base < last_row; base += kRows) {
+        const int row = base + warp / ROW_WARPS, i = row / p.group, q_head = head * p.group + row % p.group;
+        const int share = warp % ROW_WARPS;
+        const bool there = row < last_row && i < s.count;
+        const int position = s.length - s.count + i;
+        if (there && share == 0) {
+            const T* from = reinterpret_cast<const T*>(p.q) + b * p.q_batch + i * p.q_token + q_head * p.q_head;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
-    auto part = [&](int run) {
-        return part_of(p, run, run_begin(total, active, run) >= begin, tile_rows, D) + in_tile * (D + 2);
-    };
-    for (int run = first + warp; run <= last; run += kWarps) best = fmaxf(best, part(run)[D]);
+            for (int e = 0; e < kDims; ++e) queries[warp / ROW_WARPS][e * 32 + lane] = widen<T>(from[e * 32 + lane]);
+        }
+        __syncthreads();
+        // the tail: lane t has token t's score, then each lane its dims
+        float top = kNone, weight = 0.0f, acc[kDims];
+#pragma unroll
+        for (int e = 0; e < kDims; ++e) acc[e] = 0.0f;
+        const int seen = there ? min(held, position - s.blocks * kKvBlock + 1) : 0;
+        if (share == 0 && seen > 0) {
+            float score = -INFINITY;
+            if (lane < seen) {
+                const float4* q = reinterpret_cast<const float4*>(queries[warp / ROW_WARPS]);
+                const uint4* k = reinterpret_cast<const uint4*>(keys + lane * kStride);
+                float dot[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < D / 8; ++e) {
+                    const uint4 eight = k[e];
+                    const float4 q0 = q[2 * e], q1 = q[2 * e + 1];
+                    const float2 k0 = widen2<T>(eight.x), k1 = widen2<T>(eight.y), k2 = widen2<T>(eight.z), k3 = widen2<T>(eight.w);
+                    dot[0] = fmaf(q0.x, k0.x, fmaf(q0.y, k0.y, fmaf(q0.z, k1.x, fmaf(q0.w, k1.y, dot[0]))));
+                    dot[1] = fmaf(q1.x, k2.x, fmaf(q1.y, k2.y, fmaf(q1.z, k3.x, fmaf(q1.w, k3.y, dot[1]))));
+                }
+                score = (dot[0] + dot[1]) * p.scale;
+                top = fmaxf(top, score);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float mine = lane < seen ? exp2_fast(score - top) : 0.0f;
+            weight = mine;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, o);
 #pragma unroll 4
-    for (int run = first + warp; run <= last; run += kWarps) {
-        const float* from = part(run);
-        const float w = exp2_fast(from[D] - best);
-        weight += w * from[D + 1];
+            for (int t = 0; t < seen; ++t) {
+                const float w = __shfl_sync(0xffffffffu, mine, t);
+                const T* v = values + t * D + lane * kDims;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] += w * from[i * 32 + lane];
-    }
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) sums[warp][i * 32 + lane] = acc[i];
-    if (lane == 0) {
-        tops[warp] = best;
-        weights[warp] = weight;
-    }
-    __syncthreads();
-    if (tid < D) {
-        float all = 0.0f, x = 0.0f;
-        best = kNone;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) best = fmaxf(best, tops[w]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float by = exp2_fast(tops[w] - best);
-            all += by * weights[w];
-            x += by * sums[w][tid];
+                for (int e = 0; e < kDims; e += 2) {
+                    const float2 two = widen2<T>(*reinterpret_cast<const uint32_t*>(v + e));
+                    acc[e] = fmaf(w, two.x, acc[e]);
+                    acc[e + 1] = fmaf(w, two.y, acc[e + 1]);
+                }
+            }
         }
-        T* to = reinterpret_cast<T*>(p.out) +
-                ((static_cast<size_t>(b) * p.tokens + row / p.group) * p.q_heads + head * p.group + row % p.group) * D;
-        to[tid] = narrow<T>(all > 0.0f ? x / all : all);
+        if (!waited) pdl_wait_for_upstream();
+        waited = true;
+        if (there && s.blocks > 0) {
+            const Runs runs(p, plan[0]);
+            const int tile = row / p.tile_rows;
+            const int begin = plan[1] + (head * s.row_tiles + tile) * (s.blocks + kUnitCost) + kUnitCost;
+            const int first = runs.of(begin), count = runs.of(begin + s.blocks - 1) - first + 1;
+            const size_t stride = static_cast<size_t>(p.tile_rows) * (D + 2);
+            const float* parts = part_of(p, b, head, tile, first, D) + row % p.tile_rows * (D + 2);
+            float best = kNone;
+            for (int r = lane; r < count; r += 32) best = fmaxf(best, parts[r * stride + D]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+            if (share == 0) best = fmaxf(best, top);
+            const float shrink = exp2_fast(top - best);
+            weight *= shrink;
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) acc[e] *= shrink;
+            top = best;
+            float more = 0.0f;
+            for (int r = share + lane * ROW_WARPS; r < count; r += 32 * ROW_WARPS) {
+                more += exp2_fast(parts[r * stride + D] - best) * parts[r * stride + D + 1];
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+            weight += more;
+#pragma unroll 8
+            for (int r = share; r < count; r += ROW_WARPS) {
+                const float* from = parts + r * stride;
+                const float w = exp2_fast(from[D] - best);
+#pragma unroll
+                for (int e = 0; e < kDims; e += 2) {
+                    const float2 two = *reinterpret_cast<const float2*>(from + lane * kDims + e);
+                    acc[e] = fmaf(w, two.x, acc[e]);
+                    acc[e + 1] = fmaf(w, two.y, acc[e + 1]);
+                }
+            }
+        }
+        if (ROW_WARPS > 1) {                              // (one row: the CTA's only one at a time)
+            __shared__ float tops[kWarps], weights[kWarps];
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) sums[warp][lane * kDims + e] = acc[e];
+            if (lane == 0) {
+                tops[warp] = top;
+                weights[warp] = weight;
+            }
+            __syncthreads();
+            top = kNone;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, tops[w]);
+            weight = 0.0f;
+#pragma unroll
+            for (int e = 0; e < kDims; ++e) acc[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float by = exp2_fast(tops[w] - top);
+                weight += by * weights[w];
+#pragma unroll
+                for (int e = 0; e < kDims; ++e) acc[e] += by * sums[w][lane * kDims + e];
+            }
+        }
+        if (row < last_row && share == 0) {
+            const float by = weight > 0.0f ? 1.0f / weight : weight;       // (no weight: nothing is seen)
+            T* to = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.tokens + i) * p.q_heads + q_head) * D + lane * kDims;
+#pragma unroll
+            for (int e = 0; e < kDims; e += 2) *reinterpret_cast<uint32_t*>(to + e) = narrow2<T>(acc[e] * by, acc[e + 1] * by);
+        }
+        __syncthreads();                                  // the next rows' queries take these rows' place
     }
 }
 
@@ -706,20 +768,17 @@ struct DeviceState {
     int sms = 0;
 };
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT, int MT>
 int allow_shared() {
-    return cudaFuncSetAttribute(kv_attention_kernel<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                static_cast<int>(AttentionShape<T, D, MT>::kSharedBytes)) == cudaSuccess
+    return cudaFuncSetAttribute(kv_attention_kernel<T, D, NT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(AttentionShape<T, D, NT, MT>::kSharedBytes)) == cudaSuccess
                ? 0
                : W4A16_ERR_LAUNCH;
 }
 
-template <typename T>
+template <typename T, int D>
 int allow_all() {
-    int status = 0;
-    status |= allow_shared<T, 64, 1>() | allow_shared<T, 64, 2>() | allow_shared<T, 64, 4>();
-    status |= allow_shared<T, 128, 1>() | allow_shared<T, 128, 2>() | allow_shared<T, 128, 4>();
-    return status;
+    return allow_shared<T, D, 1, 1>() | allow_shared<T, D, 2, 1>() | allow_shared<T, D, 2, 2>() | allow_shared<T, D, 2, 4>();
 }
 
 int device_state(const DeviceState** state) {
@@ -728,45 +787,54 @@ int device_state(const DeviceState** state) {
     if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return W4A16_ERR_LAUNCH;
     return devices.get(device, [&](DeviceState& fresh) -> int {
         if (cudaDeviceGetAttribute(&fresh.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return W4A16_ERR_LAUNCH;
-        return allow_all<__half>() != 0 || allow_all<__nv_bfloat16>() != 0 ? W4A16_ERR_LAUNCH : 0;
+        const int allowed = allow_all<__half, 64>() | allow_all<__half, 128>() | allow_all<__nv_bfloat16, 64>() | allow_all<__nv_bfloat16, 128>();
+        return allowed != 0 ? W4A16_ERR_LAUNCH : 0;
     }, state);
 }
 
-// 16-row tiles of a team: as many as hold the rows, at most four.
-int tiles_for(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-
 struct Shape {
-    int mt, row_tiles;
-    int64_t units, grid;
-    bool split;
+    int tile_rows, row_tiles;      // rows of a CTA: 8, 16, 32 or 64
+    int64_t units, grid;           // sequences x heads x tiles; CTAs of the first kernel, 0 where no block can be full
+    size_t workspace;
 };
 
 Shape shape_of(const w4a16_kv8_cache& cache, int q_heads, int64_t tokens, int sms) {
     Shape s{};
     const int64_t rows = tokens * (q_heads / cache.kv_heads);
-    s.mt = tiles_for(rows);
-    s.row_tiles = static_cast<int>((rows + 16 * s.mt - 1) / (16 * s.mt));
+    s.tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    s.row_tiles = static_cast<int>((rows + s.tile_rows - 1) / s.tile_rows);
     s.units = static_cast<int64_t>(cache.batch) * cache.kv_heads * s.row_tiles;
-    const int64_t blocks = (cache.max_len + kKvBlock - 1) / kKvBlock;
-    s.split = blocks > kMinRun;
-    s.grid = s.split ? std::min<int64_t>(2 * sms, std::max<int64_t>(1, s.units * blocks / kMinRun)) : s.units;
+    const int64_t blocks = cache.max_len / kKvBlock;
+    const int resident = s.tile_rows == 8 ? 3 : 2;
+    if (blocks > 0) s.grid = std::min<int64_t>(resident * sms, std::max<int64_t>(1, s.units * (blocks + kUnitCost) / kMinRun));
+    s.workspace = static_cast<size_t>(s.units + s.grid) * s.tile_rows * (cache.head_dim + 2) * sizeof(float);
     return s;
 }
 
 template <typename T, int D>
 int launch_shape(const AttentionParams& p, const Shape& s, bool programmatic, cudaStream_t stream) {
-    auto run = [&](auto tiles) {
-        constexpr int kMt = decltype(tiles)::value;
-        return kv_launch(kv_attention_kernel<T, D, kMt>, dim3(static_cast<unsigned>(s.grid)), dim3(kThreads),
-                         AttentionShape<T, D, kMt>::kSharedBytes, programmatic, stream, p);
+    auto run = [&](auto row_tiles, auto members) {
+        constexpr int kNt = decltype(row_tiles)::value, kMt = decltype(members)::value;
+        return kv_launch(kv_attention_kernel<T, D, kNt, kMt>, dim3(static_cast<unsigned>(s.grid)), dim3(kThreads),
+                         AttentionShape<T, D, kNt, kMt>::kSharedBytes, programmatic, stream, p);
     };
-    const int status = s.mt == 1   ? run(std::integral_constant<int, 1>{})
-                       : s.mt == 2 ? run(std::integral_constant<int, 2>{})
-                                   : run(std::integral_constant<int, 4>{});
-    if (status != W4A16_OK || !s.split) return status;
-    const int64_t rows = static_cast<int64_t>(p.cache.batch) * p.cache.kv_heads * p.tokens * p.group;
-    // (always programmatic: it waits for the kernel in front itself, which is the one above)
-    return kv_launch(kv_combine_kernel<T, D>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, true, stream, p, 16 * s.mt);
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Four = std::integral_constant<int, 4>;
+    if (s.grid > 0) {
+        const int status = s.tile_rows == 8    ? run(One{}, One{})
+                           : s.tile_rows == 16 ? run(Two{}, One{})
+                           : s.tile_rows == 32 ? run(Two{}, Two{})
+                                               : run(Two{}, Four{});
+        if (status != W4A16_OK) return status;
+    }
+    // Behind the first kernel always programmatic: it waits for that one itself.  Four warps a row while rows are few.
+    const int64_t pairs = static_cast<int64_t>(p.cache.batch) * p.cache.kv_heads, rows = p.tokens * static_cast<int64_t>(p.group);
+    const bool few = pairs * rows <= 1024;
+    const int rows_per_cta = few ? 1 : rows <= 64 ? 4 : 32;
+    const int64_t ctas = pairs * ((rows + rows_per_cta - 1) / rows_per_cta);
+    return kv_launch(few ? kv_finish_kernel<T, D, 4> : kv_finish_kernel<T, D, 1>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0,
+                     s.grid > 0 || programmatic, stream, p, rows_per_cta);
 }
 
 }  // namespace
@@ -775,7 +843,7 @@ size_t kv_attention_workspace_bytes(const w4a16_kv8_cache& cache, int q_heads, i
     const DeviceState* state = nullptr;
     const int sms = device_state(&state) == 0 ? state->sms : 148;
     const Shape s = shape_of(cache, q_heads, tokens, sms);
-    return s.split ? static_cast<size_t>(s.grid) * 2 * 16 * s.mt * (cache.head_dim + 2) * sizeof(float) : 0;
+    return s.grid > 0 ? s.workspace : 0;
 }
 
 int launch_kv_attention(const w4a16_kv8_cache& cache, const w4a16_rows& q, void* out, int q_heads, int64_t tokens,
@@ -785,8 +853,8 @@ int launch_kv_attention(const w4a16_kv8_cache& cache, const w4a16_rows& q, void*
     if (const int status = device_state(&state); status != 0) return status;
     const Shape s = shape_of(cache, q_heads, tokens, state->sms);
     const int64_t rows = static_cast<int64_t>(cache.batch) * q_heads * tokens;
-    if (rows > INT32_MAX || s.units > INT32_MAX) return W4A16_ERR_TOO_LARGE;
-    if (s.split && (workspace == nullptr || workspace_bytes < kv_attention_workspace_bytes(cache, q_heads, tokens))) return W4A16_ERR_WORKSPACE;
+    if (rows > INT32_MAX || s.units > INT32_MAX / (cache.max_len / kKvBlock + kUnitCost)) return W4A16_ERR_TOO_LARGE;
+    if (s.grid > 0 && (workspace == nullptr || workspace_bytes < s.workspace)) return W4A16_ERR_WORKSPACE;
     AttentionParams p{};
     p.cache = kv_view(cache);
     p.q = static_cast<const char*>(q.data);
@@ -798,13 +866,13 @@ int launch_kv_attention(const w4a16_kv8_cache& cache, const w4a16_rows& q, void*
     p.tokens = static_cast<int>(tokens);
     p.q_heads = q_heads;
     p.group = q_heads / cache.kv_heads;
+    p.tile_rows = s.tile_rows;
     p.row_tiles = s.row_tiles;
     p.lengths = lengths;
     p.counts = counts;
     p.scale = softmax_scale * kLog2e;
     p.parts = static_cast<float*>(workspace);
     p.grid = static_cast<int>(s.grid);
-    p.split = s.split;
     const bool bf16 = cache.type == W4A16_TYPE_BF16;
     if (cache.head_dim == 64) {
         return bf16 ? launch_shape<__nv_bfloat16, 64>(p, s, programmatic, stream) : launch_shape<__half, 64>(p, s, programmatic, stream);
