@@ -34,8 +34,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMinRun = 2 * kWarps;             // blocks that are worth a CTA
-constexpr int kUnitCost = 4;                    // what starting and ending a sequence, head and tile costs, in blocks
+constexpr int kMinRun = 8;                      // blocks that are worth a CTA, with what starting costs
+constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
 constexpr float kNone = -1.0e30f;               // the maximum of nothing
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;            // probabilities are held in FP16 times this: 2^10,
@@ -49,6 +49,7 @@ struct AttentionParams {
     bool q_wide;                                 // rows can be read 16 bytes at a time
     char* out;                                   // [batch][tokens][q heads][D]
     int tokens, q_heads, group;
+    float per_group;                             // 1 / group
     int tile_rows, row_tiles;                    // rows of a CTA, and as many tiles as `tokens` queries make
     const long long* lengths;
     const long long* counts;                     // null: all `tokens` of every sequence
@@ -56,6 +57,15 @@ struct AttentionParams {
     float* parts;                                // workspace: see part_of()
     int grid;                                    // CTAs of the first kernel
 };
+
+// row / group; rows are fewer than 2^24, so that the quotient in FP32 is off by one at most.
+__device__ __forceinline__ int by_group(const AttentionParams& p, int row) {
+    int quotient = static_cast<int>(static_cast<float>(row) * p.per_group);
+    const int rest = row - quotient * p.group;
+    if (rest < 0) --quotient;
+    if (rest >= p.group) ++quotient;
+    return quotient;
+}
 
 struct Sequence {
     int length, count, blocks, row_tiles;        // full blocks; tiles of this sequence's queries
@@ -178,23 +188,25 @@ __device__ __forceinline__ float power_for(float top, float& inverse) {
     return __int_as_float((127 + exponent) << 23);
 }
 
-__device__ __forceinline__ float finite_magnitude(float x) {
-    const float m = fabsf(x);
-    return m <= 3.4028235e38f ? m : 0.0f;
-}
-
 // A team of MT warps shares a ring; each has 8 * NT rows of its own, and the kWarps / MT teams take the blocks in turn.
 template <typename T, int D, int NT, int MT>
 struct AttentionShape {
     static constexpr int kTeams = kWarps / MT;
     static constexpr int kTileRows = 8 * NT * MT;
     static constexpr int kSlotBytes = kKvBlock * D;                    // a block's keys, or its values
-    static constexpr int kSlots = (NT == 1 ? 3 : MT == 1 ? 4 : 8) * (128 / D);
-    static constexpr int kResident = NT == 1 ? 3 : 2;                  // CTAs that fit an SM
+    static constexpr int kSlots = (NT == 1 ? 3 : MT == 1 ? 4 : MT == 2 ? 6 : 8) * (128 / D);
+    static constexpr int kResident = NT == 1 ? 3 : 2;                  // CTAs that fit an SM, beside one of the second kernel
+    static constexpr int kRegisters = NT == 1 ? 152 : 224;
     static constexpr size_t kRingBytes = static_cast<size_t>(kTeams) * kSlots * kSlotBytes;
-    static constexpr size_t kSharedBytes = kRingBytes + static_cast<size_t>(kTeams) * kTileRows * (D + 2) * sizeof(float);
+    static constexpr size_t kMergeBytes = static_cast<size_t>(kTeams) * kTileRows * (D + 2) * sizeof(float);
+    static constexpr size_t kSharedBytes = kRingBytes + kMergeBytes + static_cast<size_t>(kTileRows) * D * 2;      // and the queries
     static_assert(kResident * (kSharedBytes + 2048) <= 227 * 1024);
 };
+
+// 8-row tiles of a warp in the variants for 32 and 64 rows: as many as its registers hold, since they share what makes FP16 of codes.
+// (8 sequences, 40 rows each, D = 64: two tiles and four warps to a ring 20.7 us, four and two WIDEUS.)
+template <int D>
+constexpr int kWide = D == 64 ? 4 : 2;
 
 // What one thread of a team asks for next.  It runs ahead of the team by the ring's slots, across the ends of segments.
 struct Feed {
@@ -205,15 +217,16 @@ struct Feed {
 };
 
 template <typename T, int D, int NT, int MT>
-__global__ void __launch_bounds__(kThreads, AttentionShape<T, D, NT, MT>::kResident)
+__global__ void __maxnreg__((AttentionShape<T, D, NT, MT>::kRegisters))
 kv_attention_kernel(const AttentionParams p) {
     using Shape = AttentionShape<T, D, NT, MT>;
     constexpr int kTeams = Shape::kTeams, kSlots = Shape::kSlots, kTileRows = Shape::kTileRows, kSteps = D / 16;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ __align__(128) uint8_t shared[];
     __shared__ __align__(8) unsigned long long bars[kTeams][kSlots][2];        // full; empty, where several warps share a ring
-    __shared__ Feed feeds[kTeams];
     __shared__ int plan[3];                    // all work; this CTA's sequence; work before it
+    __shared__ __align__(8) float row_scales[kTileRows];       // what the scores of a row are multiplied with
+    __shared__ __align__(8) int row_places[kTileRows];         // its query's position
     pdl_wait_for_upstream();
     pdl_release_downstream();                  // (behind the wait: what the next kernel reads of ours before its own wait is there)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -221,6 +234,7 @@ kv_attention_kernel(const AttentionParams p) {
     const int g = lane >> 2, c = lane & 3;
     uint8_t* const ring = shared + static_cast<size_t>(team) * kSlots * Shape::kSlotBytes;
     float* const merge = reinterpret_cast<float*>(shared + Shape::kRingBytes);
+    uint4* const staged = reinterpret_cast<uint4*>(shared + Shape::kRingBytes + Shape::kMergeBytes);
     const bool feeder = lane == 0 && member == 0;
     if (feeder) {
         for (int s = 0; s < kSlots; ++s) {
@@ -275,7 +289,7 @@ kv_attention_kernel(const AttentionParams p) {
     const int end = runs.begin(blockIdx.x + 1);
 
     bool healthy = true;
-    Feed& feed = feeds[team];
+    Feed feed{at, 0, nullptr, nullptr, 0};           // (the feeder's; others' stays as it is)
     // Asks for what the team needs next, if there is anything left: by the feeder, into the slot that has just become free.
     auto ask = [&]() {
         while (feed.left == 0) {
@@ -292,20 +306,13 @@ kv_attention_kernel(const AttentionParams p) {
             healthy = false;
             return;
         }
-        const uint8_t*& next = feed.left & 1 ? feed.values : feed.keys;
         const unsigned full_bar = smem_u32(&bars[team][slot][0]);
         mbar_arrive_expect_tx(full_bar, Shape::kSlotBytes);
-        bulk_load(smem_u32(ring + slot * Shape::kSlotBytes), next, Shape::kSlotBytes, full_bar);
-        next += kTeams * Shape::kSlotBytes;
+        bulk_load(smem_u32(ring + slot * Shape::kSlotBytes), feed.left & 1 ? feed.values : feed.keys, Shape::kSlotBytes, full_bar);
+        (feed.left & 1 ? feed.values : feed.keys) += kTeams * Shape::kSlotBytes;
         --feed.left;
         ++feed.fill;
     };
-    if (feeder) {
-        feed.at = at;
-        feed.left = 0;
-        feed.fill = 0;
-        for (int i = 0; i < kSlots; ++i) ask();
-    }
     unsigned take = 0;                           // slots that this warp has used
     // A slot, once it has been filled; null if that did not happen.
     auto arrived = [&](unsigned number) -> const uint8_t* {
@@ -340,70 +347,95 @@ kv_attention_kernel(const AttentionParams p) {
         };
         load_scales(first_block);
 
-        // queries as the second operand: row g of each of this warp's 8-row tiles, dims in the order of the codes' bytes
-        const int rows = seg.count * p.group;
-        const int first_row = seg.tile * kTileRows + member * 8 * NT;
-        uint32_t q[NT][kSteps][2];
-        float q_scale[NT][2];                      // of rows 2c and 2c + 1
-        int place[NT][2];                          // their queries' positions
-        int lowest = INT_MAX;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = first_row + n * 8 + g;
+        const int rows = seg.count * p.group, first_row = seg.tile * kTileRows;
+        if (first_segment && member == 0) {        // the ring's first slots: a lane for each, as far as this segment goes
+            const int now = min(kSlots, 2 * coded);
+            const uint8_t* keys = p.cache.k_codes + (pair * p.cache.blocks + first_block) * Shape::kSlotBytes;
+            const uint8_t* values = p.cache.v_codes + (pair * p.cache.blocks + first_block) * Shape::kSlotBytes;
+            if (lane < now) {
+                const unsigned full_bar = smem_u32(&bars[team][lane][0]);
+                mbar_arrive_expect_tx(full_bar, Shape::kSlotBytes);
+                bulk_load(smem_u32(ring + lane * Shape::kSlotBytes), (lane & 1 ? values : keys) + lane / 2 * kTeams * Shape::kSlotBytes,
+                          Shape::kSlotBytes, full_bar);
+            }
+            feed.at = at;
+            feed.left = 2 * coded - now;
+            feed.keys = keys + (now + 1) / 2 * kTeams * Shape::kSlotBytes;
+            feed.values = values + now / 2 * kTeams * Shape::kSlotBytes;
+            feed.fill = now;
+            if (lane == 0) {
+                for (int i = now; i < kSlots; ++i) ask();
+            }
+        }
+        // The queries, as they become the second operand: [8-row tile][two steps of sixteen dims][lane][...], dims in the order of the
+        // codes' bytes.  A thread takes sixteen dims of a row.
+        for (int at = tid; at < kTileRows * kSteps; at += kThreads) {
+            const int tile_row = at / kSteps, chunk = at % kSteps, row = first_row + tile_row;
             const bool there = row < rows;
-            const T* from = reinterpret_cast<const T*>(p.q) + seg.b * p.q_batch + (row / p.group) * p.q_token +
-                            (seg.head * p.group + row % p.group) * p.q_head + c * 16;
-            uint32_t raw[D / 8];                   // sixteen dims of each run of 64
+            const int token = by_group(p, row);
+            const T* from = reinterpret_cast<const T*>(p.q) + seg.b * p.q_batch + token * p.q_token +
+                            (seg.head * p.group + row - token * p.group) * p.q_head + chunk * 16;
+            uint32_t raw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (there && p.q_wide) {
+                const uint4 a = *reinterpret_cast<const uint4*>(from), b = *(reinterpret_cast<const uint4*>(from) + 1);
+                raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+                raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
+            } else if (there) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
 #pragma unroll
-            for (int i = 0; i < D / 8; i += 4) {
-                const T* at = from + i / 8 * 64 + i % 8 * 2;
-                uint4 four = make_uint4(0u, 0u, 0u, 0u);
-                if (there && p.q_wide) {
-                    four = *reinterpret_cast<const uint4*>(at);
-                } else if (there) {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(at);
-                    four = make_uint4(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16,
-                                      h[4] | static_cast<uint32_t>(h[5]) << 16, h[6] | static_cast<uint32_t>(h[7]) << 16);
-                }
-                raw[i] = four.x;
-                raw[i + 1] = four.y;
-                raw[i + 2] = four.z;
-                raw[i + 3] = four.w;
+                for (int i = 0; i < 8; ++i) raw[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
             }
             float back = 1.0f;
             if constexpr (kBf16) {
                 // BF16 queries become FP16 by a power of two of their row's own: a number keeps all its bits unless it is 2^-23
                 // of the row's largest or less.  FP16 ones are taken as they are.
-                float largest = 0.0f;
+                uint32_t largest = 0;                  // (FP32 bits: those of numbers without a sign are ordered like them)
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const float2 f = widen2<T>(raw[i]);
-                    largest = fmaxf(largest, fmaxf(finite_magnitude(f.x), finite_magnitude(f.y)));
-                }
-                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                const float by = power_for(largest, back);
+                for (int i = 0; i < 8; ++i) largest = max(largest, max(raw[i] << 16 & 0x7fffffffu, raw[i] & 0x7fff0000u));
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
+                for (int o = 1; o < kSteps; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+                const float by = power_for(__uint_as_float(min(largest, 0x7f7f0000u)), back);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
                     const float2 f = widen2<T>(raw[i]);
                     raw[i] = pack_half(f.x * by, f.y * by);
                 }
             }
+            // dims 4 w .. 4 w + 3 of the sixteen are step w of their run of 64: the first and third, the second and fourth
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                q[n][i][0] = prmt(raw[2 * i], raw[2 * i + 1], 0x5410);
-                q[n][i][1] = prmt(raw[2 * i], raw[2 * i + 1], 0x7632);
+            for (int w = 0; w < 4; w += 2) {
+                const int to = (tile_row / 8 * (kSteps / 2) + chunk / 4 * 2 + w / 2) * 32 + tile_row % 8 * 4 + chunk % 4;
+                staged[to] = make_uint4(prmt(raw[2 * w], raw[2 * w + 1], 0x5410), prmt(raw[2 * w], raw[2 * w + 1], 0x7632),
+                                        prmt(raw[2 * w + 2], raw[2 * w + 3], 0x5410), prmt(raw[2 * w + 2], raw[2 * w + 3], 0x7632));
             }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                q_scale[n][r] = p.scale * __shfl_sync(0xffffffffu, back, (2 * c + r) * 4);
-                const int of = first_row + n * 8 + 2 * c + r;
-                place[n][r] = of < rows ? seg.length - seg.count + of / p.group : INT_MAX;      // (rows that are not there: anything goes)
-                lowest = min(lowest, place[n][r]);
+            if (chunk == 0) {
+                row_scales[tile_row] = p.scale * back;
+                row_places[tile_row] = there ? seg.length - seg.count + token : INT_MAX;      // (a row that is not there: anything goes)
             }
         }
-        lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 1));
-        lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, 2));
+        __syncthreads();
+        uint32_t q[NT][kSteps][2];
+        float q_scale[NT][2];                      // of rows 2c and 2c + 1
+        int place[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int tile_row = (member * NT + n) * 8;
+#pragma unroll
+            for (int i = 0; i < kSteps; i += 2) {
+                const uint4 four = staged[(tile_row / 8 * (kSteps / 2) + i / 2) * 32 + lane];
+                q[n][i][0] = four.x;
+                q[n][i][1] = four.y;
+                q[n][i + 1][0] = four.z;
+                q[n][i + 1][1] = four.w;
+            }
+            const float2 scales = *reinterpret_cast<const float2*>(row_scales + tile_row + 2 * c);
+            const int2 places = *reinterpret_cast<const int2*>(row_places + tile_row + 2 * c);
+            q_scale[n][0] = scales.x;
+            q_scale[n][1] = scales.y;
+            place[n][0] = places.x;
+            place[n][1] = places.y;
+        }
+        const int lowest = row_places[member * NT * 8];        // (positions go up with the rows)
 
         float acc[NT][kSteps][4];                  // dims 16 j + g and + 8, rows 2c and 2c + 1
         float top[NT][2], sum[NT][2];              // the sum is of this lane's tokens
@@ -421,19 +453,30 @@ kv_attention_kernel(const AttentionParams p) {
         // of them, as operands of the second product: row g, tokens 4c, 4c + 2 and 4c + 1, 4c + 3 of each group.
         uint32_t prob[NT][2][2];
         auto probabilities = [&](float (&score)[NT][2][4], int block, float k_scale, float v_scale) {
-            const bool masked = (block + 1) * kKvBlock - 1 > lowest;
+            const int token = block * kKvBlock + 2 * g;
             bool lag = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float by = k_scale * q_scale[n][r];
+                    // relative to the maximum so far, or to zero while the row has seen nothing
+                    const bool fresh = top[n][r] == kNone;
+                    const float by = k_scale * q_scale[n][r], from = fresh ? 0.0f : -top[n][r], limit = fresh ? -INFINITY : kMaxLag;
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         float& x = score[n][t >> 1][(t & 1) * 2 + r];
-                        x *= by;
-                        if (masked && block * kKvBlock + (t >> 1) * 16 + 2 * g + (t & 1) > place[n][r]) x = -INFINITY;
-                        lag = lag || x > top[n][r] + kMaxLag;
+                        x = fmaf(x, by, from);
+                        lag = lag || x > limit;
+                    }
+                }
+            }
+            if ((block + 1) * kKvBlock - 1 > lowest) {
+                lag = true;                         // (what is masked now may have been what was large)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        if (token + (t >> 2) * 16 + (t >> 1 & 1) > place[n][t & 1]) score[n][t >> 2][t & 3] = -INFINITY;
                     }
                 }
             }
@@ -449,14 +492,18 @@ kv_attention_kernel(const AttentionParams p) {
                     float shrink[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float now = fmaxf(fmaxf(score[n][0][r], score[n][0][2 + r]), fmaxf(score[n][1][r], score[n][1][2 + r]));
+                        const bool fresh = top[n][r] == kNone;
+                        float more = fmaxf(fmaxf(score[n][0][r], score[n][0][2 + r]), fmaxf(score[n][1][r], score[n][1][2 + r]));
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-                        now = fmaxf(now, top[n][r]);
-                        shrink[r] = exp2_fast(top[n][r] - now);
-                        top[n][r] = now;
+                        for (int o = 4; o < 32; o <<= 1) more = fmaxf(more, __shfl_xor_sync(0xffffffffu, more, o));
+                        if (!fresh) more = fmaxf(more, 0.0f);
+                        if (more == -INFINITY) more = 0.0f;               // still nothing seen
+                        else top[n][r] = fresh ? more : top[n][r] + more;
+                        shrink[r] = fresh ? 1.0f : exp2_fast(-more);
                         sum[n][r] *= shrink[r];
                         shrink[r] *= unit_change;
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) score[n][t >> 1][(t & 1) * 2 + r] -= more;
                     }
 #pragma unroll
                     for (int j = 0; j < kSteps; ++j) {
@@ -467,7 +514,15 @@ kv_attention_kernel(const AttentionParams p) {
                     }
                 }
             }
-            const float weight = v_scale * per_scale;
+            float weight = v_scale * per_scale;
+            if (weight != weight) {                 // the block's values are NaN, for the rows that see any of them
+                weight = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (block * kKvBlock <= place[n][0]) sum[n][0] = __int_as_float(0x7fc00000);
+                    if (block * kKvBlock <= place[n][1]) sum[n][1] = __int_as_float(0x7fc00000);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -475,11 +530,9 @@ kv_attention_kernel(const AttentionParams p) {
                     float w[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float x = score[n][t >> 1][(t & 1) * 2 + r];
-                        const float e = exp2_fast(x - top[n][r]);
+                        const float e = exp2_fast(score[n][t >> 1][(t & 1) * 2 + r]);
                         sum[n][r] += e;
                         w[r] = e * weight;
-                        if (masked && x == -INFINITY) w[r] = 0.0f;           // (the block's scale may be NaN)
                     }
                     prob[n][t >> 1][t & 1] = transpose8x8(pack_half(w[0], w[1]));
                 }
@@ -547,7 +600,7 @@ kv_attention_kernel(const AttentionParams p) {
                 for (int o = 4; o < 32; o <<= 1) sum[n][r] += __shfl_xor_sync(0xffffffffu, sum[n][r], o);
             }
         }
-        if (!first_segment) __syncthreads();        // the segment before has been read
+        __syncthreads();                            // the segment before has been read
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -597,7 +650,7 @@ kv_attention_kernel(const AttentionParams p) {
 // multiplied in FP32 as they are.  A CTA has `rows` rows of one sequence and key/value head, ROW_WARPS warps for each at a time.  What
 // needs no part is done before the kernel in front has ended; that one lets this one start only when all before it has.
 template <typename T, int D, int ROW_WARPS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, ROW_WARPS > 1 ? 9 : 6)
 kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
     constexpr int kRows = kWarps / ROW_WARPS;            // at a time
     constexpr int kDims = D / 32;                        // of a lane
@@ -606,6 +659,7 @@ kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
     __shared__ __align__(16) T values[kKvBlock * D];
     __shared__ __align__(16) float queries[kRows][D];
     __shared__ float sums[kWarps][D];
+    __shared__ float2 states[kWarps];
     __shared__ int plan[2];                              // all work; work before this sequence
     if (p.grid == 0) pdl_wait_for_upstream();            // there is no kernel of ours in front
     pdl_release_downstream();
@@ -641,9 +695,8 @@ kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
             if (!s.sound) atomicOr(p.cache.status, kKvBadLength);
         }
     }
-    bool waited = false;
     for (int base = first_row; base < last_row; base += kRows) {
-        const int row = base + warp / ROW_WARPS, i = row / p.group, q_head = head * p.group + row % p.group;
+        const int row = base + warp / ROW_WARPS, i = by_group(p, row), q_head = head * p.group + row - i * p.group;
         const int share = warp % ROW_WARPS;
         const bool there = row < last_row && i < s.count;
         const int position = s.length - s.count + i;
@@ -693,65 +746,81 @@ kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
                 }
             }
         }
-        if (!waited) pdl_wait_for_upstream();
-        waited = true;
+        const float* parts = nullptr;                     // of this row in the runs that have one, `stride` apart
+        int count = 0;
+        const size_t stride = static_cast<size_t>(p.tile_rows) * (D + 2);
         if (there && s.blocks > 0) {
             const Runs runs(p, plan[0]);
             const int tile = row / p.tile_rows;
             const int begin = plan[1] + (head * s.row_tiles + tile) * (s.blocks + kUnitCost) + kUnitCost;
-            const int first = runs.of(begin), count = runs.of(begin + s.blocks - 1) - first + 1;
-            const size_t stride = static_cast<size_t>(p.tile_rows) * (D + 2);
-            const float* parts = part_of(p, b, head, tile, first, D) + row % p.tile_rows * (D + 2);
-            float best = kNone;
-            for (int r = lane; r < count; r += 32) best = fmaxf(best, parts[r * stride + D]);
+            const int first = runs.of(begin);
+            count = runs.of(begin + s.blocks - 1) - first + 1;
+            parts = part_of(p, b, head, tile, first, D) + row % p.tile_rows * (D + 2);
+        }
+        // Before the first rows' parts are there the loop below goes over whatever lies in their place, and what comes of that is
+        // dropped: it brings the code in, which otherwise takes as long as the work itself.
+        const float tail_top = top, tail_weight = weight;
+        float tail_acc[kDims];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-            if (share == 0) best = fmaxf(best, top);
-            const float shrink = exp2_fast(top - best);
-            weight *= shrink;
+        for (int d = 0; d < kDims; ++d) tail_acc[d] = acc[d];
+        for (int pass = base == first_row ? 0 : 1; pass < 2; ++pass) {
+            if (pass == 1 && base == first_row) pdl_wait_for_upstream();
+            top = tail_top;
+            weight = tail_weight;
 #pragma unroll
-            for (int e = 0; e < kDims; ++e) acc[e] *= shrink;
-            top = best;
-            float more = 0.0f;
-            for (int r = share + lane * ROW_WARPS; r < count; r += 32 * ROW_WARPS) {
-                more += exp2_fast(parts[r * stride + D] - best) * parts[r * stride + D + 1];
-            }
+            for (int d = 0; d < kDims; ++d) acc[d] = tail_acc[d];
+            // a few parts at a time, all of their numbers requested together
+            constexpr int kBatch = 16 / kDims;
+            for (int r = share; r < count; r += kBatch * ROW_WARPS) {
+                float2 state[kBatch], numbers[kBatch][kDims / 2];          // maximum and sum
+                float best = top;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
-            weight += more;
-#pragma unroll 8
-            for (int r = share; r < count; r += ROW_WARPS) {
-                const float* from = parts + r * stride;
-                const float w = exp2_fast(from[D] - best);
+                for (int e = 0; e < kBatch; ++e) {
+                    const float* from = parts + (r + e * ROW_WARPS) * stride;
+                    const bool one = r + e * ROW_WARPS < count;
+                    state[e] = one ? __ldcg(reinterpret_cast<const float2*>(from + D)) : make_float2(kNone, 0.0f);
 #pragma unroll
-                for (int e = 0; e < kDims; e += 2) {
-                    const float2 two = *reinterpret_cast<const float2*>(from + lane * kDims + e);
-                    acc[e] = fmaf(w, two.x, acc[e]);
-                    acc[e + 1] = fmaf(w, two.y, acc[e + 1]);
+                    for (int d = 0; d < kDims / 2; ++d) {
+                        numbers[e][d] = one ? __ldcg(reinterpret_cast<const float2*>(from + lane * kDims) + d) : make_float2(0.0f, 0.0f);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) best = fmaxf(best, state[e].x);
+                const float shrink = exp2_fast(top - best);
+                top = best;
+                weight *= shrink;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) acc[d] *= shrink;
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) {
+                    const float w = exp2_fast(state[e].x - best);
+                    weight = fmaf(w, state[e].y, weight);
+#pragma unroll
+                    for (int d = 0; d < kDims / 2; ++d) {
+                        acc[2 * d] = fmaf(w, numbers[e][d].x, acc[2 * d]);
+                        acc[2 * d + 1] = fmaf(w, numbers[e][d].y, acc[2 * d + 1]);
+                    }
                 }
             }
-        }
-        if (ROW_WARPS > 1) {                              // (one row: the CTA's only one at a time)
-            __shared__ float tops[kWarps], weights[kWarps];
+            if (ROW_WARPS > 1) {                          // (one row: the CTA's only one at a time)
+                __syncthreads();
 #pragma unroll
-            for (int e = 0; e < kDims; ++e) sums[warp][lane * kDims + e] = acc[e];
-            if (lane == 0) {
-                tops[warp] = top;
-                weights[warp] = weight;
-            }
-            __syncthreads();
-            top = kNone;
+                for (int e = 0; e < kDims; ++e) sums[warp][lane * kDims + e] = acc[e];
+                if (lane == 0) states[warp] = make_float2(top, weight);
+                __syncthreads();
+                top = kNone;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, tops[w]);
-            weight = 0.0f;
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, states[w].x);
+                weight = 0.0f;
 #pragma unroll
-            for (int e = 0; e < kDims; ++e) acc[e] = 0.0f;
+                for (int e = 0; e < kDims; ++e) acc[e] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float by = exp2_fast(tops[w] - top);
-                weight += by * weights[w];
+                for (int w = 0; w < kWarps; ++w) {
+                    const float by = exp2_fast(states[w].x - top);
+                    weight += by * states[w].y;
 #pragma unroll
-                for (int e = 0; e < kDims; ++e) acc[e] += by * sums[w][lane * kDims + e];
+                    for (int e = 0; e < kDims; ++e) acc[e] += by * sums[w][lane * kDims + e];
+                }
             }
         }
         if (row < last_row && share == 0) {
@@ -768,17 +837,22 @@ struct DeviceState {
     int sms = 0;
 };
 
-template <typename T, int D, int NT, int MT>
-int allow_shared() {
-    return cudaFuncSetAttribute(kv_attention_kernel<T, D, NT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                static_cast<int>(AttentionShape<T, D, NT, MT>::kSharedBytes)) == cudaSuccess
+template <typename Kernel>
+int allow_shared(Kernel kernel, size_t bytes) {
+    // (all that an SM has, so that the second kernel's CTAs find room beside the first's)
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess &&
+                   cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) == cudaSuccess
                ? 0
                : W4A16_ERR_LAUNCH;
 }
 
 template <typename T, int D>
 int allow_all() {
-    return allow_shared<T, D, 1, 1>() | allow_shared<T, D, 2, 1>() | allow_shared<T, D, 2, 2>() | allow_shared<T, D, 2, 4>();
+    return allow_shared(kv_attention_kernel<T, D, 1, 1>, AttentionShape<T, D, 1, 1>::kSharedBytes) |
+           allow_shared(kv_attention_kernel<T, D, 2, 1>, AttentionShape<T, D, 2, 1>::kSharedBytes) |
+           allow_shared(kv_attention_kernel<T, D, kWide<D>, 4 / kWide<D>>, AttentionShape<T, D, kWide<D>, 4 / kWide<D>>::kSharedBytes) |
+           allow_shared(kv_attention_kernel<T, D, kWide<D>, 8 / kWide<D>>, AttentionShape<T, D, kWide<D>, 8 / kWide<D>>::kSharedBytes) |
+           allow_shared(kv_finish_kernel<T, D, 1>, 0) | allow_shared(kv_finish_kernel<T, D, 4>, 0);
 }
 
 int device_state(const DeviceState** state) {
@@ -820,12 +894,14 @@ int launch_shape(const AttentionParams& p, const Shape& s, bool programmatic, cu
     };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
-    using Four = std::integral_constant<int, 4>;
+    using Wide = std::integral_constant<int, kWide<D>>;
+    using Half = std::integral_constant<int, 4 / kWide<D>>;
+    using Whole = std::integral_constant<int, 8 / kWide<D>>;
     if (s.grid > 0) {
         const int status = s.tile_rows == 8    ? run(One{}, One{})
                            : s.tile_rows == 16 ? run(Two{}, One{})
-                           : s.tile_rows == 32 ? run(Two{}, Two{})
-                                               : run(Two{}, Four{});
+                           : s.tile_rows == 32 ? run(Wide{}, Half{})
+                                               : run(Wide{}, Whole{});
         if (status != W4A16_OK) return status;
     }
     // Behind the first kernel always programmatic: it waits for that one itself.  Four warps a row while rows are few.
@@ -853,7 +929,7 @@ int launch_kv_attention(const w4a16_kv8_cache& cache, const w4a16_rows& q, void*
     if (const int status = device_state(&state); status != 0) return status;
     const Shape s = shape_of(cache, q_heads, tokens, state->sms);
     const int64_t rows = static_cast<int64_t>(cache.batch) * q_heads * tokens;
-    if (rows > INT32_MAX || s.units > INT32_MAX / (cache.max_len / kKvBlock + kUnitCost)) return W4A16_ERR_TOO_LARGE;
+    if (rows > INT32_MAX || rows / cache.batch / cache.kv_heads >= 1 << 24 || s.units > INT32_MAX / (cache.max_len / kKvBlock + kUnitCost)) return W4A16_ERR_TOO_LARGE;
     if (s.grid > 0 && (workspace == nullptr || workspace_bytes < s.workspace)) return W4A16_ERR_WORKSPACE;
     AttentionParams p{};
     p.cache = kv_view(cache);
@@ -866,6 +942,7 @@ int launch_kv_attention(const w4a16_kv8_cache& cache, const w4a16_rows& q, void*
     p.tokens = static_cast<int>(tokens);
     p.q_heads = q_heads;
     p.group = q_heads / cache.kv_heads;
+    p.per_group = 1.0f / static_cast<float>(p.group);
     p.tile_rows = s.tile_rows;
     p.row_tiles = s.row_tiles;
     p.lengths = lengths;
