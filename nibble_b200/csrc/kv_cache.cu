@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "kernels.h"
@@ -73,74 +74,93 @@ struct RotaryRows {
     bool interleaved;
     bool wide;                                   // rows can be read and written 16 bytes at a time
     bool in_place;                               // what is not turned is there already
+    int pieces, piece_bits;                      // of a head, eight numbers or eight pairs each (wide), and bits that number them
 };
 
 // Turns `heads` heads from `first_head` on of `tokens` tokens; table[token * rotary_dim / 2 + pair] holds the factors.
-template <typename T>
-__device__ void rotate_rows(const RotaryRows& r, const float2* table, long long b, long long first_token, int tokens, int first_head,
-                            int heads) {
-    const int half = r.rotary_dim / 2;
-    const int unit = r.wide ? 8 : 1;             // pairs of a piece (halves); numbers of a piece (pairs, rest)
-    const int turned = r.interleaved ? (r.wide ? r.rotary_dim / 8 : half) : half / unit;
-    const int pieces = turned + (r.in_place ? 0 : (r.head_dim - r.rotary_dim) / unit);
-    const int total = tokens * heads * pieces;
-    const int per_token = heads * pieces;
-    constexpr int kBatch = 4;                    // pieces requested together
-    for (int base = threadIdx.x; base < total; base += kBatch * blockDim.x) {
-        const T* from[kBatch];
-        T* to[kBatch];
-        int piece[kBatch];
-        const float2* f[kBatch];
-        uint4 lo[kBatch], hi[kBatch];
+//
+// Wide rows: a thread keeps to one piece of a head and takes heads (and tokens, while heads are few) in turn, so that nothing is
+// divided out on the way and a token's factors are read once.  (With the pieces of a tile numbered through, 4096 tokens of 72
+// heads of 128 took 77 us, most of it divisions.)
+template <typename T, bool INTERLEAVED>
+__device__ __forceinline__ void rotate_rows_wide(const RotaryRows& r, const float2* table, long long b, long long first_token, int tokens,
+                                                 int first_head, int heads) {
+    constexpr int kFactors = INTERLEAVED ? 4 : 8;
+    constexpr int kBatch = INTERLEAVED ? 4 : 2;  // heads requested together
+    const int half = r.rotary_dim / 2, turned = half / kFactors;
+    const int piece = threadIdx.x & ((1 << r.piece_bits) - 1), row = threadIdx.x >> r.piece_bits, rows = blockDim.x >> r.piece_bits;
+    if (piece >= r.pieces) return;
+    const bool plain = piece >= turned;          // left as it is
+    const int d = plain ? r.rotary_dim + (piece - turned) * 8 : piece * 8;
+    int abreast = 1;                             // heads that a pass takes side by side
+    while (abreast < heads && abreast < rows) abreast *= 2;
+    const int token_step = rows / abreast, first = row & (abreast - 1);
+    const long long in_step = abreast * r.in.head, out_step = abreast * r.out.head;
+    for (int token = row / abreast; token < tokens; token += token_step) {
+        const float2* factors = table + token * half + piece * kFactors;
+        const T* in = row_of<T>(r.in, b, first_token + token, first_head + first) + d;
+        T* out = const_cast<T*>(row_of<T>(r.out, b, first_token + token, first_head + first)) + d;
+        float2 f[kFactors];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            const int at = base + e * static_cast<int>(blockDim.x);
-            if (at >= total) break;
-            const int token = at / per_token, rest = at - token * per_token;
-            const int head = rest / pieces;
-            piece[e] = rest - head * pieces;
-            from[e] = row_of<T>(r.in, b, first_token + token, first_head + head);
-            to[e] = const_cast<T*>(row_of<T>(r.out, b, first_token + token, first_head + head));
-            f[e] = table + token * half;
-            if (!r.wide) continue;
-            if (piece[e] >= turned) {
-                const int d = r.rotary_dim + (piece[e] - turned) * 8;
-                lo[e] = *reinterpret_cast<const uint4*>(from[e] + d);
-            } else {
-                lo[e] = *reinterpret_cast<const uint4*>(from[e] + piece[e] * 8);
-                if (!r.interleaved) hi[e] = *reinterpret_cast<const uint4*>(from[e] + half + piece[e] * 8);
-            }
+        for (int i = 0; i < kFactors; i += 2) {
+            if (plain) break;
+            const float4 two = *reinterpret_cast<const float4*>(factors + i);      // (a piece's factors begin at an even one)
+            f[i] = make_float2(two.x, two.y);
+            f[i + 1] = make_float2(two.z, two.w);
         }
+        for (int head = first; head < heads; head += kBatch * abreast, in += kBatch * in_step, out += kBatch * out_step) {
+            uint4 lo[kBatch], hi[kBatch];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) {
-            if (base + e * static_cast<int>(blockDim.x) >= total) break;
-            if (r.wide) {
-                if (piece[e] >= turned) {
-                    const int d = r.rotary_dim + (piece[e] - turned) * 8;
-                    *reinterpret_cast<uint4*>(to[e] + d) = lo[e];
-                } else if (r.interleaved) {
-                    turn8_pairs<T>(lo[e], f[e] + piece[e] * 4);
-                    *reinterpret_cast<uint4*>(to[e] + piece[e] * 8) = lo[e];
-                } else {
-                    turn8_halves<T>(lo[e], hi[e], f[e] + piece[e] * 8);
-                    *reinterpret_cast<uint4*>(to[e] + piece[e] * 8) = lo[e];
-                    *reinterpret_cast<uint4*>(to[e] + half + piece[e] * 8) = hi[e];
+            for (int e = 0; e < kBatch; ++e) {
+                if (head + e * abreast >= heads) break;
+                lo[e] = *reinterpret_cast<const uint4*>(in + e * in_step);
+                if (!INTERLEAVED && !plain) hi[e] = *reinterpret_cast<const uint4*>(in + e * in_step + half);
+            }
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                if (head + e * abreast >= heads) break;
+                if (!plain) {
+                    if constexpr (INTERLEAVED) {
+                        turn8_pairs<T>(lo[e], f);
+                    } else {
+                        turn8_halves<T>(lo[e], hi[e], f);
+                        *reinterpret_cast<uint4*>(out + e * out_step + half) = hi[e];
+                    }
                 }
-            } else if (piece[e] >= turned) {
-                const int d = r.rotary_dim + piece[e] - turned;
-                to[e][d] = from[e][d];
-            } else {
-                const int da = r.interleaved ? 2 * piece[e] : piece[e], db = r.interleaved ? da + 1 : da + half;
-                const float x = widen<T>(from[e][da]), y = widen<T>(from[e][db]);
-                to[e][da] = narrow<T>(rotary_first(x, y, f[e][piece[e]]));
-                to[e][db] = narrow<T>(rotary_second(x, y, f[e][piece[e]]));
+                *reinterpret_cast<uint4*>(out + e * out_step) = lo[e];
             }
         }
     }
 }
 
+template <typename T>
+__device__ void rotate_rows(const RotaryRows& r, const float2* table, long long b, long long first_token, int tokens, int first_head,
+                            int heads) {
+    if (r.wide) {
+        if (r.interleaved) rotate_rows_wide<T, true>(r, table, b, first_token, tokens, first_head, heads);
+        else rotate_rows_wide<T, false>(r, table, b, first_token, tokens, first_head, heads);
+        return;
+    }
+    const int half = r.rotary_dim / 2, pieces = half + (r.in_place ? 0 : r.head_dim - r.rotary_dim);      // pairs, and the rest
+    const int total = tokens * heads * pieces;
+    for (int at = threadIdx.x; at < total; at += blockDim.x) {
+        const int row = at / pieces, piece = at - row * pieces, token = row / heads, head = row - token * heads;
+        const T* from = row_of<T>(r.in, b, first_token + token, first_head + head);
+        T* to = const_cast<T*>(row_of<T>(r.out, b, first_token + token, first_head + head));
+        if (piece >= half) {
+            to[half + piece] = from[half + piece];
+            continue;
+        }
+        const int da = r.interleaved ? 2 * piece : piece, db = r.interleaved ? da + 1 : da + half;
+        const float x = widen<T>(from[da]), y = widen<T>(from[db]);
+        const float2 f = table[token * half + piece];
+        to[da] = narrow<T>(rotary_first(x, y, f));
+        to[db] = narrow<T>(rotary_second(x, y, f));
+    }
+}
+
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryTokens = 8;                 // of a CTA, which forms their cosines and sines once for all its heads
+constexpr int kRotaryTokens = 4;                 // of a CTA, which forms their cosines and sines once for all its heads
 constexpr int kMaxRotaryDim = 256;
 
 struct RotaryParams {
@@ -153,9 +173,9 @@ struct RotaryParams {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kRotaryThreads)
+__global__ void __launch_bounds__(kRotaryThreads, 4)
 rotary_kernel(const RotaryParams p) {
-    __shared__ float2 table[kRotaryTokens * kMaxRotaryDim / 2];
+    __shared__ __align__(16) float2 table[kRotaryTokens * kMaxRotaryDim / 2];
     pdl_release_downstream();
     pdl_wait_for_upstream();
     const int part = blockIdx.x % p.head_parts;
@@ -174,12 +194,7 @@ rotary_kernel(const RotaryParams p) {
 
 // ------------------------------------------------------------------ tokens into the cache
 
-// The larger of two numbers; NaN if either is.
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
-}
+constexpr int64_t kAppendCtas = 148 * 8;          // two rounds of what the SMs hold
 
 struct AppendParams {
     KvCache cache;
@@ -188,7 +203,7 @@ struct AppendParams {
     const long long* start;
     const long long* counts;                     // null: all `tokens` of every sequence
     bool wide;                                   // k and v can be read 16 bytes at a time
-    int chunks;                                  // CTAs of a sequence and head: blocks that its tokens can touch
+    int chunks;                                  // CTAs of a sequence and head, which take the blocks that its tokens touch in turn
     // with rotary positions
     const float* inv_freq;
     float rope_scale;
@@ -213,55 +228,99 @@ __device__ __forceinline__ void load16(const T* src, bool wide, uint32_t (&w)[8]
 }
 
 // Largest magnitude of sixteen numbers, NaN if one is NaN.
+__device__ __forceinline__ uint32_t max2_or_nan(uint32_t a, uint32_t b, __half) {
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    return a;
+}
+__device__ __forceinline__ uint32_t max2_or_nan(uint32_t a, uint32_t b, __nv_bfloat16) {
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    return a;
+}
+// (Bits of 16-bit numbers without a sign are ordered as the numbers are, NaN last: from here on the maximum is an integer's.)
 template <typename T>
-__device__ __forceinline__ float magnitude16(const uint32_t (&w)[8]) {
-    float m = 0.0f;
+__device__ __forceinline__ unsigned magnitude16(const uint32_t (&w)[8]) {
+    uint32_t m = w[0] & 0x7fff7fffu;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float2 f = widen2<T>(w[i]);
-        m = max_or_nan(m, max_or_nan(fabsf(f.x), fabsf(f.y)));
-    }
-    return m;
+    for (int i = 1; i < 8; ++i) m = max2_or_nan(m, w[i] & 0x7fff7fffu, T());
+    return max(m & 0xffffu, m >> 16);
 }
 
-// Four codes of a word each.  round_half_even(127 x / top): 127 x is exact in FP32 (11 + 7 bits) and the quotient is rounded
-// correctly; unless 127 x / top lies on a tie it is further from one than the quotient's rounding, and a tie is exact.  So the
-// codes are those of exact arithmetic.
+// Four codes of a word each: round_half_even(127 x / top).
+//
+// Exactly: x and top have eleven bits at most, so 127 x / top is either on a tie k + 1/2 or further from one than 2^-20 of itself.
+// 127 / top is taken a little too large and a little too small (by 2^-22 to 2^-21); the products with x, rounded to an integer by adding
+// 1.5 * 2^23, whose low byte then is the code, are the same unless 127 x / top is a tie.  A lane that sees one does its sixteen
+// over with the division: 127 x has 18 bits, and the quotient, correctly rounded, is the tie.  (With the division throughout 2 x 8191
+// tokens written and read back took 62 us.)
 template <typename T>
 __device__ __forceinline__ void codes16(const uint32_t (&w)[8], float top, uint32_t (&codes)[4]) {
-    // (a top near the end of BF16's range: both brought down, so that 127 x stays finite)
-    const float shrink = top > 1.0e36f ? 1.0f / 256.0f : 1.0f;
-    const float by = top * shrink;
-    const bool plain = top > 0.0f && top <= 3.4028235e38f;               // not for blocks of zeros, nor with a NaN or infinity
+    constexpr float kMagic = 12582912.0f;
+    if (!(top > 0.0f && top <= 3.4028235e38f)) {                         // a block of zeros, or with a NaN or infinity in it
+        codes[0] = codes[1] = codes[2] = codes[3] = 0;
+        return;
+    }
+    const float by = __fdividef(127.0f, top);
+    const float above = by * 1.0000004f, below = by * 0.9999996f;
+    uint32_t differ = top > 1.0e-30f && top < 1.0e30f ? 0u : 1u;         // (beyond these 127 / top may not be a normal number)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 a = widen2<T>(w[2 * i]), b = widen2<T>(w[2 * i + 1]);
         const float x[4] = {a.x, a.y, b.x, b.y};
-        uint32_t word = 0;
+        uint32_t bits[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int code = plain ? __float2int_rn(__fdiv_rn(x[e] * shrink * 127.0f, by)) : 0;
-            word |= (static_cast<uint32_t>(code) & 0xffu) << (8 * e);
+            bits[e] = __float_as_uint(fmaf(x[e], above, kMagic));
+            differ |= bits[e] ^ __float_as_uint(fmaf(x[e], below, kMagic));
         }
-        codes[i] = word;
+        codes[i] = __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
+    }
+    if (differ != 0) {
+        // (a top near the end of BF16's range: both brought down, so that 127 x stays finite)
+        const float shrink = top > 1.0e36f ? 1.0f / 256.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 x = widen2<T>(w[2 * i + e]);
+                const int lo = __float2int_rn(__fdiv_rn(x.x * shrink * 127.0f, top * shrink));
+                const int hi = __float2int_rn(__fdiv_rn(x.y * shrink * 127.0f, top * shrink));
+                word |= (static_cast<uint32_t>(lo) & 0xffu | (static_cast<uint32_t>(hi) & 0xffu) << 8) << (16 * e);
+            }
+            codes[i] = word;
+        }
     }
 }
+
+// Four words of four bytes each, rows and columns exchanged.
+__device__ __forceinline__ void transpose_bytes(uint32_t (&w)[4]) {
+    const uint32_t lo01 = __byte_perm(w[0], w[1], 0x5140), hi01 = __byte_perm(w[0], w[1], 0x7362);      // 0a 1a 0b 1b; 0c 1c 0d 1d
+    const uint32_t lo23 = __byte_perm(w[2], w[3], 0x5140), hi23 = __byte_perm(w[2], w[3], 0x7362);
+    w[0] = __byte_perm(lo01, lo23, 0x5410);
+    w[1] = __byte_perm(lo01, lo23, 0x7632);
+    w[2] = __byte_perm(hi01, hi23, 0x5410);
+    w[3] = __byte_perm(hi01, hi23, 0x7632);
+}
+
+// Where a 16-byte piece of a block's value codes is kept in shared memory: in its line of 32, moved so that threads that work on
+// other lines meet other banks.
+__device__ __forceinline__ int value_piece(int line, int piece) { return line * 32 + (piece ^ (line & 7)); }
 
 __device__ __forceinline__ float scale_of(float top) {
     return top <= 3.4028235e38f ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fc00000);
 }
 
-// One CTA for a block of one sequence and key/value head that the new tokens touch: a thread owns sixteen numbers of a key and of a
+// A CTA takes blocks of one sequence and key/value head that the new tokens touch: a thread owns sixteen numbers of a key and of a
 // value.  A block that becomes full is read (older tokens from the tail), its codes and scales are written; of the newest two blocks
 // the numbers themselves go to the tail, into the slot of the block's parity.  The CTA of the first block reads a tail slot that the
 // newest blocks may write, so it writes that slot itself, after it has read.
 template <typename T, int D, bool ROTARY>
-__global__ void __launch_bounds__(2 * D)
+__global__ void __launch_bounds__(2 * D, (ROTARY ? 768 : 1024) / (2 * D))
 kv_append_kernel(const AppendParams p) {
     constexpr int kThreads = 2 * D, kWarps = kThreads / 32;
-    extern __shared__ float2 factors[];                              // [32][rotary_dim / 2]
-    __shared__ __align__(16) uint8_t turned_codes[kKvBlock * D];      // a block's value codes in the cache's order
-    __shared__ float tops[2][kWarps];
+    extern __shared__ __align__(16) float2 factors[];                              // [32][rotary_dim / 2]
+    __shared__ __align__(16) uint4 turned_codes[2 * D];               // a block's value codes in the cache's order
+    __shared__ unsigned tops[2][kWarps];
     pdl_release_downstream();
     pdl_wait_for_upstream();
     const int tid = threadIdx.x;
@@ -292,20 +351,29 @@ kv_append_kernel(const AppendParams p) {
     }
     const int begin = static_cast<int>(start), end = begin + static_cast<int>(count);
     const int first_block = begin / kKvBlock, newest = end / kKvBlock;   // `newest`: the one that the next token goes to
-    const int block = first_block + chunk;
-    if (count == 0 || block * kKvBlock >= end) return;
-    // this thread's token and sixteen dims: byte tid * 16 of the block's key codes
-    constexpr int kRuns = D / 64;
+    if (count == 0) return;
+    // this thread's token and sixteen dims of the keys: byte tid * 16 of the block's key codes
+    constexpr int kRuns = D / 64, kChunks = D / 16;
     const int line = tid / 32, lane = tid % 32;
     const int slot = line / kRuns / 2 * 16 + lane / 4 * 2 + line / kRuns % 2;
     const int d0 = line % kRuns * 64 + lane % 4 * 16;
+    // and of the values: four lanes kChunks apart have four tokens in a row
+    const int v_slot = tid / kChunks, v_d0 = tid % kChunks * 16;
 
     T* const k_tail = reinterpret_cast<T*>(p.cache.k_tail) + static_cast<size_t>(pair) * 2 * kKvBlock * D;
     T* const v_tail = reinterpret_cast<T*>(p.cache.v_tail) + static_cast<size_t>(pair) * 2 * kKvBlock * D;
 
     // The numbers of a block's token as the cache gets them (the key turned), as they lie in the tail, or zeros.
     auto fetch = [&](int of_block, uint32_t (&k)[8], uint32_t (&v)[8]) {
-        const int t = of_block * kKvBlock + slot;
+        const int t = of_block * kKvBlock + slot, v_t = of_block * kKvBlock + v_slot;
+        if (v_t < begin) {
+            load16<T>(v_tail + ((of_block & 1) * kKvBlock + v_slot) * D + v_d0, true, v);
+        } else if (v_t < end) {
+            load16<T>(row_of<T>(p.v, b, v_t - begin, head) + v_d0, p.wide, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0;
+        }
         if (ROTARY) {
             __syncthreads();
             const int half = p.rotary_dim / 2;
@@ -316,11 +384,9 @@ kv_append_kernel(const AppendParams p) {
         }
         if (t < begin) {
             load16<T>(k_tail + ((of_block & 1) * kKvBlock + slot) * D + d0, true, k);
-            load16<T>(v_tail + ((of_block & 1) * kKvBlock + slot) * D + d0, true, v);
         } else if (t < end) {
             const T* from = row_of<T>(p.k, b, t - begin, head);
             load16<T>(from + d0, p.wide, k);
-            load16<T>(row_of<T>(p.v, b, t - begin, head) + d0, p.wide, v);
             if (ROTARY) {
                 const int half = p.rotary_dim / 2;
                 const float2* f = factors + slot * half;
@@ -346,64 +412,77 @@ kv_append_kernel(const AppendParams p) {
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) k[i] = v[i] = 0;
+            for (int i = 0; i < 8; ++i) k[i] = 0;
         }
     };
     auto keep = [&](int of_block, const uint32_t (&k)[8], const uint32_t (&v)[8]) {
-        const int t = of_block * kKvBlock + slot;
-        if (t < begin || t >= end) return;
-        const size_t at = static_cast<size_t>((of_block & 1) * kKvBlock + slot) * D + d0;
-        uint4* to_k = reinterpret_cast<uint4*>(k_tail + at);
-        uint4* to_v = reinterpret_cast<uint4*>(v_tail + at);
-        to_k[0] = make_uint4(k[0], k[1], k[2], k[3]);
-        to_k[1] = make_uint4(k[4], k[5], k[6], k[7]);
-        to_v[0] = make_uint4(v[0], v[1], v[2], v[3]);
-        to_v[1] = make_uint4(v[4], v[5], v[6], v[7]);
+        const int t = of_block * kKvBlock + slot, v_t = of_block * kKvBlock + v_slot;
+        if (t >= begin && t < end) {
+            uint4* to = reinterpret_cast<uint4*>(k_tail + static_cast<size_t>((of_block & 1) * kKvBlock + slot) * D + d0);
+            to[0] = make_uint4(k[0], k[1], k[2], k[3]);
+            to[1] = make_uint4(k[4], k[5], k[6], k[7]);
+        }
+        if (v_t >= begin && v_t < end) {
+            uint4* to = reinterpret_cast<uint4*>(v_tail + static_cast<size_t>((of_block & 1) * kKvBlock + v_slot) * D + v_d0);
+            to[0] = make_uint4(v[0], v[1], v[2], v[3]);
+            to[1] = make_uint4(v[4], v[5], v[6], v[7]);
+        }
     };
 
-    uint32_t k[8], v[8];
-    fetch(block, k, v);
-    if (block < newest) {                                             // all of its 32 tokens are there
-        float k_top = magnitude16<T>(k), v_top = magnitude16<T>(v);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            k_top = max_or_nan(k_top, __shfl_xor_sync(0xffffffffu, k_top, o));
-            v_top = max_or_nan(v_top, __shfl_xor_sync(0xffffffffu, v_top, o));
-        }
-        if (lane == 0) {
-            tops[0][tid / 32] = k_top;
-            tops[1][tid / 32] = v_top;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            k_top = max_or_nan(k_top, tops[0][w]);
-            v_top = max_or_nan(v_top, tops[1][w]);
-        }
-        const size_t at = static_cast<size_t>(pair) * p.cache.blocks + block;
-        uint32_t codes[4];
-        codes16<T>(k, k_top, codes);
-        *reinterpret_cast<uint4*>(p.cache.k_codes + at * (kKvBlock * D) + tid * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-        codes16<T>(v, v_top, codes);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            turned_codes[kv_value_offset<D>(slot, d0 + e)] = static_cast<uint8_t>(codes[e / 4] >> (8 * (e % 4)));
-        }
-        if (tid == 0) {
-            p.cache.k_scales[at] = scale_of(k_top);
-            p.cache.v_scales[at] = scale_of(v_top);
-        }
-        __syncthreads();
-        *reinterpret_cast<uint4*>(p.cache.v_codes + at * (kKvBlock * D) + tid * 16) = *reinterpret_cast<const uint4*>(turned_codes + tid * 16);
-    }
     // A newest block of the first one's parity shares its tail slot: the first one's CTA writes it, if it read that slot.
     const int shared = ((newest - first_block) & 1) == 0 ? newest : newest - 1;
     const bool first_reads = begin % kKvBlock != 0 && first_block < newest && shared > first_block;
-    if (block >= newest - 1 && !(first_reads && block == shared)) keep(block, k, v);
-    if (first_reads && block == first_block && shared * kKvBlock < end) {
-        __syncthreads();                                              // all of the old slot has been read
-        fetch(shared, k, v);
-        keep(shared, k, v);
+    uint32_t k[8], v[8];
+    for (int block = first_block + chunk; block * kKvBlock < end; block += p.chunks) {
+        fetch(block, k, v);
+        if (block < newest) {                                             // all of its 32 tokens are there
+            unsigned k_bits = __reduce_max_sync(0xffffffffu, magnitude16<T>(k)), v_bits = __reduce_max_sync(0xffffffffu, magnitude16<T>(v));
+            if (lane == 0) {
+                tops[0][tid / 32] = k_bits;
+                tops[1][tid / 32] = v_bits;
+            }
+            __syncthreads();
+            k_bits = __reduce_max_sync(0xffffffffu, tops[0][lane % kWarps]);
+            v_bits = __reduce_max_sync(0xffffffffu, tops[1][lane % kWarps]);
+            const float k_top = widen2<T>(k_bits).x, v_top = widen2<T>(v_bits).x;
+            const size_t at = static_cast<size_t>(pair) * p.cache.blocks + block;
+            uint32_t codes[4];
+            codes16<T>(k, k_top, codes);
+            *reinterpret_cast<uint4*>(p.cache.k_codes + at * (kKvBlock * D) + tid * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+            codes16<T>(v, v_top, codes);
+            // Four tokens of four dims each to a lane, in two exchanges (word i of a lane is dims 4 i to 4 i + 3 of its token; then word u
+            // of lane i is those of token u), and then bytes, so that a word is four tokens of a dim.
+            const int quarter = lane / kChunks % 4;
+#pragma unroll
+            for (int bit = 1; bit < 4; bit *= 2) {
+                const bool upper = (quarter & bit) != 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i & bit) continue;
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? codes[i] : codes[i + bit], bit * kChunks);
+                    if (upper) codes[i] = got;
+                    else codes[i + bit] = got;
+                }
+            }
+            transpose_bytes(codes);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at_byte = kv_value_offset<D>(v_slot & ~3, v_d0 + quarter * 4 + i);
+                reinterpret_cast<uint32_t*>(turned_codes + value_piece(at_byte / 512, at_byte / 16 % 32))[at_byte / 4 % 4] = codes[i];
+            }
+            if (tid == 0) {
+                p.cache.k_scales[at] = scale_of(k_top);
+                p.cache.v_scales[at] = scale_of(v_top);
+            }
+            __syncthreads();
+            *reinterpret_cast<uint4*>(p.cache.v_codes + at * (kKvBlock * D) + tid * 16) = turned_codes[value_piece(line, lane)];
+        }
+        if (block >= newest - 1 && !(first_reads && block == shared)) keep(block, k, v);
+        if (first_reads && block == first_block && shared * kKvBlock < end) {
+            __syncthreads();                                              // all of the old slot has been read
+            fetch(shared, k, v);
+            keep(shared, k, v);
+        }
     }
 }
 
@@ -419,12 +498,21 @@ struct ReadParams {
     int chunks;
 };
 
-// A CTA for a block of one sequence and head; a thread for sixteen numbers of a key and of a value.
+// A word of four codes times a scale, rounded: (c0, c1) and (c2, c3).
+template <typename T>
+__device__ __forceinline__ uint2 values4(uint32_t word, float scale) {
+    const uint32_t even = hsub2_u32(and_xor(word, 0x00ff00ffu, 0x64806480u), 0x64806480u);              // c0, c2 in FP16
+    const uint32_t odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
+    const float2 a = widen2<__half>(even), b = widen2<__half>(odd);
+    return make_uint2(narrow2<T>(a.x * scale, b.x * scale), narrow2<T>(a.y * scale, b.y * scale));
+}
+
+// A CTA for a block of one sequence and head; a thread for sixteen numbers of a key, and of the values for four dims of four tokens.
 template <typename T, int D>
 __global__ void __launch_bounds__(2 * D)
 kv_read_kernel(const ReadParams p) {
     constexpr int kRuns = D / 64;
-    __shared__ __align__(16) uint8_t turned_codes[kKvBlock * D];
+    __shared__ __align__(16) uint4 turned_codes[2 * D];
     pdl_release_downstream();
     pdl_wait_for_upstream();
     const int tid = threadIdx.x, line = tid / 32, lane = tid % 32;
@@ -432,48 +520,60 @@ kv_read_kernel(const ReadParams p) {
     const unsigned pair = blockIdx.x / p.chunks;
     const int b = pair / p.cache.kv_heads, head = pair % p.cache.kv_heads;
     long long length = p.lengths[b];
-    const long long first = p.first == nullptr ? 0 : p.first[b];
+    long long first = p.first == nullptr ? 0 : p.first[b];
     if (length < 0 || length > p.cache.max_len || first < 0) {
         if (tid == 0) atomicOr(p.cache.status, kKvBadLength);
         length = 0;
+        first = max(first, 0ll);
     }
-    const long long block = (first < 0 ? 0 : first / kKvBlock) + chunk;
+    const long long block = first / kKvBlock + chunk;
     const int slot = line / kRuns / 2 * 16 + lane / 4 * 2 + line / kRuns % 2;
     const int d0 = line % kRuns * 64 + lane % 4 * 16;
-    const long long t = block * kKvBlock + slot;
-    const long long row = t - (first < 0 ? 0 : first);                 // of the output
-    uint32_t k[8], v[8];
+    const int quad = tid / (D / 4), v_d0 = tid % (D / 4) * 4;          // tokens 4 quad to 4 quad + 3, dims v_d0 to v_d0 + 3
+    uint2 k[4], v[4];
     if (block < length / kKvBlock) {
         const size_t at = static_cast<size_t>(pair) * p.cache.blocks + block;
         const uint4 k_codes = __ldcs(reinterpret_cast<const uint4*>(p.cache.k_codes + at * (kKvBlock * D) + tid * 16));
-        *reinterpret_cast<uint4*>(turned_codes + tid * 16) =
-            __ldcs(reinterpret_cast<const uint4*>(p.cache.v_codes + at * (kKvBlock * D) + tid * 16));
+        turned_codes[value_piece(line, lane)] = __ldcs(reinterpret_cast<const uint4*>(p.cache.v_codes + at * (kKvBlock * D) + tid * 16));
         const float k_scale = p.cache.k_scales[at], v_scale = p.cache.v_scales[at];
-        const int8_t* codes = reinterpret_cast<const int8_t*>(&k_codes);
+        k[0] = values4<T>(k_codes.x, k_scale);
+        k[1] = values4<T>(k_codes.y, k_scale);
+        k[2] = values4<T>(k_codes.z, k_scale);
+        k[3] = values4<T>(k_codes.w, k_scale);
         __syncthreads();
+        uint32_t words[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            k[i] = narrow2<T>(codes[2 * i] * k_scale, codes[2 * i + 1] * k_scale);
-            const int8_t a = static_cast<int8_t>(turned_codes[kv_value_offset<D>(slot, d0 + 2 * i)]);
-            const int8_t c = static_cast<int8_t>(turned_codes[kv_value_offset<D>(slot, d0 + 2 * i + 1)]);
-            v[i] = narrow2<T>(a * v_scale, c * v_scale);
+        for (int i = 0; i < 4; ++i) {
+            const int at_byte = kv_value_offset<D>(quad * 4, v_d0 + i);
+            words[i] = reinterpret_cast<const uint32_t*>(turned_codes + value_piece(at_byte / 512, at_byte / 16 % 32))[at_byte / 4 % 4];
         }
-    } else if (t < length) {
-        const size_t at = ((static_cast<size_t>(pair) * 2 + (block & 1)) * kKvBlock + slot) * D + d0;
-        load16<T>(reinterpret_cast<const T*>(p.cache.k_tail) + at, true, k);
-        load16<T>(reinterpret_cast<const T*>(p.cache.v_tail) + at, true, v);
-    } else {
+        transpose_bytes(words);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0;
+        for (int i = 0; i < 4; ++i) v[i] = values4<T>(words[i], v_scale);
+    } else {
+        const size_t tail = (static_cast<size_t>(pair) * 2 + (block & 1)) * kKvBlock * D;
+        const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + tail + slot * D + d0;
+        const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + tail + quad * 4 * D + v_d0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            k[i] = block * kKvBlock + slot < length ? reinterpret_cast<const uint2*>(k_tail)[i] : make_uint2(0u, 0u);
+            v[i] = block * kKvBlock + quad * 4 + i < length ? *reinterpret_cast<const uint2*>(v_tail + i * D) : make_uint2(0u, 0u);
+        }
     }
-    if (row < 0 || row >= p.tokens) return;
-    const size_t at = ((static_cast<size_t>(b) * p.tokens + row) * p.cache.kv_heads + head) * D + d0;
-    uint4* to_k = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.k_out) + at);
-    uint4* to_v = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.v_out) + at);
-    __stcs(to_k, make_uint4(k[0], k[1], k[2], k[3]));
-    __stcs(to_k + 1, make_uint4(k[4], k[5], k[6], k[7]));
-    __stcs(to_v, make_uint4(v[0], v[1], v[2], v[3]));
-    __stcs(to_v + 1, make_uint4(v[4], v[5], v[6], v[7]));
+    const long long before = block * kKvBlock - first;                  // rows of the output in front of this block's
+    const size_t row_numbers = static_cast<size_t>(p.cache.kv_heads) * D;
+    const size_t out = (static_cast<size_t>(b) * p.tokens * p.cache.kv_heads + head) * D;
+    if (before + slot >= 0 && before + slot < p.tokens) {
+        uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.k_out) + out + (before + slot) * row_numbers + d0);
+        __stcs(to, make_uint4(k[0].x, k[0].y, k[1].x, k[1].y));
+        __stcs(to + 1, make_uint4(k[2].x, k[2].y, k[3].x, k[3].y));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long row = before + quad * 4 + i;
+        if (row < 0 || row >= p.tokens) continue;
+        __stcs(reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.v_out) + out + row * row_numbers + v_d0), v[i]);
+    }
 }
 
 bool wide_rows(const w4a16_rows& r) {
@@ -485,9 +585,11 @@ RowView view_of(const w4a16_rows& r) {
 }
 
 RotaryRows rotary_rows(const w4a16_rotary_spec& spec, const w4a16_rows& in, const w4a16_rows& out, int head_dim) {
-    RotaryRows rows{view_of(in), view_of(out), head_dim, spec.rotary_dim, spec.interleaved != 0, false, in.data == out.data};
+    RotaryRows rows{view_of(in), view_of(out), head_dim, spec.rotary_dim, spec.interleaved != 0, false, in.data == out.data, 0, 0};
     rows.wide = wide_rows(in) && wide_rows(out) && head_dim % 8 == 0 &&
                 (spec.interleaved ? spec.rotary_dim : spec.rotary_dim / 2) % 8 == 0 && (head_dim - spec.rotary_dim) % 8 == 0;
+    rows.pieces = spec.rotary_dim / (spec.interleaved ? 8 : 16) + (rows.in_place ? 0 : (head_dim - spec.rotary_dim) / 8);
+    while (1 << rows.piece_bits < rows.pieces) ++rows.piece_bits;
     return rows;
 }
 
@@ -534,8 +636,9 @@ int launch_kv_append(const w4a16_kv8_cache& cache, const w4a16_rows& k, const w4
     p.wide = wide_rows(k) && wide_rows(v);
     // (tokens beyond the cache are refused on the device; here they would only make CTAs without work)
     const int64_t at_most = tokens < cache.max_len ? tokens : cache.max_len;
-    p.chunks = static_cast<int>((at_most + 2 * kKvBlock - 2) / kKvBlock);
-    int64_t ctas = static_cast<int64_t>(cache.batch) * cache.kv_heads * p.chunks;
+    const int64_t pairs = static_cast<int64_t>(cache.batch) * cache.kv_heads, touched = (at_most + 2 * kKvBlock - 2) / kKvBlock;
+    p.chunks = static_cast<int>(std::min(touched, std::max<int64_t>(1, kAppendCtas / pairs)));
+    int64_t ctas = pairs * p.chunks;
     size_t smem = 0;
     if (rotary != nullptr) {
         p.inv_freq = rotary->inv_freq;
