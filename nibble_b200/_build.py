@@ -29,7 +29,7 @@ CHECKED_LIB = PKG / "libw4a16_b200_checked.so"
 TORCH_LIB = PKG / "_C.so"
 
 CUDA_SOURCES = ["capi.cu", "linear_mma.cu", "linear_mma_groups.cu", "linear_generic.cu", "dequantize.cu", "linear_static_scratch.cu", "linear_gemm.cu", "linear_gemm_pair.cu", "quantize.cu", "decode_ops.cu", "decode_persistent.cu",
-                "kv_cache.cu", "kv_attention.cu"]
+                "kv_cache.cu", "kv_attention.cu", "kv_prefill.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++20", "-lineinfo",

@@ -570,9 +570,16 @@ static bool fits_queries(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t 
     return q_heads > 0 && q_heads % cache->kv_heads == 0 && tokens >= 0 && tokens <= INT32_MAX / 64 / q_heads;
 }
 
+// Whether a call goes to the tensor cores' larger tiles.
+static bool many_queries(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t tokens) {
+    const int64_t rows = tokens * (q_heads / cache->kv_heads);
+    return rows > 64;
+}
+
 size_t w4a16_kv8_attention_workspace_bytes(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t tokens) {
     if (check_cache(cache) != W4A16_OK || !fits_queries(cache, q_heads, tokens) || tokens == 0) return 0;
-    return w4a16::kv_attention_workspace_bytes(*cache, q_heads, tokens);
+    return many_queries(cache, q_heads, tokens) ? w4a16::kv_prefill_workspace_bytes(*cache, q_heads, tokens)
+                                                : w4a16::kv_attention_workspace_bytes(*cache, q_heads, tokens);
 }
 
 int w4a16_kv8_attention(const w4a16_kv8_cache* cache, const w4a16_rows* q, void* out, int32_t q_heads, int64_t tokens,
@@ -584,9 +591,10 @@ int w4a16_kv8_attention(const w4a16_kv8_cache* cache, const w4a16_rows* q, void*
     if (const int status = check_rows(q); status != W4A16_OK) return status;
     if (out == nullptr || lengths == nullptr) return W4A16_ERR_NULL_POINTER;
     if (!aligned16(out) || !aligned16(workspace)) return W4A16_ERR_MISALIGNED;
-    return w4a16::launch_kv_attention(*cache, *q, out, q_heads, tokens, reinterpret_cast<const long long*>(lengths),
-                                      reinterpret_cast<const long long*>(counts), softmax_scale, workspace, workspace_bytes,
-                                      programmatic(flags), reinterpret_cast<cudaStream_t>(stream));
+    auto launch = many_queries(cache, q_heads, tokens) ? w4a16::launch_kv_prefill : w4a16::launch_kv_attention;
+    return launch(*cache, *q, out, q_heads, tokens, reinterpret_cast<const long long*>(lengths),
+                  reinterpret_cast<const long long*>(counts), softmax_scale, workspace, workspace_bytes, programmatic(flags),
+                  reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

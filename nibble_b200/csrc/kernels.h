@@ -107,7 +107,8 @@ int decode_plan_build(const w4a16_decode_model* model, void* plan, size_t plan_b
                       w4a16_decode_plan_info* info, cudaStream_t stream);
 int launch_decode_step(const void* plan, int32_t n_ops, int32_t grid, int32_t head_dim, uint32_t smem_bytes, cudaStream_t stream);
 
-// Rotary positions, and the 8-bit key/value cache: tokens written, read back (kv_cache.cu) and attended over (kv_attention.cu).
+// Rotary positions, and the 8-bit key/value cache: tokens written, read back (kv_cache.cu) and attended over, by few queries
+// (kv_attention.cu) or by many (kv_prefill.cu).
 int launch_rotary(const w4a16_rotary_spec& spec, const w4a16_rows& x, const w4a16_rows& out, int64_t batch, int64_t tokens, int heads,
                   int head_dim, const long long* positions, bool bf16, bool programmatic, cudaStream_t stream);
 int launch_kv_append(const w4a16_kv8_cache& cache, const w4a16_rows& k, const w4a16_rows& v, int64_t tokens, const long long* start,
@@ -119,6 +120,10 @@ size_t kv_attention_workspace_bytes(const w4a16_kv8_cache& cache, int q_heads, i
 int launch_kv_attention(const w4a16_kv8_cache& cache, const w4a16_rows& q, void* out, int q_heads, int64_t tokens,
                         const long long* lengths, const long long* counts, float softmax_scale, void* workspace, size_t workspace_bytes,
                         bool programmatic, cudaStream_t stream);
+size_t kv_prefill_workspace_bytes(const w4a16_kv8_cache& cache, int q_heads, int64_t tokens);
+int launch_kv_prefill(const w4a16_kv8_cache& cache, const w4a16_rows& q, void* out, int q_heads, int64_t tokens,
+                      const long long* lengths, const long long* counts, float softmax_scale, void* workspace, size_t workspace_bytes,
+                      bool programmatic, cudaStream_t stream);
 
 // Quantise + pack on the device (quantize.cu): FP16 or FP32 weights -> packed codes and FP16 scales.
 int launch_quantize_pack(const void* weights, bool is_f32, uint8_t* packed, __half* scales, int64_t N, int64_t K,

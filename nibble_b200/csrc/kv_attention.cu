@@ -446,8 +446,8 @@ kv_attention_kernel(const AttentionParams p) {
             top[n][0] = top[n][1] = kNone;
             sum[n][0] = sum[n][1] = 0.0f;
         }
-        float unit_scale = 1.0e-30f;               // of the accumulators: values are acc * unit_scale / kHeadroom
-        float per_scale = kHeadroom / 1.0e-30f;    // kHeadroom / unit_scale
+        float unit_scale = 0x1p-100f;               // of the accumulators: values are acc * unit_scale / kHeadroom
+        float per_scale = kHeadroom / 0x1p-100f;    // kHeadroom / unit_scale
 
         // Scores of a block, [group of 16 tokens][token 2g: rows 2c, 2c + 1; token 2g + 1: the same], and the probabilities that come
         // of them, as operands of the second product: row g, tokens 4c, 4c + 2 and 4c + 1, 4c + 3 of each group.
@@ -482,10 +482,12 @@ kv_attention_kernel(const AttentionParams p) {
             }
             const bool new_unit = v_scale > kMaxRatio * unit_scale;
             if (__any_sync(0xffffffffu, lag || new_unit)) {
-                const float unit_change = new_unit ? unit_scale / v_scale : 1.0f;
-                if (new_unit) {
-                    unit_scale = v_scale;
-                    per_scale = kHeadroom / v_scale;
+                float unit_change = 1.0f;
+                if (new_unit) {                     // (a power of two, which has no part in how probabilities are rounded)
+                    const float now = next_power(v_scale);
+                    unit_change = unit_scale / now;
+                    unit_scale = now;
+                    per_scale = kHeadroom / now;
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {

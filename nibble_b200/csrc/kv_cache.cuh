@@ -118,6 +118,9 @@ __device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The power of two at or above a positive normal number.
+__device__ __forceinline__ float next_power(float x) { return __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0xff800000u); }
+
 template <typename... Params, typename... Args>
 int kv_launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, bool programmatic, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t launch = {};

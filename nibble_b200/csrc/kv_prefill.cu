@@ -1,0 +1,813 @@
+// Attention of many new tokens (a prompt, or a chunk of one) over the 8-bit cache, on the 5th-generation tensor cores.
+//
+// The same definition as kv_attention.cu, and the same arithmetic: codes are exact FP16 integers in both products, the keys' scales
+// multiply FP32 scores, the values' scales enter the probabilities before those are rounded to FP16 (relative to the largest scale
+// of the piece of work, times 2^10), maxima, sums and outputs are FP32.
+//
+// A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
+// against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's fourteen warps, one CTA per SM:
+//   warps 0-3, 4-7   softmax of tile A and of tile B: a thread per row.  Stages its row of queries, then in every step takes the
+//                    row's 128 scores out of TMEM twice (their maximum, then the exponentials), leaves the probabilities in TMEM in
+//                    the scores' place, and in the end the output.
+//   warps 8-11       make FP16 operands in shared memory of a block's codes each, swizzled by 128 bytes: keys [token][d], values
+//                    [d][token]; of the block that is being filled, of its 16-bit numbers; zeros behind the last.
+//   warp 12          allocates TMEM and issues the MMAs: S = Q K^T with both operands in shared memory, O += P V with P in TMEM.
+// TMEM: scores (and probabilities) of A and B, outputs of A and B, 128 columns each.
+//
+// The order within a step is O_A, S_A of the next step, O_B, S_B of the next step: while one tile's softmax runs, the tensor core works
+// on the other's.  Bounds: MMAs and exponentials take the same 2048 clocks of a step on paper; shared memory (operands written once
+// and read by two MMAs each) is close behind.
+//
+// Work split.  As many whole units as make full rounds of the CTAs; what is left of the last round is cut along the tokens, so that
+// all CTAs have a piece, and a small kernel adds the pieces up.  (2048 tokens of 64 heads on 8: 512 units, 148 CTAs.)
+//
+// Every wait is bounded; one that gives up sets the cache's status word, later ones return at once, and the CTA still runs to its
+// TMEM deallocation.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.h"
+#include "kv_cache.cuh"
+#include "per_device.h"
+#include "tcgen05.cuh"
+#include "unpack.cuh"
+
+namespace w4a16 {
+namespace {
+
+constexpr int kRows = 128;                      // of a tile
+constexpr int kUnitRows = 2 * kRows;
+constexpr int kStepBlocks = 4;
+constexpr int kStepTokens = kStepBlocks * kKvBlock;
+constexpr int kSoftmaxWarps = 8, kDequantWarps = 4;
+constexpr int kMmaWarp = kSoftmaxWarps + kDequantWarps;
+constexpr int kPrefillThreads = (kMmaWarp + 1) * 32;
+constexpr float kNone = -1.0e30f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHeadroom = 1024.0f;
+constexpr float kMaxLag = 3.0f;                 // how far (log2) a maximum may rise before outputs are rescaled
+
+struct PrefillParams {
+    KvCache cache;
+    const char* q;
+    long long q_batch, q_token, q_head;
+    bool q_wide;
+    char* out;                                   // [batch][tokens][q heads][D]
+    int tokens, q_heads, group;
+    float per_group;                             // 1 / group
+    int row_tiles;                               // units of a sequence and head: as many as `tokens` queries make
+    const long long* lengths;
+    const long long* counts;
+    float scale;                                 // |softmax scale| * log2 e
+    bool negate;                                 // the softmax scale is negative: the queries are taken with the other sign
+    float* parts;                                // [piece][256][D + 4]: sums, maximum, sum of weights
+    int units, whole, pieces;                    // units in all; those of full rounds; pieces of each of the others
+};
+
+__device__ __forceinline__ int by_group(const PrefillParams& p, int row) {
+    int quotient = static_cast<int>(static_cast<float>(row) * p.per_group);
+    const int rest = row - quotient * p.group;
+    if (rest < 0) --quotient;
+    if (rest >= p.group) ++quotient;
+    return quotient;
+}
+
+// A unit or a piece of one: steps [begin, stop) of its visible tokens.
+struct Work {
+    int b, head, first_row, rows, length, count;      // rows: of the sequence, from row 0 of the unit's tile 0 on
+    int begin, stop;
+    int full, held;                                   // full blocks, tokens of the block that is being filled
+    int piece;                                        // -1: a whole unit
+};
+
+__device__ __forceinline__ Work unit_of(const PrefillParams& p, int unit, int piece) {
+    Work w;
+    const int pairs = p.cache.batch * p.cache.kv_heads;
+    const int tile = p.row_tiles - 1 - unit / pairs;      // the longest first
+    const int pair = unit % pairs;
+    w.b = pair / p.cache.kv_heads;
+    w.head = pair - w.b * p.cache.kv_heads;
+    w.first_row = tile * kUnitRows;
+    w.piece = piece;
+    const long long length = p.lengths[w.b], count = p.counts == nullptr ? p.tokens : p.counts[w.b];
+    const bool sound = length >= 0 && length <= p.cache.max_len && count >= 0 && count <= p.tokens;
+    if (!sound && threadIdx.x == 0) atomicOr(p.cache.status, kKvBadLength);
+    w.length = sound ? static_cast<int>(length) : 0;
+    w.count = sound ? static_cast<int>(count) : 0;
+    w.rows = w.count * p.group;
+    w.full = w.length / kKvBlock;
+    w.held = w.length - w.full * kKvBlock;
+    const int last_row = min(w.rows, w.first_row + kUnitRows) - 1;
+    const int last = last_row >= w.first_row ? w.length - w.count + by_group(p, last_row) : -1;      // position of its query
+    const int steps = last < 0 ? 0 : last / kStepTokens + 1;
+    w.begin = piece < 0 ? 0 : static_cast<int>(static_cast<long long>(steps) * piece / p.pieces);
+    w.stop = piece < 0 ? steps : static_cast<int>(static_cast<long long>(steps) * (piece + 1) / p.pieces);
+    return w;
+}
+
+// This CTA's n-th work; false behind the last.
+__device__ __forceinline__ bool work_of(const PrefillParams& p, int n, Work& w) {
+    const int unit = static_cast<int>(blockIdx.x) + n * static_cast<int>(gridDim.x);
+    if (unit < p.whole) {
+        w = unit_of(p, unit, -1);
+        return true;
+    }
+    if (n * static_cast<int>(gridDim.x) != p.whole || static_cast<int>(blockIdx.x) >= (p.units - p.whole) * p.pieces) return false;
+    w = unit_of(p, p.whole + blockIdx.x / p.pieces, blockIdx.x % p.pieces);
+    return true;
+}
+
+template <int D>
+struct PrefillShape {
+    static constexpr int kHalves = D / 64;                              // 128-byte halves of a row of keys or queries
+    static constexpr int kQueryBytes = kRows * D * 2;                   // of a tile
+    static constexpr int kKeyBytes = kStepTokens * D * 2, kValueBytes = D * kStepTokens * 2;      // of a step
+    static constexpr int kKeysAt = 2 * kQueryBytes, kValuesAt = kKeysAt + 2 * kKeyBytes;
+    static constexpr size_t kSharedBytes = kValuesAt + 2 * kValueBytes + 1024;                    // and to align it
+};
+
+struct PrefillBarriers {
+    unsigned long long q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float power_for(float top, float& inverse) {
+    const int exponent = top > 0.0f ? max(-100, min(100, 9 - ilogbf(top))) : 0;
+    inverse = __int_as_float((127 - exponent) << 23);
+    return __int_as_float((127 + exponent) << 23);
+}
+__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& even, uint32_t& odd) {
+    even = hsub2_u32(and_xor(word, 0x00ff00ffu, 0x64806480u), 0x64806480u);
+    odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
+}
+
+// D (TMEM) += A (shared memory) x B (shared memory).
+__device__ __forceinline__ void umma_f16_shared(unsigned tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instr_desc,
+                                                uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instr_desc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 columns of this thread's TMEM lane, there once this returns; and the other way, sixteen, on their way.
+__device__ __forceinline__ void tmem_load32(unsigned address, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+          "=r"(v[30]), "=r"(v[31])
+        : "r"(address)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(unsigned address, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(address),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+// 128-byte swizzle: where 16-byte chunk c of row r of a [rows][128 bytes] tile lies.
+__device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+// What a tail's numbers are multiplied with to become FP16, and the scale that stands for it.  FP16 ones stay as they are.
+template <typename T>
+__device__ __forceinline__ float tail_power(float top, float& scale) {
+    if constexpr (std::is_same<T, __half>::value) {
+        scale = 1.0f;
+        return 1.0f;
+    }
+    return power_for(top, scale);
+}
+
+// Largest finite magnitude of a warp's share of `numbers` (an even number of them), by all lanes.
+template <typename T>
+__device__ __forceinline__ float finite_top(const T* numbers, int count, int first, int step) {
+    float top = 0.0f;
+    for (int i = first; i < count / 2; i += step) {
+        const float2 f = widen2<T>(reinterpret_cast<const uint32_t*>(numbers)[i]);
+        const float a = fabsf(f.x), b = fabsf(f.y);
+        if (a <= 3.4028235e38f) top = fmaxf(top, a);
+        if (b <= 3.4028235e38f) top = fmaxf(top, b);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefillThreads, 1)
+kv_prefill_kernel(const PrefillParams p) {
+    using Shape = PrefillShape<D>;
+    constexpr int kHalves = Shape::kHalves;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr unsigned kOutputs = 256;                   // TMEM columns: scores A, B at 0 and 128, outputs A, B from here on
+    extern __shared__ uint8_t unaligned[];
+    __shared__ __align__(8) PrefillBarriers bars;
+    __shared__ unsigned tmem_word;
+    // Of a step's blocks, keys' and values', four steps: operands are made two steps ahead of the scores, and those of step n + 2 are
+    // formed only when both tiles' probabilities of step n + 1 are there.
+    __shared__ float scales[4][2][kStepBlocks];
+    __shared__ float tops[2][4];
+    __shared__ int odd_tail[4];                          // number of the work (plus one) whose tail's values have an infinity or NaN
+    uint8_t* const shared = unaligned + (1024 - (smem_u32(unaligned) & 1023)) % 1024;
+    pdl_wait_for_upstream();
+    pdl_release_downstream();
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    if (tid == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(smem_u32(&bars.q_full[t]), 4);
+            mbar_init(smem_u32(&bars.k_full[t]), kDequantWarps);
+            mbar_init(smem_u32(&bars.v_full[t]), kDequantWarps);
+            mbar_init(smem_u32(&bars.k_empty[t]), 1);
+            mbar_init(smem_u32(&bars.v_empty[t]), 1);
+            mbar_init(smem_u32(&bars.s_full[t]), 1);
+            mbar_init(smem_u32(&bars.p_full[t]), 4);
+            mbar_init(smem_u32(&bars.o_done[t]), 1);
+        }
+        for (int i = 0; i < 4; ++i) odd_tail[i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_word)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = tmem_word;
+    bool healthy = true;
+    // Waits for phase number `n` of a barrier; by a converged warp, all of whose lanes then know whether it came.
+    auto wait = [&](unsigned long long& bar, int n) {
+        if (healthy) healthy = mbar_wait(smem_u32(&bar), n & 1, kKvGaveUp, p.cache.status);
+        healthy = __all_sync(0xffffffffu, healthy);
+    };
+    // This warp's arrival, behind its writes to shared memory for the tensor core.
+    auto arrive = [&](unsigned long long& bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar));
+    };
+
+    if (warp < kSoftmaxWarps) {
+        // ---------------------------------------------------------------- softmax: one row a thread
+        const int t = warp / 4, row_in_tile = tid & (kRows - 1);
+        const unsigned lanes = static_cast<unsigned>(warp % 4 * 32) << 16;
+        const unsigned score_at = tmem + t * 128 + lanes, out_at = tmem + kOutputs + t * 128 + lanes;
+        int steps_done = 0, steps_of_all = 0;            // of this tile; of both, up to this work
+        Work w;
+        for (int n = 0; work_of(p, n, w); steps_of_all += w.stop - w.begin, ++n) {
+            const int row = w.first_row + t * kRows + row_in_tile, token = by_group(p, row);
+            const int place = row < w.rows ? w.length - w.count + token : -1;
+            const int q_head = w.head * p.group + row - token * p.group;
+            const size_t pair = static_cast<size_t>(w.b) * p.cache.kv_heads + w.head;
+            const bool active = w.stop > w.begin && w.rows > w.first_row + t * kRows;      // this tile has rows, and they see something
+            const bool has_tail = active && w.held > 0 && w.stop * kStepBlocks > w.full;
+            const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (w.full & 1)) * kKvBlock * D;
+            float top = kNone, sum = 0.0f, unit_scale = 0.0f, q_scale = p.scale;
+            if (active) {
+                // the row of queries: [half][row][128 bytes], dims in the order of the codes' bytes
+                uint8_t* const to = shared + t * Shape::kQueryBytes;
+                const T* from = reinterpret_cast<const T*>(p.q) + w.b * p.q_batch + token * p.q_token + q_head * p.q_head;
+                const uint32_t sign = p.negate ? 0x80008000u : 0u;
+                auto load = [&](int chunk, uint32_t (&raw)[4]) {         // eight dims
+                    raw[0] = raw[1] = raw[2] = raw[3] = 0;
+                    if (row >= w.rows) return;
+                    if (p.q_wide) {
+                        const uint4 four = *reinterpret_cast<const uint4*>(from + chunk * 8);
+                        raw[0] = four.x; raw[1] = four.y; raw[2] = four.z; raw[3] = four.w;
+                    } else {
+                        const uint16_t* h = reinterpret_cast<const uint16_t*>(from + chunk * 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) raw[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
+                    }
+                };
+                float by = 1.0f;
+                if constexpr (kBf16) {
+                    // BF16 becomes FP16 by a power of two of the row's own: a number keeps all its bits unless it is 2^-23 of the
+                    // row's largest or less
+                    uint32_t largest = 0;
+                    for (int chunk = 0; chunk < D / 8; ++chunk) {
+                        uint32_t raw[4];
+                        load(chunk, raw);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) largest = max(largest, max(raw[i] << 16 & 0x7fffffffu, raw[i] & 0x7fff0000u));
+                    }
+                    float back;
+                    by = power_for(__uint_as_float(min(largest, 0x7f7f0000u)), back);
+                    q_scale *= back;
+                }
+#pragma unroll 4
+                for (int chunk = 0; chunk < D / 8; ++chunk) {
+                    uint32_t raw[4];
+                    load(chunk, raw);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (kBf16) {
+                            const float2 f = widen2<T>(raw[i]);
+                            raw[i] = pack_half(f.x * by, f.y * by);
+                        }
+                        raw[i] ^= sign;
+                    }
+                    *reinterpret_cast<uint4*>(to + chunk / 8 * (kRows * 128) + swizzled(row_in_tile, chunk % 8)) =
+                        make_uint4(prmt(raw[0], raw[1], 0x5410), prmt(raw[0], raw[1], 0x7632), prmt(raw[2], raw[3], 0x5410), prmt(raw[2], raw[3], 0x7632));
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(bars.q_full[t]);
+                // What the accumulator's numbers are relative to: the largest scale of the values that this work meets.  Rounded up to a
+                // power of two, so that what a row does not see has no part in how its probabilities are rounded.
+                const float* v_scales = p.cache.v_scales + pair * p.cache.blocks;
+                for (int block = w.begin * kStepBlocks + row_in_tile; block < min(w.stop * kStepBlocks, w.full); block += kRows) {
+                    unit_scale = fmaxf(unit_scale, v_scales[block]);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) unit_scale = fmaxf(unit_scale, __shfl_xor_sync(0xffffffffu, unit_scale, o));
+                if (has_tail) {
+                    float scale;
+                    tail_power<T>(kBf16 ? finite_top(v_tail, w.held * D, lane, 32) : 0.0f, scale);
+                    unit_scale = fmaxf(unit_scale, scale);
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");      // (the last work's have been read)
+                if (lane == 0) tops[t][warp % 4] = unit_scale;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+                unit_scale = next_power(fmaxf(fmaxf(fmaxf(tops[t][0], tops[t][1]), fmaxf(tops[t][2], tops[t][3])), 1.0e-30f));
+            }
+            const float per_scale = kHeadroom / unit_scale;
+            const int lowest = __reduce_min_sync(0xffffffffu, row < w.rows ? place : INT_MAX);
+            for (int step = w.begin; active && step < w.stop; ++step, ++steps_done) {
+                wait(bars.s_full[t], steps_done);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float* k_scale = scales[(steps_of_all + step - w.begin) & 3][0];
+                const float* v_scale = scales[(steps_of_all + step - w.begin) & 3][1];
+                const bool masked = (step + 1) * kStepTokens - 1 > lowest;
+                // the largest score (a score's factor is not negative)
+                float more = kNone;
+#pragma unroll 1
+                for (int block = 0; block < kStepBlocks; ++block) {
+                    uint32_t s[32];
+                    tmem_load32(score_at + block * 32, s);
+                    float largest = -INFINITY;
+                    if (masked) {
+                        const int last = place - (step * kStepBlocks + block) * kKvBlock;      // tokens of the block up to it are seen
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int at = (i & ~3) | (i & 1) << 1 | (i & 2) >> 1;            // columns of a four: tokens 0, 2, 1, 3
+                            if (at <= last) largest = fmaxf(largest, __uint_as_float(s[i]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) largest = fmaxf(largest, __uint_as_float(s[i]));
+                    }
+                    more = fmaxf(more, largest * (k_scale[block] * q_scale));
+                }
+                const bool fresh = top == kNone;
+                const bool rises = fresh ? more > kNone : more > top + kMaxLag;
+                float shrink = 1.0f;
+                if (rises) {
+                    shrink = fresh ? 1.0f : exp2_fast(top - more);
+                    top = more;
+                    sum *= shrink;
+                }
+                if (step > w.begin && __any_sync(0xffffffffu, shrink != 1.0f)) {
+                    wait(bars.o_done[t], steps_done - 1);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        uint32_t o[32], half[16];
+                        tmem_load32(out_at + d, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) half[i] = o[h * 16 + i];
+                            tmem_store16(out_at + d + h * 16, half);
+                        }
+                    }
+                }
+                const float from = fresh && !rises ? 0.0f : top;      // (a row that has seen nothing yet: all it meets is masked)
+#pragma unroll 1
+                for (int block = 0; block < kStepBlocks; ++block) {
+                    uint32_t s[32], packed[16];
+                    tmem_load32(score_at + block * 32, s);
+                    // the value's scale goes into the exponent, and out of the sum again
+                    float weight = v_scale[block] * per_scale;
+                    if (weight < 0x1p-80f) weight = 0x1p-80f;
+                    const float by = k_scale[block] * q_scale, with = log2f(weight) - from;
+                    const int last = place - (step * kStepBlocks + block) * kKvBlock;
+                    float block_sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float e[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int j = i + h, at = (j & ~3) | (j & 1) << 1 | (j & 2) >> 1;
+                            float x = fmaf(__uint_as_float(s[j]), by, with);
+                            if (masked && at > last) x = -INFINITY;
+                            e[h] = exp2_fast(x);
+                            block_sum[h] += e[h];
+                        }
+                        packed[i / 2] = pack_half(e[0], e[1]);
+                    }
+                    if (last >= 0) sum = fmaf(block_sum[0] + block_sum[1], __fdividef(1.0f, weight), sum);      // (the scale may be NaN)
+                    tmem_store16(score_at + block * 16, packed);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                arrive(bars.p_full[t]);
+            }
+            // the rows' results
+            const bool to_part = w.piece >= 0;
+            float* part = p.parts + (static_cast<size_t>(blockIdx.x) * kUnitRows + t * kRows + row_in_tile) * (D + 4);
+            const bool write = to_part ? active : row < p.tokens * p.group;
+            T* out = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(w.b) * p.tokens + token) * p.q_heads + q_head) * D;
+            const float by = to_part ? unit_scale / kHeadroom : sum > 0.0f ? unit_scale / kHeadroom / sum : sum;
+            bool odd = false;
+            if (active) {
+                wait(bars.o_done[t], steps_done - 1);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                odd = has_tail && *const_cast<volatile int*>(&odd_tail[n & 3]) == n + 1;
+            }
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+                uint32_t o[32];
+                if (active) tmem_load32(out_at + d, o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = active && row < w.rows ? __float_as_uint(__uint_as_float(o[i]) * by) : 0u;
+                if (odd) {                               // infinities and NaN of the tail, which were kept out of the products
+                    for (int i = 0; i < w.held; ++i) {
+                        if (w.full * kKvBlock + i > place) break;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float v = widen<T>(v_tail[i * D + d + e]);
+                            if (!(fabsf(v) <= 3.4028235e38f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + v);
+                        }
+                    }
+                }
+                if (!write) continue;
+                if (to_part) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part + d + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        auto two = [&](int j) { return narrow2<T>(__uint_as_float(o[i + j]), __uint_as_float(o[i + j + 1])); };
+                        *reinterpret_cast<uint4*>(out + d + i) = make_uint4(two(0), two(2), two(4), two(6));
+                    }
+                }
+            }
+            if (write && to_part) *reinterpret_cast<float2*>(part + D) = make_float2(top, sum);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // (the next work's first arrival lets O be overwritten)
+        }
+    } else if (warp < kMmaWarp) {
+        // ---------------------------------------------------------------- operands: one block of a step a warp
+        const int mine = warp - kSoftmaxWarps, g = lane >> 2, c = lane & 3;
+        constexpr int kVectors = D / 16;                 // 16-byte pieces of a block's keys, and values, for a lane
+        uint4 codes[kVectors];
+        // Step number `steps` of all, this CTA's works one after the other.
+        int steps = 0;
+        Work w;
+        for (int n = 0; work_of(p, n, w); ++n) {
+            const size_t pair = static_cast<size_t>(w.b) * p.cache.kv_heads + w.head;
+            for (int step = w.begin; step < w.stop; ++step, ++steps) {
+                const int block = step * kStepBlocks + mine, stage = steps & 1;
+                const bool coded = block < w.full, tail = block == w.full && w.held > 0;
+                const size_t at = (pair * p.cache.blocks + block) * (kKvBlock * D) + lane * 16;
+                const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + (pair * 2 + (block & 1)) * kKvBlock * D;
+                const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (block & 1)) * kKvBlock * D;
+                float k_scale = 0.0f, v_scale = 0.0f, k_by = 1.0f, v_by = 1.0f;
+                if (coded) {
+                    k_scale = p.cache.k_scales[pair * p.cache.blocks + block];
+                    v_scale = p.cache.v_scales[pair * p.cache.blocks + block];
+#pragma unroll
+                    for (int i = 0; i < kVectors; ++i) codes[i] = *reinterpret_cast<const uint4*>(p.cache.k_codes + at + i * 512);
+                } else if (tail) {
+                    k_by = tail_power<T>(kBf16 ? finite_top(k_tail, w.held * D, lane, 32) : 0.0f, k_scale);
+                    v_by = tail_power<T>(kBf16 ? finite_top(v_tail, w.held * D, lane, 32) : 0.0f, v_scale);
+                }
+                auto to_half = [&](uint32_t word, float by) {
+                    if constexpr (!kBf16) return word;
+                    const float2 f = widen2<T>(word);
+                    return pack_half(f.x * by, f.y * by);
+                };
+                // keys: row of a token, four tokens in the order 0, 2, 1, 3
+                if (steps >= 2) wait(bars.k_empty[stage], steps / 2 - 1);
+                {
+                    uint8_t* const to = shared + Shape::kKeysAt + stage * Shape::kKeyBytes;
+#pragma unroll
+                    for (int i = 0; i < kVectors; ++i) {         // [group of 16 tokens][parity][half of the dims]
+                        const int half = i % kHalves, parity = i / kHalves % 2, group = i / kHalves / 2;
+                        const int row = mine * 32 + group * 16 + g / 2 * 4 + g % 2 + parity * 2;
+                        uint32_t words[8];
+                        if (coded) {
+                            codes_to_half(codes[i].x, words[0], words[1]);
+                            codes_to_half(codes[i].y, words[2], words[3]);
+                            codes_to_half(codes[i].z, words[4], words[5]);
+                            codes_to_half(codes[i].w, words[6], words[7]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) words[e] = 0;
+                            const int token = group * 16 + g * 2 + parity;
+                            if (tail && token < w.held) {
+                                const uint32_t* raw = reinterpret_cast<const uint32_t*>(k_tail + token * D + half * 64 + c * 16);
+#pragma unroll
+                                for (int e = 0; e < 8; e += 2) {
+                                    const uint32_t lo = to_half(raw[e], k_by), hi = to_half(raw[e + 1], k_by);
+                                    words[e] = prmt(lo, hi, 0x5410);
+                                    words[e + 1] = prmt(lo, hi, 0x7632);
+                                }
+                            }
+                        }
+                        uint8_t* const at_half = to + half * (kStepTokens * 128);
+                        *reinterpret_cast<uint4*>(at_half + swizzled(row, 2 * c)) = make_uint4(words[0], words[1], words[2], words[3]);
+                        *reinterpret_cast<uint4*>(at_half + swizzled(row, 2 * c + 1)) = make_uint4(words[4], words[5], words[6], words[7]);
+                    }
+                }
+                if (lane == 0) {
+                    scales[steps & 3][0][mine] = k_scale;
+                    scales[steps & 3][1][mine] = v_scale;
+                }
+                if (coded) {
+#pragma unroll
+                    for (int i = 0; i < kVectors; ++i) codes[i] = *reinterpret_cast<const uint4*>(p.cache.v_codes + at + i * 512);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(bars.k_full[stage]);
+                // values: row of a dim, tokens in the columns' order
+                if (steps >= 2) wait(bars.v_empty[stage], steps / 2 - 1);
+                uint8_t* const to = shared + Shape::kValuesAt + stage * Shape::kValueBytes + mine / 2 * (D * 128);
+                if (coded || !tail) {
+#pragma unroll
+                    for (int i = 0; i < kVectors; ++i) {         // sixteen dims: [half of them][group of 16 tokens]
+                        const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t even = 0, odd = 0;
+                            if (coded) codes_to_half(words[e], even, odd);
+                            const int d = i * 16 + e / 2 * 8 + g;
+                            *reinterpret_cast<uint2*>(to + swizzled(d, mine % 2 * 4 + e % 2 * 2 + c / 2) + c % 2 * 8) = make_uint2(even, odd);
+                        }
+                    }
+                } else {
+                    bool odd_values = false;
+                    for (int i = lane; i < 8 * (D / 8); i += 32) {      // eight dims of four tokens
+                        const int quad = i / (D / 8), d0 = i % (D / 8) * 8;
+                        uint32_t raw[4][4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint4 four = make_uint4(0u, 0u, 0u, 0u);
+                            if (quad * 4 + e < w.held) four = *reinterpret_cast<const uint4*>(v_tail + (quad * 4 + e) * D + d0);
+                            raw[e][0] = four.x; raw[e][1] = four.y; raw[e][2] = four.z; raw[e][3] = four.w;
+#pragma unroll
+                            for (int f = 0; f < 4; ++f) {
+                                const float2 v = widen2<T>(raw[e][f]);
+                                if (!(fabsf(v.x) <= 3.4028235e38f)) raw[e][f] &= 0xffff0000u, odd_values = true;
+                                if (!(fabsf(v.y) <= 3.4028235e38f)) raw[e][f] &= 0x0000ffffu, odd_values = true;
+                                raw[e][f] = to_half(raw[e][f], v_by);
+                            }
+                        }
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const unsigned pick = h == 0 ? 0x5410u : 0x7632u;
+                                const int chunk = mine % 2 * 4 + quad / 2;
+                                *reinterpret_cast<uint2*>(to + swizzled(d0 + 2 * f + h, chunk) + quad % 2 * 8) =
+                                    make_uint2(prmt(raw[0][f], raw[2][f], pick), prmt(raw[1][f], raw[3][f], pick));
+                            }
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, odd_values) && lane == 0) odd_tail[n & 3] = n + 1;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive(bars.v_full[stage]);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- MMAs
+        constexpr uint32_t kCommon = (1u << 4) | (static_cast<uint32_t>(kRows >> 4) << 24);      // FP32 sums of FP16, 128 rows, K-major
+        constexpr uint32_t kScoreDesc = kCommon | (static_cast<uint32_t>(kStepTokens >> 3) << 17);
+        constexpr uint32_t kOutputDesc = kCommon | (static_cast<uint32_t>(D >> 3) << 17);
+        const bool chosen = elect_one();
+        int steps = 0, works[2] = {0, 0}, tile_steps[2] = {0, 0};          // steps of all; works and steps of each tile
+        auto scores = [&](int t, int stage) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (chosen && healthy) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint64_t a = operand_desc(smem_u32(shared) + t * Shape::kQueryBytes + i / 4 * (kRows * 128) + i % 4 * 32);
+                    const uint64_t b = operand_desc(smem_u32(shared) + Shape::kKeysAt + stage * Shape::kKeyBytes + i / 4 * (kStepTokens * 128) + i % 4 * 32);
+                    umma_f16_shared(tmem + t * 128, a, b, kScoreDesc, i > 0 ? 1u : 0u);
+                }
+                umma_commit(smem_u32(&bars.s_full[t]));
+            }
+            __syncwarp();
+        };
+        Work w;
+        for (int n = 0; work_of(p, n, w); ++n) {
+            if (w.stop <= w.begin || w.rows <= w.first_row) continue;
+            const int tiles = w.rows > w.first_row + kRows ? 2 : 1;
+            const int first = steps;
+            for (int t = 0; t < tiles; ++t) {
+                wait(bars.q_full[t], works[t]++);
+                if (t == 0) wait(bars.k_full[steps & 1], steps / 2);
+                if (tile_steps[t] > 0) wait(bars.o_done[t], tile_steps[t] - 1);      // (the last probabilities lie where the scores go)
+                scores(t, steps & 1);
+            }
+            if (chosen && healthy) umma_commit(smem_u32(&bars.k_empty[steps & 1]));
+            __syncwarp();
+            for (int step = w.begin; step < w.stop; ++step, ++steps) {
+                const int stage = steps & 1;
+                const bool last = step + 1 == w.stop;
+                for (int t = 0; t < tiles; ++t) {
+                    if (t == 0) wait(bars.v_full[stage], steps / 2);
+                    wait(bars.p_full[t], tile_steps[t]);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (chosen && healthy) {
+#pragma unroll
+                        for (int i = 0; i < kStepTokens / 16; ++i) {
+                            const uint64_t b = operand_desc(smem_u32(shared) + Shape::kValuesAt + stage * Shape::kValueBytes + i / 4 * (D * 128) + i % 4 * 32);
+                            umma_f16_tmem_a(tmem + kOutputs + t * 128, tmem + t * 128 + i * 8, b, kOutputDesc, steps > first || i > 0 ? 1u : 0u);
+                        }
+                        umma_commit(smem_u32(&bars.o_done[t]));
+                        if (t == tiles - 1) umma_commit(smem_u32(&bars.v_empty[stage]));
+                    }
+                    __syncwarp();
+                    if (!last) {
+                        if (t == 0) wait(bars.k_full[(steps + 1) & 1], (steps + 1) / 2);
+                        wait(bars.o_done[t], tile_steps[t]);
+                        scores(t, (steps + 1) & 1);
+                        if (t == tiles - 1 && chosen && healthy) umma_commit(smem_u32(&bars.k_empty[(steps + 1) & 1]));
+                        __syncwarp();
+                    }
+                    ++tile_steps[t];
+                }
+            }
+        }
+        // nothing may be in flight when TMEM goes
+        for (int t = 0; t < 2; ++t) {
+            if (tile_steps[t] > 0) mbar_wait(smem_u32(&bars.o_done[t]), (tile_steps[t] - 1) & 1, kKvGaveUp, p.cache.status);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Adds up the pieces of the units that were cut; a warp for a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+kv_pieces_kernel(const PrefillParams p) {
+    pdl_wait_for_upstream();
+    pdl_release_downstream();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int unit = blockIdx.x / (kUnitRows / 4), in_unit = blockIdx.x % (kUnitRows / 4) * 4 + warp;
+    const Work first = unit_of(p, p.whole + unit, -1);
+    const int row = first.first_row + in_unit;
+    if (row >= p.tokens * p.group) return;
+    constexpr int kDims = D / 32;
+    float top = kNone, weight = 0.0f, acc[kDims];
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) acc[d] = 0.0f;
+    if (row < first.rows) {
+        for (int piece = 0; piece < p.pieces; ++piece) {
+            if (static_cast<long long>(first.stop) * piece / p.pieces == static_cast<long long>(first.stop) * (piece + 1) / p.pieces) continue;
+            const float* part = p.parts + (static_cast<size_t>(unit * p.pieces + piece) * kUnitRows + in_unit) * (D + 4);
+            const float2 state = *reinterpret_cast<const float2*>(part + D);
+            const float best = fmaxf(top, state.x), mine = exp2_fast(top - best), theirs = exp2_fast(state.x - best);
+            top = best;
+            weight = weight * mine + state.y * theirs;
+#pragma unroll
+            for (int d = 0; d < kDims; d += 2) {
+                const float2 two = *reinterpret_cast<const float2*>(part + lane * kDims + d);
+                acc[d] = acc[d] * mine + two.x * theirs;
+                acc[d + 1] = acc[d + 1] * mine + two.y * theirs;
+            }
+        }
+    }
+    const float by = weight > 0.0f ? 1.0f / weight : weight;
+    const int token = by_group(p, row), q_head = first.head * p.group + row - token * p.group;
+    T* to = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(first.b) * p.tokens + token) * p.q_heads + q_head) * D + lane * kDims;
+#pragma unroll
+    for (int d = 0; d < kDims; d += 2) *reinterpret_cast<uint32_t*>(to + d) = narrow2<T>(acc[d] * by, acc[d + 1] * by);
+}
+
+struct DeviceState {
+    int sms = 0;
+};
+
+template <typename T, int D>
+int allow_shared() {
+    return cudaFuncSetAttribute(kv_prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(PrefillShape<D>::kSharedBytes)) == cudaSuccess
+               ? 0
+               : W4A16_ERR_LAUNCH;
+}
+
+int device_state(const DeviceState** state) {
+    static PerDevice<DeviceState> devices;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return W4A16_ERR_LAUNCH;
+    return devices.get(device, [&](DeviceState& fresh) -> int {
+        if (cudaDeviceGetAttribute(&fresh.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return W4A16_ERR_LAUNCH;
+        const int allowed = allow_shared<__half, 64>() | allow_shared<__half, 128>() | allow_shared<__nv_bfloat16, 64>() |
+                            allow_shared<__nv_bfloat16, 128>();
+        return allowed != 0 ? W4A16_ERR_LAUNCH : 0;
+    }, state);
+}
+
+struct Split {
+    int64_t row_tiles, units, whole, pieces, grid;
+};
+
+Split split_of(const w4a16_kv8_cache& cache, int q_heads, int64_t tokens, int sms) {
+    Split s;
+    const int64_t rows = tokens * (q_heads / cache.kv_heads);
+    s.row_tiles = (rows + kUnitRows - 1) / kUnitRows;
+    s.units = s.row_tiles * cache.batch * cache.kv_heads;
+    s.whole = s.units / sms * sms;
+    const int64_t rest = s.units - s.whole;
+    // (a piece is worth two steps or more)
+    const int64_t steps = (cache.max_len + kStepTokens - 1) / kStepTokens;
+    s.pieces = rest > 0 ? std::max<int64_t>(1, std::min<int64_t>(sms / rest, steps / 2)) : 1;
+    s.grid = s.whole > 0 ? sms : rest * s.pieces;
+    return s;
+}
+
+}  // namespace
+
+size_t kv_prefill_workspace_bytes(const w4a16_kv8_cache& cache, int q_heads, int64_t tokens) {
+    const DeviceState* state = nullptr;
+    const Split s = split_of(cache, q_heads, tokens, device_state(&state) == 0 ? state->sms : 148);
+    return static_cast<size_t>((s.units - s.whole) * s.pieces) * kUnitRows * (cache.head_dim + 4) * sizeof(float);
+}
+
+int launch_kv_prefill(const w4a16_kv8_cache& cache, const w4a16_rows& q, void* out, int q_heads, int64_t tokens, const long long* lengths,
+                      const long long* counts, float softmax_scale, void* workspace, size_t workspace_bytes, bool programmatic,
+                      cudaStream_t stream) {
+    const DeviceState* state = nullptr;
+    if (const int status = device_state(&state); status != 0) return status;
+    const Split s = split_of(cache, q_heads, tokens, state->sms);
+    const int64_t group = q_heads / cache.kv_heads;
+    if (s.units > INT32_MAX / 2 || tokens * group >= 1 << 24) return W4A16_ERR_TOO_LARGE;
+    const int64_t rest = s.units - s.whole;
+    if (rest > 0 && (workspace == nullptr || workspace_bytes < kv_prefill_workspace_bytes(cache, q_heads, tokens))) return W4A16_ERR_WORKSPACE;
+    PrefillParams p{};
+    p.cache = kv_view(cache);
+    p.q = static_cast<const char*>(q.data);
+    p.q_batch = q.batch_stride;
+    p.q_token = q.token_stride;
+    p.q_head = q.head_stride;
+    p.q_wide = reinterpret_cast<uintptr_t>(q.data) % 16 == 0 && q.batch_stride % 8 == 0 && q.token_stride % 8 == 0 && q.head_stride % 8 == 0;
+    p.out = static_cast<char*>(out);
+    p.tokens = static_cast<int>(tokens);
+    p.q_heads = q_heads;
+    p.group = static_cast<int>(group);
+    p.per_group = 1.0f / static_cast<float>(group);
+    p.row_tiles = static_cast<int>(s.row_tiles);
+    p.lengths = lengths;
+    p.counts = counts;
+    p.scale = (softmax_scale < 0.0f ? -softmax_scale : softmax_scale) * kLog2e;
+    p.negate = softmax_scale < 0.0f;
+    p.parts = static_cast<float*>(workspace);
+    p.units = static_cast<int>(s.units);
+    p.whole = static_cast<int>(s.whole);
+    p.pieces = static_cast<int>(s.pieces);
+    const bool bf16 = cache.type == W4A16_TYPE_BF16;
+    auto run = [&](auto type, auto dims) {
+        using T = decltype(type);
+        constexpr int kD = decltype(dims)::value;
+        const int status = kv_launch(kv_prefill_kernel<T, kD>, dim3(static_cast<unsigned>(s.grid)), dim3(kPrefillThreads),
+                                     PrefillShape<kD>::kSharedBytes, programmatic, stream, p);
+        if (status != W4A16_OK || rest == 0) return status;
+        return kv_launch(kv_pieces_kernel<T, kD>, dim3(static_cast<unsigned>(rest * (kUnitRows / 4))), dim3(128), 0, true, stream, p);
+    };
+    using Small = std::integral_constant<int, 64>;
+    using Large = std::integral_constant<int, 128>;
+    if (cache.head_dim == 64) return bf16 ? run(__nv_bfloat16(), Small{}) : run(__half(), Small{});
+    return bf16 ? run(__nv_bfloat16(), Large{}) : run(__half(), Large{});
+}
+
+}  // namespace w4a16

@@ -1,6 +1,8 @@
 """The 8-bit cache, rotary positions and attention over the cache, in 64 bits from their definitions."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 BLOCK = 32
@@ -52,15 +54,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, length: int, co
     group = q_heads // k.shape[1]
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     weight = torch.zeros_like(out)
-    for i in range(count):
-        last = length - count + i
-        if last < 0:
-            continue
-        for head in range(k.shape[1]):
-            rows = q[i, head * group:(head + 1) * group].double()
-            p = torch.softmax(rows @ k[:last + 1, head].T * softmax_scale, -1)
-            out[i, head * group:(head + 1) * group] = p @ v[:last + 1, head]
-            weight[i, head * group:(head + 1) * group] = p @ v[:last + 1, head].abs()
+    last = length - count + torch.arange(count, device=q.device)                  # position of each query
+    hidden = torch.arange(length, device=q.device)[None, :] > last[:, None]
+    some = (last >= 0)[:, None, None]
+    for head in range(k.shape[1] if length > 0 and count > 0 else 0):
+        rows = q[:count, head * group:(head + 1) * group].double()
+        scores = torch.einsum("ihd,td->iht", rows, k[:, head]) * softmax_scale
+        p = torch.softmax(scores.masked_fill(hidden[:, None, :] & some, -math.inf), -1)
+        out[:count, head * group:(head + 1) * group] = torch.where(some, p @ v[:, head], 0.0)
+        weight[:count, head * group:(head + 1) * group] = torch.where(some, p @ v[:, head].abs(), 0.0)
     return out, weight
 
 

@@ -310,7 +310,24 @@ def test_attention_of_several_tokens(tokens, q_heads, kv_heads, head_dim, dtype)
     cache.check()
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 40])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads", "head_dim", "lengths"), [
+    (128, 1, 1, 64, [128]), (256, 1, 1, 128, [256]), (100, 2, 1, 128, [1000]), (33, 8, 2, 64, [513, 33, 100]),
+    (300, 8, 2, 128, [300, 777, 3011]), (257, 12, 4, 64, [257, 600]), (130, 3, 1, 64, [2000]), (700, 16, 4, 64, [700, 1000, 701, 900]),
+    (40, 40, 8, 128, [40, 73, 4000])])
+def test_attention_of_a_prompts_chunk(tokens, q_heads, kv_heads, head_dim, lengths, dtype):
+    """Tiles and steps that end anywhere, units that are cut along the tokens and rounds of whole ones."""
+    cache, k, v = _filled(len(lengths), kv_heads, max(lengths) + 5, head_dim, dtype, lengths)
+    q = _draw((len(lengths), tokens, q_heads, head_dim), dtype, 46, 1.5)
+    first = _check_attention(cache, k, v, q, lengths, None)
+    assert torch.equal(cache.attention(q, _words(lengths)), first)
+    counts = [max(0, tokens - 50 * b) for b in range(len(lengths))]
+    _check_attention(cache, k, v, q, lengths, counts)
+    _check_attention(cache, k, v, q, lengths, None, -0.05)
+    cache.check()
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 40, 90])
 def test_queries_without_a_position_and_short_caches(tokens):
     """More queries than tokens held: the ones in front of the first token see nothing."""
     lengths = [1, 0, 2, 35]
