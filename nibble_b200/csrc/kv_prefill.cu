@@ -5,18 +5,20 @@
 // of the piece of work, times 2^10), maxima, sums and outputs are FP32.
 //
 // A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
-// against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's fourteen warps, one CTA per SM:
+// against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's sixteen warps, one CTA per SM:
 //   warps 0-3, 4-7   softmax of tile A and of tile B: a thread per row.  Stages its row of queries, then in every step takes the
-//                    row's 128 scores out of TMEM twice (their maximum, then the exponentials), leaves the probabilities in TMEM in
-//                    the scores' place, and in the end the output.
-//   warps 8-11       make FP16 operands in shared memory of a block's codes each, swizzled by 128 bytes: keys [token][d], values
+//                    row's 128 scores out of TMEM, leaves the probabilities there, and in the end takes the output.
+//   warps 8-11       make FP16 operands in shared memory of a block's codes each (which they have copied in a step ahead), swizzled by 128 bytes: keys [token][d], values
 //                    [d][token]; of the block that is being filled, of its 16-bit numbers; zeros behind the last.
-//   warp 12          allocates TMEM and issues the MMAs: S = Q K^T with both operands in shared memory, O += P V with P in TMEM.
-// TMEM: scores (and probabilities) of A and B, outputs of A and B, 128 columns each.
+//   warp 12          (13-15: nothing) allocates TMEM and issues the MMAs: S = Q K^T with both operands in shared memory, O += P V with P in TMEM.
+// TMEM: 128 columns of scores, 64 of probabilities for each tile, 128 of outputs for each.
 //
-// The order within a step is O_A, S_A of the next step, O_B, S_B of the next step: while one tile's softmax runs, the tensor core works
-// on the other's.  Bounds: MMAs and exponentials take the same 2048 clocks of a step on paper; shared memory (operands written once
-// and read by two MMAs each) is close behind.
+// The tiles share the columns of the scores: a softmax thread takes its row's into registers in one go, and the MMAs of the other
+// tile's scores, which that will want half a round later, follow in their place.  So neither softmax waits for its scores.  (With
+// columns for each tile, probabilities in the scores' place, a tile's next scores had to wait for its last output, and its softmax for
+// both: 592 us where this takes NOWUS, 2048 of 8192 tokens, 64 heads on 8; 64 tokens at a time, twice buffered, 670, since MMAs of 64
+// columns read twice as much shared memory a column.)  Bounds: on paper MMAs and exponentials take 2048 clocks of a step each, and shared
+// memory (operands written once and read by two MMAs each) 2800.
 //
 // Work split.  As many whole units as make full rounds of the CTAs; what is left of the last round is cut along the tokens, so that
 // all CTAs have a piece, and a small kernel adds the pieces up.  (2048 tokens of 64 heads on 8: 512 units, 148 CTAs.)
@@ -46,7 +48,11 @@ constexpr int kStepBlocks = 4;
 constexpr int kStepTokens = kStepBlocks * kKvBlock;
 constexpr int kSoftmaxWarps = 8, kDequantWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kDequantWarps;
-constexpr int kPrefillThreads = (kMmaWarp + 1) * 32;
+constexpr int kPrefillThreads = (kMmaWarp + 4) * 32;      // (registers are handed over by four warps at a time)
+// Registers of a thread: of 128 at launch the makers of operands and the issuer give up what the softmax, which holds a row's 128
+// scores, is short of.
+constexpr int kSoftmaxRegisters = 208, kDequantRegisters = 64, kIssuerRegisters = 32;
+static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 * 128);
 constexpr float kNone = -1.0e30f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;
@@ -128,17 +134,48 @@ struct PrefillShape {
     static constexpr int kQueryBytes = kRows * D * 2;                   // of a tile
     static constexpr int kKeyBytes = kStepTokens * D * 2, kValueBytes = D * kStepTokens * 2;      // of a step
     static constexpr int kKeysAt = 2 * kQueryBytes, kValuesAt = kKeysAt + 2 * kKeyBytes;
-    static constexpr size_t kSharedBytes = kValuesAt + 2 * kValueBytes + 1024;                    // and to align it
+    static constexpr int kCodesAt = kValuesAt + 2 * kValueBytes;
+    static constexpr size_t kSharedBytes = kCodesAt + kDequantWarps * 2 * kKvBlock * D + 1024;    // and to align it
 };
 
+// Each is waited for phase by phase by whoever waits for it, so that a parity names a phase.
 struct PrefillBarriers {
-    unsigned long long q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2];
+    unsigned long long q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+    unsigned long long s_full[2], s_taken[2], p_full[2], o_done[2];      // of a tile
+    unsigned long long codes[kDequantWarps][2];
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two FP32 operations an instruction.
+__device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) { return pair_of(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ float2 both_of(uint64_t pair) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(pair));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -154,6 +191,12 @@ __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& even, uin
     odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
 }
 
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 // D (TMEM) += A (shared memory) x B (shared memory).
 __device__ __forceinline__ void umma_f16_shared(unsigned tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instr_desc,
                                                 uint32_t accumulate) {
@@ -165,20 +208,52 @@ __device__ __forceinline__ void umma_f16_shared(unsigned tmem_d, uint64_t a_desc
         : "memory");
 }
 
-// 32 columns of this thread's TMEM lane, there once this returns; and the other way, sixteen, on their way.
+// Columns of this thread's TMEM lane, there once this returns.  Load and wait are one statement: between two, registers that have not
+// arrived yet could be moved or spilled.
 __device__ __forceinline__ void tmem_load32(unsigned address, uint32_t (&v)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
-          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
-          "=r"(v[30]), "=r"(v[31])
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(address)
         : "memory");
 }
-__device__ __forceinline__ void tmem_store16(unsigned address, const uint32_t (&v)[16]) {
+__device__ __forceinline__ void tmem_load128(unsigned address, uint32_t (&v)[128]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]),
+          "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
+          "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]),
+          "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+          "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63]),
+          "=r"(v[64]), "=r"(v[65]), "=r"(v[66]), "=r"(v[67]), "=r"(v[68]), "=r"(v[69]), "=r"(v[70]), "=r"(v[71]),
+          "=r"(v[72]), "=r"(v[73]), "=r"(v[74]), "=r"(v[75]), "=r"(v[76]), "=r"(v[77]), "=r"(v[78]), "=r"(v[79]),
+          "=r"(v[80]), "=r"(v[81]), "=r"(v[82]), "=r"(v[83]), "=r"(v[84]), "=r"(v[85]), "=r"(v[86]), "=r"(v[87]),
+          "=r"(v[88]), "=r"(v[89]), "=r"(v[90]), "=r"(v[91]), "=r"(v[92]), "=r"(v[93]), "=r"(v[94]), "=r"(v[95]),
+          "=r"(v[96]), "=r"(v[97]), "=r"(v[98]), "=r"(v[99]), "=r"(v[100]), "=r"(v[101]), "=r"(v[102]), "=r"(v[103]),
+          "=r"(v[104]), "=r"(v[105]), "=r"(v[106]), "=r"(v[107]), "=r"(v[108]), "=r"(v[109]), "=r"(v[110]), "=r"(v[111]),
+          "=r"(v[112]), "=r"(v[113]), "=r"(v[114]), "=r"(v[115]), "=r"(v[116]), "=r"(v[117]), "=r"(v[118]), "=r"(v[119]),
+          "=r"(v[120]), "=r"(v[121]), "=r"(v[122]), "=r"(v[123]), "=r"(v[124]), "=r"(v[125]), "=r"(v[126]), "=r"(v[127])
+        : "r"(address), "r"(address + 32), "r"(address + 64), "r"(address + 96)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(unsigned address, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(address),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
@@ -220,13 +295,14 @@ kv_prefill_kernel(const PrefillParams p) {
     using Shape = PrefillShape<D>;
     constexpr int kHalves = Shape::kHalves;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-    constexpr unsigned kOutputs = 256;                   // TMEM columns: scores A, B at 0 and 128, outputs A, B from here on
+    // TMEM columns: scores, probabilities of A, of B, outputs of A, of B
+    constexpr unsigned kProbabilities = 128, kOutputs = 256;
     extern __shared__ uint8_t unaligned[];
     __shared__ __align__(8) PrefillBarriers bars;
     __shared__ unsigned tmem_word;
     // Of a step's blocks, keys' and values', four steps: operands are made two steps ahead of the scores, and those of step n + 2 are
     // formed only when both tiles' probabilities of step n + 1 are there.
-    __shared__ float scales[4][2][kStepBlocks];
+    __shared__ __align__(16) float scales[4][2][kStepBlocks];
     __shared__ float tops[2][4];
     __shared__ int odd_tail[4];                          // number of the work (plus one) whose tail's values have an infinity or NaN
     uint8_t* const shared = unaligned + (1024 - (smem_u32(unaligned) & 1023)) % 1024;
@@ -242,10 +318,15 @@ kv_prefill_kernel(const PrefillParams p) {
             mbar_init(smem_u32(&bars.k_empty[t]), 1);
             mbar_init(smem_u32(&bars.v_empty[t]), 1);
             mbar_init(smem_u32(&bars.s_full[t]), 1);
+            mbar_init(smem_u32(&bars.s_taken[t]), 4);
             mbar_init(smem_u32(&bars.p_full[t]), 4);
             mbar_init(smem_u32(&bars.o_done[t]), 1);
         }
         for (int i = 0; i < 4; ++i) odd_tail[i] = 0;
+        for (int i = 0; i < kDequantWarps; ++i) {
+            mbar_init(smem_u32(&bars.codes[i][0]), 1);
+            mbar_init(smem_u32(&bars.codes[i][1]), 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -269,10 +350,11 @@ kv_prefill_kernel(const PrefillParams p) {
     };
 
     if (warp < kSoftmaxWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
         // ---------------------------------------------------------------- softmax: one row a thread
         const int t = warp / 4, row_in_tile = tid & (kRows - 1);
         const unsigned lanes = static_cast<unsigned>(warp % 4 * 32) << 16;
-        const unsigned score_at = tmem + t * 128 + lanes, out_at = tmem + kOutputs + t * 128 + lanes;
+        const unsigned score_at = tmem + lanes, prob_at = tmem + kProbabilities + t * 64 + lanes, out_at = tmem + kOutputs + t * 128 + lanes;
         int steps_done = 0, steps_of_all = 0;            // of this tile; of both, up to this work
         Work w;
         for (int n = 0; work_of(p, n, w); steps_of_all += w.stop - w.begin, ++n) {
@@ -356,28 +438,44 @@ kv_prefill_kernel(const PrefillParams p) {
             for (int step = w.begin; active && step < w.stop; ++step, ++steps_done) {
                 wait(bars.s_full[t], steps_done);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float* k_scale = scales[(steps_of_all + step - w.begin) & 3][0];
-                const float* v_scale = scales[(steps_of_all + step - w.begin) & 3][1];
+                uint32_t score[kStepTokens];
+                tmem_load128(score_at, score);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                arrive(bars.s_taken[t]);                 // the other tile's scores may come in their place
+                // Of each block: a score's factor, not negative, and the logarithm of a probability's factor, which goes into the exponent
+                // (and out of the sum again).  Either may be NaN; a row that sees nothing of the block is kept out of that.
+                const float4 k_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][0]);
+                const float4 v_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][1]);
+                float by[kStepBlocks] = {k_scale.x, k_scale.y, k_scale.z, k_scale.w};
+                float weight[kStepBlocks] = {v_scale.x, v_scale.y, v_scale.z, v_scale.w};
                 const bool masked = (step + 1) * kStepTokens - 1 > lowest;
-                // the largest score (a score's factor is not negative)
-                float more = kNone;
-#pragma unroll 1
+                const int last = place - step * kStepTokens;             // tokens of the step up to it are seen
+#pragma unroll
                 for (int block = 0; block < kStepBlocks; ++block) {
-                    uint32_t s[32];
-                    tmem_load32(score_at + block * 32, s);
-                    float largest = -INFINITY;
-                    if (masked) {
-                        const int last = place - (step * kStepBlocks + block) * kKvBlock;      // tokens of the block up to it are seen
+                    by[block] *= q_scale;
+                    weight[block] *= per_scale;
+                    if (by[block] == 0.0f) by[block] = 0x1p-100f;
+                    if (weight[block] < 0x1p-80f) weight[block] = 0x1p-80f;
+                    if (masked && block * kKvBlock > last) by[block] = weight[block] = 1.0f;
+                }
+                if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int at = (i & ~3) | (i & 1) << 1 | (i & 2) >> 1;            // columns of a four: tokens 0, 2, 1, 3
-                            if (at <= last) largest = fmaxf(largest, __uint_as_float(s[i]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) largest = fmaxf(largest, __uint_as_float(s[i]));
+                    for (int i = 0; i < kStepTokens; ++i) {
+                        const int token = (i & ~3) | (i & 1) << 1 | (i & 2) >> 1;         // columns of a four: tokens 0, 2, 1, 3
+                        if (token > last) score[i] = 0xff800000u;
                     }
-                    more = fmaxf(more, largest * (k_scale[block] * q_scale));
+                }
+                float more = kNone;
+#pragma unroll
+                for (int block = 0; block < kStepBlocks; ++block) {
+                    const float* x = reinterpret_cast<const float*>(score + block * 32);
+                    float largest[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
+#pragma unroll
+                    for (int i = 6; i < 30; i += 4) {
+                        largest[0] = max3(largest[0], x[i], x[i + 1]);
+                        largest[1] = max3(largest[1], x[i + 2], x[i + 3]);
+                    }
+                    more = fmaxf(more, max3(max3(largest[0], x[30], x[31]), largest[1], largest[1]) * by[block]);
                 }
                 const bool fresh = top == kNone;
                 const bool rises = fresh ? more > kNone : more > top + kMaxLag;
@@ -387,49 +485,36 @@ kv_prefill_kernel(const PrefillParams p) {
                     top = more;
                     sum *= shrink;
                 }
+                if (steps_done > 0) wait(bars.o_done[t], steps_done - 1);      // the probabilities before these have been used
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (step > w.begin && __any_sync(0xffffffffu, shrink != 1.0f)) {
-                    wait(bars.o_done[t], steps_done - 1);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int d = 0; d < D; d += 32) {
-                        uint32_t o[32], half[16];
+                        uint32_t o[32];
                         tmem_load32(out_at + d, o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) half[i] = o[h * 16 + i];
-                            tmem_store16(out_at + d + h * 16, half);
-                        }
+                        tmem_store16(out_at + d, o);
+                        tmem_store16(out_at + d + 16, o + 16);
                     }
                 }
                 const float from = fresh && !rises ? 0.0f : top;      // (a row that has seen nothing yet: all it meets is masked)
-#pragma unroll 1
+#pragma unroll
                 for (int block = 0; block < kStepBlocks; ++block) {
-                    uint32_t s[32], packed[16];
-                    tmem_load32(score_at + block * 32, s);
-                    // the value's scale goes into the exponent, and out of the sum again
-                    float weight = v_scale[block] * per_scale;
-                    if (weight < 0x1p-80f) weight = 0x1p-80f;
-                    const float by = k_scale[block] * q_scale, with = log2f(weight) - from;
-                    const int last = place - (step * kStepBlocks + block) * kKvBlock;
-                    float block_sum[2] = {0.0f, 0.0f};
+                    uint32_t packed[16];
+                    const float with = __log2f(weight[block]) - from;
+                    const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with);
+                    uint64_t sums[2] = {0, 0};
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        float e[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int j = i + h, at = (j & ~3) | (j & 1) << 1 | (j & 2) >> 1;
-                            float x = fmaf(__uint_as_float(s[j]), by, with);
-                            if (masked && at > last) x = -INFINITY;
-                            e[h] = exp2_fast(x);
-                            block_sum[h] += e[h];
-                        }
-                        packed[i / 2] = pack_half(e[0], e[1]);
+                        const float2 x = both_of(fma2(pair_of(score[block * 32 + i], score[block * 32 + i + 1]), by2, with2));
+                        const float a = exp2_fast(x.x), b = exp2_fast(x.y);
+                        sums[i / 2 % 2] = add2(sums[i / 2 % 2], pair_of(a, b));
+                        packed[i / 2] = pack_half(a, b);
                     }
-                    if (last >= 0) sum = fmaf(block_sum[0] + block_sum[1], __fdividef(1.0f, weight), sum);      // (the scale may be NaN)
-                    tmem_store16(score_at + block * 16, packed);
+                    const float2 all = both_of(add2(sums[0], sums[1]));
+                    sum = fmaf(all.x + all.y, __fdividef(1.0f, weight[block]), sum);
+                    tmem_store16(prob_at + block * 16, packed);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -479,27 +564,51 @@ kv_prefill_kernel(const PrefillParams p) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // (the next work's first arrival lets O be overwritten)
         }
     } else if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDequantRegisters));
         // ---------------------------------------------------------------- operands: one block of a step a warp
         const int mine = warp - kSoftmaxWarps, g = lane >> 2, c = lane & 3;
         constexpr int kVectors = D / 16;                 // 16-byte pieces of a block's keys, and values, for a lane
-        uint4 codes[kVectors];
-        // Step number `steps` of all, this CTA's works one after the other.
-        int steps = 0;
+        constexpr int kBlockBytes = kKvBlock * D;
+        uint8_t* const codes = shared + Shape::kCodesAt + mine * 2 * kBlockBytes;      // of a block's keys, and of its values
+        // Asks for a block's codes (which: 0 keys, 1 values), behind all lanes' reads of those before.
+        auto ask = [&](int which, size_t pair, int block) {
+            const unsigned bar = smem_u32(&bars.codes[mine][which]);
+            mbar_arrive_expect_tx(bar, kBlockBytes);
+            bulk_load(smem_u32(codes + which * kBlockBytes), (which == 0 ? p.cache.k_codes : p.cache.v_codes) + (pair * p.cache.blocks + block) * kBlockBytes,
+                      kBlockBytes, bar);
+        };
+        int steps = 0, read = 0;                         // steps of all, this CTA's works one after the other; blocks of codes
         Work w;
+        bool asked = false;                              // whether the next step's codes were asked for
         for (int n = 0; work_of(p, n, w); ++n) {
+            if (w.stop <= w.begin) continue;
             const size_t pair = static_cast<size_t>(w.b) * p.cache.kv_heads + w.head;
+            // the step behind this work's last
+            Work after;
+            int follower = n + 1;
+            bool follows = work_of(p, follower, after);
+            while (follows && after.stop <= after.begin) follows = work_of(p, ++follower, after);
+            const size_t after_pair = static_cast<size_t>(after.b) * p.cache.kv_heads + after.head;
+            const int after_block = after.begin * kStepBlocks + mine;
+            const bool after_coded = follows && after_block < after.full;
+            if (!asked && w.begin * kStepBlocks + mine < w.full && lane == 0) {
+                ask(0, pair, w.begin * kStepBlocks + mine);
+                ask(1, pair, w.begin * kStepBlocks + mine);
+            }
+#pragma unroll 1
             for (int step = w.begin; step < w.stop; ++step, ++steps) {
                 const int block = step * kStepBlocks + mine, stage = steps & 1;
                 const bool coded = block < w.full, tail = block == w.full && w.held > 0;
-                const size_t at = (pair * p.cache.blocks + block) * (kKvBlock * D) + lane * 16;
+                const bool last = step + 1 == w.stop;
+                asked = last ? after_coded : block + kStepBlocks < w.full;
+                const size_t next_pair = last ? after_pair : pair;
+                const int next_block = last ? after_block : block + kStepBlocks;
                 const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + (pair * 2 + (block & 1)) * kKvBlock * D;
                 const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (block & 1)) * kKvBlock * D;
                 float k_scale = 0.0f, v_scale = 0.0f, k_by = 1.0f, v_by = 1.0f;
                 if (coded) {
                     k_scale = p.cache.k_scales[pair * p.cache.blocks + block];
                     v_scale = p.cache.v_scales[pair * p.cache.blocks + block];
-#pragma unroll
-                    for (int i = 0; i < kVectors; ++i) codes[i] = *reinterpret_cast<const uint4*>(p.cache.k_codes + at + i * 512);
                 } else if (tail) {
                     k_by = tail_power<T>(kBf16 ? finite_top(k_tail, w.held * D, lane, 32) : 0.0f, k_scale);
                     v_by = tail_power<T>(kBf16 ? finite_top(v_tail, w.held * D, lane, 32) : 0.0f, v_scale);
@@ -510,25 +619,35 @@ kv_prefill_kernel(const PrefillParams p) {
                     return pack_half(f.x * by, f.y * by);
                 };
                 // keys: row of a token, four tokens in the order 0, 2, 1, 3
+                if (coded) wait(bars.codes[mine][0], read);
                 if (steps >= 2) wait(bars.k_empty[stage], steps / 2 - 1);
                 {
                     uint8_t* const to = shared + Shape::kKeysAt + stage * Shape::kKeyBytes;
-#pragma unroll
-                    for (int i = 0; i < kVectors; ++i) {         // [group of 16 tokens][parity][half of the dims]
+                    auto store = [&](int i, const uint32_t (&words)[8]) {      // piece i: [group of 16 tokens][parity][half of the dims]
                         const int half = i % kHalves, parity = i / kHalves % 2, group = i / kHalves / 2;
                         const int row = mine * 32 + group * 16 + g / 2 * 4 + g % 2 + parity * 2;
-                        uint32_t words[8];
-                        if (coded) {
-                            codes_to_half(codes[i].x, words[0], words[1]);
-                            codes_to_half(codes[i].y, words[2], words[3]);
-                            codes_to_half(codes[i].z, words[4], words[5]);
-                            codes_to_half(codes[i].w, words[6], words[7]);
-                        } else {
+                        uint8_t* const at = to + half * (kStepTokens * 128);
+                        *reinterpret_cast<uint4*>(at + swizzled(row, 2 * c)) = make_uint4(words[0], words[1], words[2], words[3]);
+                        *reinterpret_cast<uint4*>(at + swizzled(row, 2 * c + 1)) = make_uint4(words[4], words[5], words[6], words[7]);
+                    };
+                    if (coded) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) words[e] = 0;
-                            const int token = group * 16 + g * 2 + parity;
+                        for (int i = 0; i < kVectors; ++i) {
+                            const uint4 four = *reinterpret_cast<const uint4*>(codes + i * 512 + lane * 16);
+                            uint32_t words[8];
+                            codes_to_half(four.x, words[0], words[1]);
+                            codes_to_half(four.y, words[2], words[3]);
+                            codes_to_half(four.z, words[4], words[5]);
+                            codes_to_half(four.w, words[6], words[7]);
+                            store(i, words);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < kVectors; ++i) {
+                            uint32_t words[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                            const int token = i / kHalves / 2 * 16 + g * 2 + i / kHalves % 2;
                             if (tail && token < w.held) {
-                                const uint32_t* raw = reinterpret_cast<const uint32_t*>(k_tail + token * D + half * 64 + c * 16);
+                                const uint32_t* raw = reinterpret_cast<const uint32_t*>(k_tail + token * D + i % kHalves * 64 + c * 16);
 #pragma unroll
                                 for (int e = 0; e < 8; e += 2) {
                                     const uint32_t lo = to_half(raw[e], k_by), hi = to_half(raw[e + 1], k_by);
@@ -536,33 +655,31 @@ kv_prefill_kernel(const PrefillParams p) {
                                     words[e + 1] = prmt(lo, hi, 0x7632);
                                 }
                             }
+                            store(i, words);
                         }
-                        uint8_t* const at_half = to + half * (kStepTokens * 128);
-                        *reinterpret_cast<uint4*>(at_half + swizzled(row, 2 * c)) = make_uint4(words[0], words[1], words[2], words[3]);
-                        *reinterpret_cast<uint4*>(at_half + swizzled(row, 2 * c + 1)) = make_uint4(words[4], words[5], words[6], words[7]);
                     }
                 }
                 if (lane == 0) {
                     scales[steps & 3][0][mine] = k_scale;
                     scales[steps & 3][1][mine] = v_scale;
                 }
-                if (coded) {
-#pragma unroll
-                    for (int i = 0; i < kVectors; ++i) codes[i] = *reinterpret_cast<const uint4*>(p.cache.v_codes + at + i * 512);
-                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.k_full[stage]);
+                if (asked && healthy && lane == 0) ask(0, next_pair, next_block);
                 // values: row of a dim, tokens in the columns' order
+                if (coded) wait(bars.codes[mine][1], read++);
                 if (steps >= 2) wait(bars.v_empty[stage], steps / 2 - 1);
                 uint8_t* const to = shared + Shape::kValuesAt + stage * Shape::kValueBytes + mine / 2 * (D * 128);
                 if (coded || !tail) {
 #pragma unroll
                     for (int i = 0; i < kVectors; ++i) {         // sixteen dims: [half of them][group of 16 tokens]
-                        const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                        uint4 four = make_uint4(0u, 0u, 0u, 0u);
+                        if (coded) four = *reinterpret_cast<const uint4*>(codes + kBlockBytes + i * 512 + lane * 16);
+                        const uint32_t words[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            uint32_t even = 0, odd = 0;
-                            if (coded) codes_to_half(words[e], even, odd);
+                            uint32_t even, odd;
+                            codes_to_half(words[e], even, odd);
                             const int d = i * 16 + e / 2 * 8 + g;
                             *reinterpret_cast<uint2*>(to + swizzled(d, mine % 2 * 4 + e % 2 * 2 + c / 2) + c % 2 * 8) = make_uint2(even, odd);
                         }
@@ -600,72 +717,82 @@ kv_prefill_kernel(const PrefillParams p) {
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.v_full[stage]);
+                if (asked && healthy && lane == 0) ask(1, next_pair, next_block);
             }
         }
+        if (!healthy && lane == 0) {                     // wait, within limits, for copies that may still be on their way
+            for (int which = 0; which < 2; ++which) mbar_wait(smem_u32(&bars.codes[mine][which]), read & 1, kKvGaveUp, p.cache.status);
+        }
     } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssuerRegisters));
         // ---------------------------------------------------------------- MMAs
         constexpr uint32_t kCommon = (1u << 4) | (static_cast<uint32_t>(kRows >> 4) << 24);      // FP32 sums of FP16, 128 rows, K-major
         constexpr uint32_t kScoreDesc = kCommon | (static_cast<uint32_t>(kStepTokens >> 3) << 17);
         constexpr uint32_t kOutputDesc = kCommon | (static_cast<uint32_t>(D >> 3) << 17);
         const bool chosen = elect_one();
-        int steps = 0, works[2] = {0, 0}, tile_steps[2] = {0, 0};          // steps of all; works and steps of each tile
-        auto scores = [&](int t, int stage) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (chosen && healthy) {
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint64_t a = operand_desc(smem_u32(shared) + t * Shape::kQueryBytes + i / 4 * (kRows * 128) + i % 4 * 32);
-                    const uint64_t b = operand_desc(smem_u32(shared) + Shape::kKeysAt + stage * Shape::kKeyBytes + i / 4 * (kStepTokens * 128) + i % 4 * 32);
-                    umma_f16_shared(tmem + t * 128, a, b, kScoreDesc, i > 0 ? 1u : 0u);
-                }
-                umma_commit(smem_u32(&bars.s_full[t]));
-            }
-            __syncwarp();
-        };
+        int steps = 0, works[2] = {0, 0};                // steps of all, up to this work; works of each tile
+        int issued[2] = {0, 0}, used[2] = {0, 0};        // of each tile: scores, outputs
+        int holder = -1;                                 // whose scores lie in TMEM
         Work w;
-        for (int n = 0; work_of(p, n, w); ++n) {
+        for (int n = 0; warp == kMmaWarp && work_of(p, n, w); ++n) {
             if (w.stop <= w.begin || w.rows <= w.first_row) continue;
-            const int tiles = w.rows > w.first_row + kRows ? 2 : 1;
-            const int first = steps;
+            const int tiles = w.rows > w.first_row + kRows ? 2 : 1, count = w.stop - w.begin;
+            auto scores = [&](int t, int step) {
+                if (step >= count) return;
+                const int stage = (steps + step) & 1;
+                if (t == 0) wait(bars.k_full[stage], (steps + step) / 2);
+                if (holder >= 0) wait(bars.s_taken[holder], issued[holder] - 1);
+                holder = t;
+                ++issued[t];
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (chosen && healthy) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint64_t a = operand_desc(smem_u32(shared) + t * Shape::kQueryBytes + i / 4 * (kRows * 128) + i % 4 * 32);
+                        const uint64_t b = operand_desc(smem_u32(shared) + Shape::kKeysAt + stage * Shape::kKeyBytes + i / 4 * (kStepTokens * 128) + i % 4 * 32);
+                        umma_f16_shared(tmem, a, b, kScoreDesc, i > 0 ? 1u : 0u);
+                    }
+                    umma_commit(smem_u32(&bars.s_full[t]));
+                    if (t == tiles - 1) umma_commit(smem_u32(&bars.k_empty[stage]));
+                }
+                __syncwarp();
+            };
+            auto outputs = [&](int t, int step) {
+                const int stage = (steps + step) & 1;
+                if (t == 0) wait(bars.v_full[stage], (steps + step) / 2);
+                wait(bars.p_full[t], used[t]++);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (chosen && healthy) {
+#pragma unroll
+                    for (int i = 0; i < kStepTokens / 16; ++i) {
+                        const uint64_t b = operand_desc(smem_u32(shared) + Shape::kValuesAt + stage * Shape::kValueBytes + i / 4 * (D * 128) + i % 4 * 32);
+                        umma_f16_tmem_a(tmem + kOutputs + t * 128, tmem + kProbabilities + t * 64 + i * 8, b, kOutputDesc, step > 0 || i > 0 ? 1u : 0u);
+                    }
+                    umma_commit(smem_u32(&bars.o_done[t]));
+                    if (t == tiles - 1) umma_commit(smem_u32(&bars.v_empty[stage]));
+                }
+                __syncwarp();
+            };
+            // A tile takes its scores as soon as it is done with the last; then the other's, which it will want half a round later, are
+            // formed in their place.
             for (int t = 0; t < tiles; ++t) {
                 wait(bars.q_full[t], works[t]++);
-                if (t == 0) wait(bars.k_full[steps & 1], steps / 2);
-                if (tile_steps[t] > 0) wait(bars.o_done[t], tile_steps[t] - 1);      // (the last probabilities lie where the scores go)
-                scores(t, steps & 1);
+                scores(t, 0);
             }
-            if (chosen && healthy) umma_commit(smem_u32(&bars.k_empty[steps & 1]));
-            __syncwarp();
-            for (int step = w.begin; step < w.stop; ++step, ++steps) {
-                const int stage = steps & 1;
-                const bool last = step + 1 == w.stop;
-                for (int t = 0; t < tiles; ++t) {
-                    if (t == 0) wait(bars.v_full[stage], steps / 2);
-                    wait(bars.p_full[t], tile_steps[t]);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (chosen && healthy) {
-#pragma unroll
-                        for (int i = 0; i < kStepTokens / 16; ++i) {
-                            const uint64_t b = operand_desc(smem_u32(shared) + Shape::kValuesAt + stage * Shape::kValueBytes + i / 4 * (D * 128) + i % 4 * 32);
-                            umma_f16_tmem_a(tmem + kOutputs + t * 128, tmem + t * 128 + i * 8, b, kOutputDesc, steps > first || i > 0 ? 1u : 0u);
-                        }
-                        umma_commit(smem_u32(&bars.o_done[t]));
-                        if (t == tiles - 1) umma_commit(smem_u32(&bars.v_empty[stage]));
-                    }
-                    __syncwarp();
-                    if (!last) {
-                        if (t == 0) wait(bars.k_full[(steps + 1) & 1], (steps + 1) / 2);
-                        wait(bars.o_done[t], tile_steps[t]);
-                        scores(t, (steps + 1) & 1);
-                        if (t == tiles - 1 && chosen && healthy) umma_commit(smem_u32(&bars.k_empty[(steps + 1) & 1]));
-                        __syncwarp();
-                    }
-                    ++tile_steps[t];
+            scores(0, 1);
+            for (int step = 0; step < count; ++step) {
+                outputs(0, step);
+                if (tiles == 2) {
+                    scores(1, step + 1);
+                    outputs(1, step);
                 }
+                scores(0, step + 2);
             }
+            steps += count;
         }
         // nothing may be in flight when TMEM goes
         for (int t = 0; t < 2; ++t) {
-            if (tile_steps[t] > 0) mbar_wait(smem_u32(&bars.o_done[t]), (tile_steps[t] - 1) & 1, kKvGaveUp, p.cache.status);
+            if (used[t] > 0) mbar_wait(smem_u32(&bars.o_done[t]), (used[t] - 1) & 1, kKvGaveUp, p.cache.status);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
