@@ -56,7 +56,7 @@ static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 
 constexpr float kNone = -1.0e30f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;
-constexpr float kMaxLag = 3.0f;                 // how far (log2) a maximum may rise before outputs are rescaled
+constexpr float kLargestSum = 65000.0f;         // of a block's probabilities times their values' scale: none is beyond FP16 then
 
 struct PrefillParams {
     KvCache cache;
@@ -261,6 +261,13 @@ __device__ __forceinline__ void tmem_store16(unsigned address, const uint32_t* v
         : "memory");
 }
 
+// Token of a step's column.  Of a block's 32: four tokens of the first sixteen, then the four of the second sixteen that a lane's values
+// codes hold beside them, each four in the order 0, 2, 1, 3 in which bytes become pairs of FP16.
+__device__ __forceinline__ constexpr int token_of(int column) {
+    const int four = column / 4 % 8;
+    return column / 32 * 32 + four % 2 * 16 + four / 2 * 4 + (column & 1) * 2 + (column & 2) / 2;
+}
+
 // 128-byte swizzle: where 16-byte chunk c of row r of a [rows][128 bytes] tile lies.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
@@ -371,56 +378,48 @@ kv_prefill_kernel(const PrefillParams p) {
                 uint8_t* const to = shared + t * Shape::kQueryBytes;
                 const T* from = reinterpret_cast<const T*>(p.q) + w.b * p.q_batch + token * p.q_token + q_head * p.q_head;
                 const uint32_t sign = p.negate ? 0x80008000u : 0u;
-                auto load = [&](int chunk, uint32_t (&raw)[4]) {         // eight dims
-                    raw[0] = raw[1] = raw[2] = raw[3] = 0;
-                    if (row >= w.rows) return;
-                    if (p.q_wide) {
-                        const uint4 four = *reinterpret_cast<const uint4*>(from + chunk * 8);
-                        raw[0] = four.x; raw[1] = four.y; raw[2] = four.z; raw[3] = four.w;
-                    } else {
-                        const uint16_t* h = reinterpret_cast<const uint16_t*>(from + chunk * 8);
+                uint32_t raw[D / 2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) raw[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
+                for (int i = 0; i < D / 2; i += 4) {                     // (all of it requested together)
+                    raw[i] = raw[i + 1] = raw[i + 2] = raw[i + 3] = 0;
+                    if (row < w.rows && p.q_wide) {
+                        const uint4 four = *reinterpret_cast<const uint4*>(from + 2 * i);
+                        raw[i] = four.x; raw[i + 1] = four.y; raw[i + 2] = four.z; raw[i + 3] = four.w;
+                    } else if (row < w.rows) {
+                        const uint16_t* h = reinterpret_cast<const uint16_t*>(from + 2 * i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) raw[i + e] = h[2 * e] | static_cast<uint32_t>(h[2 * e + 1]) << 16;
                     }
-                };
-                float by = 1.0f;
+                }
+                const float* v_scales = p.cache.v_scales + pair * p.cache.blocks;
+                for (int block = w.begin * kStepBlocks + row_in_tile; block < min(w.stop * kStepBlocks, w.full); block += kRows) {
+                    unit_scale = fmaxf(unit_scale, v_scales[block]);
+                }
                 if constexpr (kBf16) {
                     // BF16 becomes FP16 by a power of two of the row's own: a number keeps all its bits unless it is 2^-23 of the
                     // row's largest or less
                     uint32_t largest = 0;
-                    for (int chunk = 0; chunk < D / 8; ++chunk) {
-                        uint32_t raw[4];
-                        load(chunk, raw);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) largest = max(largest, max(raw[i] << 16 & 0x7fffffffu, raw[i] & 0x7fff0000u));
-                    }
+                    for (int i = 0; i < D / 2; ++i) largest = max(largest, max(raw[i] << 16 & 0x7fffffffu, raw[i] & 0x7fff0000u));
                     float back;
-                    by = power_for(__uint_as_float(min(largest, 0x7f7f0000u)), back);
+                    const float by = power_for(__uint_as_float(min(largest, 0x7f7f0000u)), back);
                     q_scale *= back;
-                }
-#pragma unroll 4
-                for (int chunk = 0; chunk < D / 8; ++chunk) {
-                    uint32_t raw[4];
-                    load(chunk, raw);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (kBf16) {
-                            const float2 f = widen2<T>(raw[i]);
-                            raw[i] = pack_half(f.x * by, f.y * by);
-                        }
-                        raw[i] ^= sign;
+                    for (int i = 0; i < D / 2; ++i) {
+                        const float2 f = widen2<T>(raw[i]);
+                        raw[i] = pack_half(f.x * by, f.y * by);
                     }
-                    *reinterpret_cast<uint4*>(to + chunk / 8 * (kRows * 128) + swizzled(row_in_tile, chunk % 8)) =
-                        make_uint4(prmt(raw[0], raw[1], 0x5410), prmt(raw[0], raw[1], 0x7632), prmt(raw[2], raw[3], 0x5410), prmt(raw[2], raw[3], 0x7632));
+                }
+#pragma unroll
+                for (int i = 0; i < D / 2; i += 4) {
+                    *reinterpret_cast<uint4*>(to + i / 32 * (kRows * 128) + swizzled(row_in_tile, i / 4 % 8)) =
+                        make_uint4(prmt(raw[i], raw[i + 1], 0x5410) ^ sign, prmt(raw[i], raw[i + 1], 0x7632) ^ sign,
+                                   prmt(raw[i + 2], raw[i + 3], 0x5410) ^ sign, prmt(raw[i + 2], raw[i + 3], 0x7632) ^ sign);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.q_full[t]);
                 // What the accumulator's numbers are relative to: the largest scale of the values that this work meets.  Rounded up to a
                 // power of two, so that what a row does not see has no part in how its probabilities are rounded.
-                const float* v_scales = p.cache.v_scales + pair * p.cache.blocks;
-                for (int block = w.begin * kStepBlocks + row_in_tile; block < min(w.stop * kStepBlocks, w.full); block += kRows) {
-                    unit_scale = fmaxf(unit_scale, v_scales[block]);
-                }
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) unit_scale = fmaxf(unit_scale, __shfl_xor_sync(0xffffffffu, unit_scale, o));
                 if (has_tail) {
@@ -461,61 +460,71 @@ kv_prefill_kernel(const PrefillParams p) {
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < kStepTokens; ++i) {
-                        const int token = (i & ~3) | (i & 1) << 1 | (i & 2) >> 1;         // columns of a four: tokens 0, 2, 1, 3
-                        if (token > last) score[i] = 0xff800000u;
+                        if (token_of(i) > last) score[i] = 0xff800000u;
                     }
-                }
-                float more = kNone;
-#pragma unroll
-                for (int block = 0; block < kStepBlocks; ++block) {
-                    const float* x = reinterpret_cast<const float*>(score + block * 32);
-                    float largest[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
-#pragma unroll
-                    for (int i = 6; i < 30; i += 4) {
-                        largest[0] = max3(largest[0], x[i], x[i + 1]);
-                        largest[1] = max3(largest[1], x[i + 2], x[i + 3]);
-                    }
-                    more = fmaxf(more, max3(max3(largest[0], x[30], x[31]), largest[1], largest[1]) * by[block]);
-                }
-                const bool fresh = top == kNone;
-                const bool rises = fresh ? more > kNone : more > top + kMaxLag;
-                float shrink = 1.0f;
-                if (rises) {
-                    shrink = fresh ? 1.0f : exp2_fast(top - more);
-                    top = more;
-                    sum *= shrink;
                 }
                 if (steps_done > 0) wait(bars.o_done[t], steps_done - 1);      // the probabilities before these have been used
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (step > w.begin && __any_sync(0xffffffffu, shrink != 1.0f)) {
+                // The maximum is looked for in the first step, and where the probabilities relative to the last one have become too
+                // large for FP16: then once more, relative to the new one.
+                float step_sum = 0.0f;
+                bool anew = step == w.begin;
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 32) {
-                        uint32_t o[32];
-                        tmem_load32(out_at + d, o);
+                for (int attempt = 0; attempt < 2; ++attempt) {
+                    if (anew) {
+                        float more = kNone;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-                        tmem_store16(out_at + d, o);
-                        tmem_store16(out_at + d + 16, o + 16);
+                        for (int block = 0; block < kStepBlocks; ++block) {
+                            const float* x = reinterpret_cast<const float*>(score + block * 32);
+                            float largest[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
+#pragma unroll
+                            for (int i = 6; i < 30; i += 4) {
+                                largest[0] = max3(largest[0], x[i], x[i + 1]);
+                                largest[1] = max3(largest[1], x[i + 2], x[i + 3]);
+                            }
+                            more = fmaxf(more, max3(max3(largest[0], x[30], x[31]), largest[1], largest[1]) * by[block]);
+                        }
+                        const float shrink = more > top && top > kNone ? exp2_fast(top - more) : 1.0f;
+                        top = fmaxf(top, more);
+                        sum *= shrink;
+                        if (step > w.begin) {
+#pragma unroll 1
+                            for (int d = 0; d < D; d += 32) {
+                                uint32_t o[32];
+                                tmem_load32(out_at + d, o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                                tmem_store16(out_at + d, o);
+                                tmem_store16(out_at + d + 16, o + 16);
+                            }
+                        }
+                        anew = false;
                     }
-                }
-                const float from = fresh && !rises ? 0.0f : top;      // (a row that has seen nothing yet: all it meets is masked)
+                    const float from = top > kNone ? top : 0.0f;      // (a row that has seen nothing yet: all it meets is masked)
+                    step_sum = 0.0f;
+                    float largest_sum = 0.0f;
 #pragma unroll
-                for (int block = 0; block < kStepBlocks; ++block) {
-                    uint32_t packed[16];
-                    const float with = __log2f(weight[block]) - from;
-                    const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with);
-                    uint64_t sums[2] = {0, 0};
+                    for (int block = 0; block < kStepBlocks; ++block) {
+                        uint32_t packed[16];
+                        const float with = __log2f(weight[block]) - from;
+                        const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with);
+                        uint64_t sums[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 x = both_of(fma2(pair_of(score[block * 32 + i], score[block * 32 + i + 1]), by2, with2));
-                        const float a = exp2_fast(x.x), b = exp2_fast(x.y);
-                        sums[i / 2 % 2] = add2(sums[i / 2 % 2], pair_of(a, b));
-                        packed[i / 2] = pack_half(a, b);
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 x = both_of(fma2(pair_of(score[block * 32 + i], score[block * 32 + i + 1]), by2, with2));
+                            const float a = exp2_fast(x.x), b = exp2_fast(x.y);
+                            sums[i / 2 % 2] = add2(sums[i / 2 % 2], pair_of(a, b));
+                            packed[i / 2] = pack_half(a, b);
+                        }
+                        const float2 all = both_of(add2(sums[0], sums[1]));
+                        largest_sum = fmaxf(largest_sum, all.x + all.y);
+                        step_sum = fmaf(all.x + all.y, __fdividef(1.0f, weight[block]), step_sum);
+                        tmem_store16(prob_at + block * 16, packed);
                     }
-                    const float2 all = both_of(add2(sums[0], sums[1]));
-                    sum = fmaf(all.x + all.y, __fdividef(1.0f, weight[block]), sum);
-                    tmem_store16(prob_at + block * 16, packed);
+                    anew = __any_sync(0xffffffffu, largest_sum > kLargestSum);
+                    if (!anew) break;
                 }
+                sum += step_sum;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 arrive(bars.p_full[t]);
@@ -618,14 +627,14 @@ kv_prefill_kernel(const PrefillParams p) {
                     const float2 f = widen2<T>(word);
                     return pack_half(f.x * by, f.y * by);
                 };
-                // keys: row of a token, four tokens in the order 0, 2, 1, 3
+                // keys: row of a token, in the order of the columns (token_of)
                 if (coded) wait(bars.codes[mine][0], read);
                 if (steps >= 2) wait(bars.k_empty[stage], steps / 2 - 1);
                 {
                     uint8_t* const to = shared + Shape::kKeysAt + stage * Shape::kKeyBytes;
                     auto store = [&](int i, const uint32_t (&words)[8]) {      // piece i: [group of 16 tokens][parity][half of the dims]
                         const int half = i % kHalves, parity = i / kHalves % 2, group = i / kHalves / 2;
-                        const int row = mine * 32 + group * 16 + g / 2 * 4 + g % 2 + parity * 2;
+                        const int row = mine * 32 + g / 2 * 8 + group * 4 + g % 2 + parity * 2;
                         uint8_t* const at = to + half * (kStepTokens * 128);
                         *reinterpret_cast<uint4*>(at + swizzled(row, 2 * c)) = make_uint4(words[0], words[1], words[2], words[3]);
                         *reinterpret_cast<uint4*>(at + swizzled(row, 2 * c + 1)) = make_uint4(words[4], words[5], words[6], words[7]);
@@ -677,11 +686,11 @@ kv_prefill_kernel(const PrefillParams p) {
                         if (coded) four = *reinterpret_cast<const uint4*>(codes + kBlockBytes + i * 512 + lane * 16);
                         const uint32_t words[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint32_t even, odd;
-                            codes_to_half(words[e], even, odd);
-                            const int d = i * 16 + e / 2 * 8 + g;
-                            *reinterpret_cast<uint2*>(to + swizzled(d, mine % 2 * 4 + e % 2 * 2 + c / 2) + c % 2 * 8) = make_uint2(even, odd);
+                        for (int half = 0; half < 2; ++half) {
+                            uint4 eight;
+                            codes_to_half(words[2 * half], eight.x, eight.y);
+                            codes_to_half(words[2 * half + 1], eight.z, eight.w);
+                            *reinterpret_cast<uint4*>(to + swizzled(i * 16 + half * 8 + g, mine % 2 * 4 + c)) = eight;
                         }
                     }
                 } else {
@@ -707,8 +716,8 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const unsigned pick = h == 0 ? 0x5410u : 0x7632u;
-                                const int chunk = mine % 2 * 4 + quad / 2;
-                                *reinterpret_cast<uint2*>(to + swizzled(d0 + 2 * f + h, chunk) + quad % 2 * 8) =
+                                const int chunk = mine % 2 * 4 + quad % 4;
+                                *reinterpret_cast<uint2*>(to + swizzled(d0 + 2 * f + h, chunk) + quad / 4 * 8) =
                                     make_uint2(prmt(raw[0][f], raw[2][f], pick), prmt(raw[1][f], raw[3][f], pick));
                             }
                         }
