@@ -204,7 +204,8 @@ struct AttentionShape {
 };
 
 // 8-row tiles of a warp in the variants for 32 and 64 rows: as many as its registers hold, since they share what makes FP16 of codes.
-// (8 sequences, 40 rows each, D = 64: two tiles and four warps to a ring 20.7 us, four and two WIDEUS.)
+// (D = 64, 32 query heads on 4: eight sequences of 8000 tokens, 40 rows: four tiles and two warps to a ring 37.4 us, two and four
+// 46.0; 24 rows 25.7 and 29.2; short sequences the same within 1 us.)
 template <int D>
 constexpr int kWide = D == 64 ? 4 : 2;
 
@@ -853,7 +854,7 @@ int allow_all() {
     return allow_shared(kv_attention_kernel<T, D, 1, 1>, AttentionShape<T, D, 1, 1>::kSharedBytes) |
            allow_shared(kv_attention_kernel<T, D, 2, 1>, AttentionShape<T, D, 2, 1>::kSharedBytes) |
            allow_shared(kv_attention_kernel<T, D, kWide<D>, 4 / kWide<D>>, AttentionShape<T, D, kWide<D>, 4 / kWide<D>>::kSharedBytes) |
-           allow_shared(kv_attention_kernel<T, D, kWide<D>, 8 / kWide<D>>, AttentionShape<T, D, kWide<D>, 8 / kWide<D>>::kSharedBytes) |
+           (D == 64 ? allow_shared(kv_attention_kernel<T, 64, kWide<64>, 8 / kWide<64>>, AttentionShape<T, 64, kWide<64>, 8 / kWide<64>>::kSharedBytes) : 0) |
            allow_shared(kv_finish_kernel<T, D, 1>, 0) | allow_shared(kv_finish_kernel<T, D, 4>, 0);
 }
 
@@ -869,7 +870,7 @@ int device_state(const DeviceState** state) {
 }
 
 struct Shape {
-    int tile_rows, row_tiles;      // rows of a CTA: 8, 16, 32 or 64
+    int tile_rows, row_tiles;      // rows of a CTA: 8, 16, 32, or 64 where D is 64
     int64_t units, grid;           // sequences x heads x tiles; CTAs of the first kernel, 0 where no block can be full
     size_t workspace;
 };
@@ -897,13 +898,18 @@ int launch_shape(const AttentionParams& p, const Shape& s, bool programmatic, cu
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
     using Wide = std::integral_constant<int, kWide<D>>;
-    using Half = std::integral_constant<int, 4 / kWide<D>>;
-    using Whole = std::integral_constant<int, 8 / kWide<D>>;
     if (s.grid > 0) {
-        const int status = s.tile_rows == 8    ? run(One{}, One{})
-                           : s.tile_rows == 16 ? run(Two{}, One{})
-                           : s.tile_rows == 32 ? run(Wide{}, Half{})
-                                               : run(Wide{}, Whole{});
+        int status;
+        if (s.tile_rows == 8) {
+            status = run(One{}, One{});
+        } else if (s.tile_rows == 16) {
+            status = run(Two{}, One{});
+        } else if (s.tile_rows == 32) {
+            status = run(Wide{}, std::integral_constant<int, 4 / kWide<D>>{});
+        } else {
+            if constexpr (D == 64) status = run(Wide{}, std::integral_constant<int, 8 / kWide<D>>{});
+            else return W4A16_ERR_BAD_SHAPE;        // (the other kernel's)
+        }
         if (status != W4A16_OK) return status;
     }
     // Behind the first kernel always programmatic: it waits for that one itself.  Four warps a row while rows are few.

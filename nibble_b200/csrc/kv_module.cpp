@@ -1,6 +1,7 @@
 // The native side of nibble_b200/kv_cache.py: checks tensors, allocates outputs and workspaces from the caching allocator, and
 // hands pointers plus the current stream of the tensors' device to the C ABI.  Every violation is a TORCH_CHECK, i.e. a
-// RuntimeError.  (Messages hold no numbers: with this image's compiler, formatting one through a stream crashes.)  Nothing here takes part in autograd: a call whose input asks for a gradient is refused.
+// RuntimeError.  (Messages hold no numbers: with this image's compiler, formatting one through a stream crashes.)  Nothing here takes
+// part in autograd: a call whose input asks for a gradient is refused.
 #include "kv_module.h"
 
 #include <ATen/ATen.h>
