@@ -13,6 +13,10 @@ FP32 RMSNorm statistics, FP16 rotary products, FP32 softmax), so logits agree wi
 eager forward up to summation order.  Short prompts are consumed one token per step; longer ones go
 through the model's own batched forward once (its linears then run the prefill kernels) and the
 resulting keys and values are copied into the runner's caches, which use the same layout.
+
+With ``cache_bits=8`` the caches are ``QuantizedKVCache``s, half the size; a block then has three kernels (append with rotary
+positions, and the attention's two) where it had one, prompts are processed in chunks that attend over the 8-bit caches as decoded
+tokens do, and rotary products are FP32, rounded once.
 """
 from __future__ import annotations
 
@@ -22,6 +26,7 @@ import torch
 
 from . import _native
 from .fusion import FusedQuantizedLinear, FusedSlice, fuse_parallel_linears
+from .kv_cache import QuantizedKVCache
 from .linear import QuantizedLinear
 
 
@@ -106,10 +111,16 @@ class LlamaDecodeRunner:
 
     ``model`` keeps ownership of the weights; the runner fuses q/k/v and gate/up (if not fused yet),
     allocates its own KV caches ``[layers, kv_heads, max_len, head_dim]`` and work buffers, and
-    captures the step in a CUDA graph at the first ``step``.
+    captures the step in a CUDA graph at the first ``step``.  ``cache_bits=8`` holds keys and values in
+    8 bits (one ``QuantizedKVCache`` per layer, in ``caches``; ``k_cache`` and ``v_cache`` are None).
     """
 
-    def __init__(self, model: torch.nn.Module, max_len: int, fuse_inputs: bool | None = None, persistent: bool = False):
+    def __init__(self, model: torch.nn.Module, max_len: int, fuse_inputs: bool | None = None, persistent: bool = False,
+                 cache_bits: int = 16):
+        if cache_bits not in (8, 16):
+            raise ValueError("cache_bits must be 8 or 16")
+        if cache_bits == 8 and persistent:
+            raise ValueError("the persistent step holds its cache in 16 bits")
         config = model.config
         self.model = model
         self.hidden = config.hidden_size
@@ -146,8 +157,15 @@ class LlamaDecodeRunner:
         self.inter = self.layers[0]["gate_up"].out_features // 2
         n_layers = len(self.layers)
         half = dict(dtype=torch.float16, device=device)
-        self.k_cache = torch.zeros((n_layers, self.kv_heads, self.max_len, self.head_dim), **half)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.caches = None
+        self.k_cache = self.v_cache = None
+        if cache_bits == 8:
+            self.caches = [QuantizedKVCache(1, self.kv_heads, self.max_len, self.head_dim, device=device) for _ in range(n_layers)]
+            self._cache_status = [cache.memory[:4].view(torch.int32) for cache in self.caches]
+            self.length = torch.zeros((1,), dtype=torch.long, device=device)      # the position's token included
+        else:
+            self.k_cache = torch.zeros((n_layers, self.kv_heads, self.max_len, self.head_dim), **half)
+            self.v_cache = torch.zeros_like(self.k_cache)
         self.token = torch.zeros((1,), dtype=torch.long, device=device)
         self.position = torch.zeros((1,), dtype=torch.long, device=device)
         self.status = torch.zeros((1,), dtype=torch.int32, device=device)
@@ -218,6 +236,20 @@ class LlamaDecodeRunner:
         return _native.InputTransform(_native.INPUT_ADD_RMSNORM, 0 if delta is None else delta.data_ptr(), weight.data_ptr(),
                                       0 if target is None else target.data_ptr(), self.eps)
 
+    def _attend(self, index: int, qkv: torch.Tensor) -> torch.Tensor:
+        """Positions, cache and attention of block ``index`` for the token whose projections are ``qkv``."""
+        if self.caches is None:
+            attention_decode(qkv, self.k_cache[index], self.v_cache[index], self.attn_out, self.position, self.inv_freq,
+                             self.q_heads, self.kv_heads, self.head_dim, self.rope_scale, self.status)
+            return self.attn_out
+        return self._attend_8bit(index, qkv, self.position, self.length)
+
+    def _attend_8bit(self, index: int, qkv: torch.Tensor, start: torch.Tensor, length: torch.Tensor) -> torch.Tensor:
+        q, k, v = (part.view(1, qkv.shape[0], -1, self.head_dim) for part in
+                   qkv.split([heads * self.head_dim for heads in (self.q_heads, self.kv_heads, self.kv_heads)], dim=1))
+        q = self.caches[index].append(k, v, start, q=q, inv_freq=self.inv_freq, rope_scale=self.rope_scale)
+        return self.caches[index].attention(q, length).view(qkv.shape[0], -1)
+
     def _enqueue_fused_step(self) -> None:
         a, b, ws = self.stream, self.stream_b, self.workspace
         silu = _native.InputTransform(_native.INPUT_SILU_MUL, 0, 0, 0, 0.0)
@@ -225,9 +257,8 @@ class LlamaDecodeRunner:
         delta = None
         for index, layer in enumerate(self.layers):
             linear_with_input(layer["qkv"], a, self.qkv_out, ws, self._norm_into(a, delta, layer["norm1"], b))
-            attention_decode(self.qkv_out, self.k_cache[index], self.v_cache[index], self.attn_out, self.position,
-                             self.inv_freq, self.q_heads, self.kv_heads, self.head_dim, self.rope_scale, self.status)
-            linear_with_input(layer["o"], self.attn_out, self.o_out, ws, None)
+            attn = self._attend(index, self.qkv_out)
+            linear_with_input(layer["o"], attn, self.o_out, ws, None)
             linear_with_input(layer["gate_up"], b, self.gate_up_out, ws, self._norm_into(b, self.o_out, layer["norm2"], a))
             linear_with_input(layer["down"], self.gate_up_out, self.down_out, ws, silu)
             delta = self.down_out
@@ -235,6 +266,8 @@ class LlamaDecodeRunner:
         argmax_advance(self.logits, self.token, self.position)
 
     def _enqueue_step(self) -> None:
+        if self.caches is not None:
+            torch.add(self.position, 1, out=self.length)
         if self.fuse_inputs:
             self._enqueue_fused_step()
             return
@@ -243,9 +276,7 @@ class LlamaDecodeRunner:
         for index, layer in enumerate(self.layers):
             add_rmsnorm(self.stream, delta, layer["norm1"], self.eps, self.normed)
             qkv = layer["qkv"](self.normed)
-            attention_decode(qkv, self.k_cache[index], self.v_cache[index], self.attn_out, self.position, self.inv_freq,
-                             self.q_heads, self.kv_heads, self.head_dim, self.rope_scale, self.status)
-            attn = layer["o"](self.attn_out)
+            attn = layer["o"](self._attend(index, qkv))
             add_rmsnorm(self.stream, attn, layer["norm2"], self.eps, self.normed)
             gate_up = layer["gate_up"](self.normed)
             silu_mul(gate_up, self.act)
@@ -261,19 +292,19 @@ class LlamaDecodeRunner:
             return
         with torch.inference_mode():
             if self._graph is None:
-                keep = (self.token.clone(), self.position.clone(), self.k_cache.clone(), self.v_cache.clone())
+                # (8-bit caches may be written twice at a position: it is the same token)
+                kept = [t for t in (self.token, self.position, self.k_cache, self.v_cache) if t is not None]
+                copies = [t.clone() for t in kept]
                 before = _native.core().w4a16_launch_count()
                 self._enqueue_step()                      # warm-up outside capture: workspaces, lazy initialisation
                 self.launches_per_step = _native.core().w4a16_launch_count() - before
                 torch.cuda.synchronize()
-                self.token.copy_(keep[0]); self.position.copy_(keep[1])
-                self.k_cache.copy_(keep[2]); self.v_cache.copy_(keep[3])
+                torch._foreach_copy_(kept, copies)
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
                     self._enqueue_step()
                 self._graph = graph
-                self.token.copy_(keep[0]); self.position.copy_(keep[1])
-                self.k_cache.copy_(keep[2]); self.v_cache.copy_(keep[3])
+                torch._foreach_copy_(kept, copies)
             self._graph.replay()
 
     def reset(self) -> None:
@@ -281,6 +312,8 @@ class LlamaDecodeRunner:
         self.status.zero_()
         if self.persistent:
             self.step_status.zero_()
+        if self.caches is not None:
+            torch._foreach_zero_(self._cache_status)
 
     # Prompts up to this many tokens are cheaper one decode step at a time than through the framework's
     # batched forward (about half a millisecond per token against a fixed ~12 ms).
@@ -299,6 +332,34 @@ class LlamaDecodeRunner:
                 self.token.copy_(prompt[i:i + 1])
                 self.step()
             return
+        count = prompt.numel()
+        if self.caches is not None:
+            self._prefill_8bit(prompt)
+        else:
+            self._prefill_16bit(prompt)
+        self.position.fill_(count)
+        from .cuda import check_device_status
+
+        check_device_status()      # the batched forward ran the prefill kernels: none of their waits may have given up
+
+    # Tokens of a prompt that go through the model together with an 8-bit cache: enough to fill the machine, and activations stay small.
+    PREFILL_CHUNK = 2048
+
+    def _prefill_8bit(self, prompt: torch.Tensor) -> None:
+        body = self.model.model
+        with torch.inference_mode():
+            for begin in range(0, prompt.numel(), self.PREFILL_CHUNK):
+                ids = prompt[begin:begin + self.PREFILL_CHUNK]
+                self.position.fill_(begin)
+                self.length.fill_(begin + ids.numel())
+                stream = self.embed[ids]
+                for index, (block, entry) in enumerate(zip(body.layers, self.layers)):
+                    qkv = entry["qkv"](block.input_layernorm(stream))
+                    stream = stream + entry["o"](self._attend_8bit(index, qkv, self.position, self.length))
+                    stream = stream + block.mlp(block.post_attention_layernorm(stream))
+            self.token.copy_(self.lm_head(body.norm(stream[-1:])).argmax(-1))
+
+    def _prefill_16bit(self, prompt: torch.Tensor) -> None:
         from transformers import StaticCache
 
         count = prompt.numel()
@@ -310,10 +371,6 @@ class LlamaDecodeRunner:
                 self.k_cache[index, :, :count].copy_(layer.keys[0, :, :count])
                 self.v_cache[index, :, :count].copy_(layer.values[0, :, :count])
             self.token.copy_(out.logits[0, -1:].argmax(-1))
-            self.position.fill_(count)
-        from .cuda import check_device_status
-
-        check_device_status()      # the batched forward ran the prefill kernels: none of their waits may have given up
 
     def generate(self, prompt_ids: torch.Tensor, new_tokens: int, batched_prefill: bool | None = None) -> torch.Tensor:
         """Greedy continuation of a 1-D prompt; returns the ``new_tokens`` generated ids."""
@@ -328,6 +385,11 @@ class LlamaDecodeRunner:
                 self.step()
         if int(self.status.item()) != 0:
             raise RuntimeError("a decode step ran past the end of the KV cache")
+        if self.caches is not None:
+            words = int(torch.cat(self._cache_status).bitwise_and(3).amax().item())
+            if words != 0:
+                raise RuntimeError("a decode step ran past the end of the KV cache" if words == 1 else
+                                   "attention over the 8-bit cache gave up waiting; its output is incomplete")
         if self.persistent and int(self.step_status.item()) != 0:
             code = int(self.step_status.item())
             raise RuntimeError("a decode step ran past the end of the KV cache" if code == 1 else

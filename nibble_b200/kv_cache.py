@@ -22,9 +22,15 @@ from .cuda import _require_extension, programmatic_launch_enabled
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
+_ops = None
+
+
 def _extension():
-    _require_extension()
-    return _native.load_torch_ops()
+    global _ops
+    if _ops is None:
+        _require_extension()
+        _ops = _native.load_torch_ops()
+    return _ops
 
 
 def apply_rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, scale: float = 1.0,
