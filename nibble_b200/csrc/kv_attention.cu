@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMinRun = 8;                      // blocks that are worth a CTA, with what starting costs
+constexpr int kMinRun = 4;                      // blocks that are worth a CTA, with what starting costs
 constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
 constexpr float kNone = -1.0e30f;               // the maximum of nothing
 constexpr float kLog2e = 1.4426950408889634f;

@@ -363,12 +363,14 @@ kv_append_kernel(const AppendParams p) {
     T* const k_tail = reinterpret_cast<T*>(p.cache.k_tail) + static_cast<size_t>(pair) * 2 * kKvBlock * D;
     T* const v_tail = reinterpret_cast<T*>(p.cache.v_tail) + static_cast<size_t>(pair) * 2 * kKvBlock * D;
 
-    // The numbers of a block's token as the cache gets them (the key turned), as they lie in the tail, or zeros.
+    // The numbers of a block's token as the cache gets them (the key turned), as they lie in the tail where the block is going to be
+    // full, or zeros.
     auto fetch = [&](int of_block, uint32_t (&k)[8], uint32_t (&v)[8]) {
         const int t = of_block * kKvBlock + slot, v_t = of_block * kKvBlock + v_slot;
-        if (v_t < begin) {
+        const bool whole = of_block < newest;
+        if (whole && v_t < begin) {
             load16<T>(v_tail + ((of_block & 1) * kKvBlock + v_slot) * D + v_d0, true, v);
-        } else if (v_t < end) {
+        } else if (v_t >= begin && v_t < end) {
             load16<T>(row_of<T>(p.v, b, v_t - begin, head) + v_d0, p.wide, v);
         } else {
 #pragma unroll
@@ -377,14 +379,15 @@ kv_append_kernel(const AppendParams p) {
         if (ROTARY) {
             __syncthreads();
             const int half = p.rotary_dim / 2;
-            for (int i = tid; i < kKvBlock * half; i += kThreads) {
+            const int from = max(0, begin - of_block * kKvBlock), to = min(kKvBlock, end - of_block * kKvBlock);      // the new tokens
+            for (int i = from * half + tid; i < to * half; i += kThreads) {
                 factors[i] = rotary_factors(static_cast<long long>(of_block) * kKvBlock + i / half, p.inv_freq[i % half], p.rope_scale);
             }
             __syncthreads();
         }
-        if (t < begin) {
+        if (whole && t < begin) {
             load16<T>(k_tail + ((of_block & 1) * kKvBlock + slot) * D + d0, true, k);
-        } else if (t < end) {
+        } else if (t >= begin && t < end) {
             const T* from = row_of<T>(p.k, b, t - begin, head);
             load16<T>(from + d0, p.wide, k);
             if (ROTARY) {

@@ -13,6 +13,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstdlib>
+#include <cstring>
 #include <optional>
 
 #include "../../include/w4a16_b200.h"
@@ -94,7 +96,11 @@ w4a16_rotary_spec spec_of(const at::Tensor& inv_freq, const at::Device& device, 
 
 w4a16_stream_t current_stream() { return reinterpret_cast<w4a16_stream_t>(at::cuda::getCurrentCUDAStream().stream()); }
 
-uint32_t launch_flags(bool programmatic) { return programmatic ? W4A16_FLAG_PROGRAMMATIC_LAUNCH : 0u; }
+// (what nibble_b200.cuda.programmatic_launch_enabled() says, which takes Python a third of such a call)
+uint32_t launch_flags() {
+    const char* knob = std::getenv("W4A16_PDL");
+    return knob != nullptr && std::strcmp(knob, "1") == 0 ? W4A16_FLAG_PROGRAMMATIC_LAUNCH : 0u;
+}
 
 bool truth_of(PyObject* object) {
     const int value = PyObject_IsTrue(object);
@@ -104,17 +110,17 @@ bool truth_of(PyObject* object) {
 
 }  // namespace
 
-// rotary(x, positions, inv_freq, scale, interleaved, out or None, programmatic) -> Tensor
+// rotary(x, positions, inv_freq, scale, interleaved, out or None) -> Tensor
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    check_count(count, 7, "rotary");
+    check_count(count, 6, "rotary");
     const at::Tensor& x = tensor_of(args[0], "x");
     const at::Tensor& positions = tensor_of(args[1], "positions");
     const at::Tensor& inv_freq = tensor_of(args[2], "inv_freq");
     const double scale = number_of(args[3]);
     const bool interleaved = truth_of(args[4]);
     std::optional<at::Tensor> given = optional_of(args[5], "out");
-    const uint32_t flags = launch_flags(truth_of(args[6]));
+    const uint32_t flags = launch_flags();
     TORCH_CHECK(x.dim() >= 2 && x.dim() <= 4, "x must have shape [heads, head_dim], [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]");
     TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "x must have dtype torch.float16 or torch.bfloat16");
     TORCH_CHECK(x.size(-1) >= 2 && x.size(-1) <= 256 && x.size(-1) % 2 == 0, "head_dim must be even, between 2 and 256");
@@ -132,18 +138,21 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
     } else {
         out = at::detail::empty_cuda(x.sizes(), x.scalar_type(), x.device(), c10::nullopt);
     }
-    auto whole = [&](const at::Tensor& t) {
-        at::Tensor four = t;
-        while (four.dim() < 4) four = four.unsqueeze(0);
-        return four;
+    TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type(), "out must be on the device of x and of its dtype");
+    TORCH_CHECK(x.numel() == 0 || (x.stride(-1) == 1 && out.stride(-1) == 1), "the last dimension of x and out must be contiguous");
+    // (as [batch, tokens, heads, head_dim], dimensions that are not there having one entry)
+    const int64_t missing = 4 - x.dim();
+    auto size = [&](int64_t dim) { return dim < missing ? 1 : x.size(dim - missing); };
+    auto rows = [&](const at::Tensor& t) {
+        auto stride = [&](int64_t dim) { return dim < missing ? 0 : t.stride(dim - missing); };
+        return w4a16_rows{t.data_ptr(), stride(0), stride(1), stride(2)};
     };
-    const at::Tensor x4 = whole(x), out4 = whole(out);
-    const w4a16_rows from = rows_of(x4, x.device(), x.scalar_type(), "x"), to = rows_of(out4, x.device(), x.scalar_type(), "out");
-    const int64_t* at_positions = words_of(positions, x.device(), x4.size(0) * x4.size(1), "positions");
+    const w4a16_rows from = rows(x), to = rows(out);
+    const int64_t* at_positions = words_of(positions, x.device(), size(0) * size(1), "positions");
     if (x.numel() > 0) {
         pybind11::gil_scoped_release unlocked;
-        check_status(w4a16_rotary(&spec, &from, &to, x4.size(0), x4.size(1), static_cast<int32_t>(x4.size(2)),
-                                  static_cast<int32_t>(x4.size(3)), at_positions,
+        check_status(w4a16_rotary(&spec, &from, &to, size(0), size(1), static_cast<int32_t>(size(2)),
+                                  static_cast<int32_t>(size(3)), at_positions,
                                   x.scalar_type() == at::kBFloat16 ? W4A16_TYPE_BF16 : W4A16_TYPE_F16, flags, current_stream()),
                      "apply_rotary");
     }
@@ -159,10 +168,10 @@ PyObject* kv8_bytes(PyObject*, PyObject* const* args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
-// kv8_append(cache..., k, v, start, counts or None, inv_freq or None, rope_scale, interleaved, q or None, programmatic) -> turned q or None
+// kv8_append(cache..., k, v, start, counts or None, inv_freq or None, rope_scale, interleaved, q or None) -> turned q or None
 PyObject* kv8_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    check_count(count, kCacheArguments + 9, "kv8_append");
+    check_count(count, kCacheArguments + 8, "kv8_append");
     const Cache cache = cache_of(args);
     args += kCacheArguments;
     const at::Tensor& k = tensor_of(args[0], "k");
@@ -173,7 +182,7 @@ PyObject* kv8_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     const double rope_scale = number_of(args[5]);
     const bool interleaved = truth_of(args[6]);
     const std::optional<at::Tensor> q = optional_of(args[7], "q");
-    const uint32_t flags = launch_flags(truth_of(args[8]));
+    const uint32_t flags = launch_flags();
     const at::Device device = cache.memory.device();
     const at::ScalarType dtype = dtype_of(cache.parts.type);
     const w4a16_rows k_rows = rows_of(k, device, dtype, "k"), v_rows = rows_of(v, device, dtype, "v");
@@ -209,16 +218,16 @@ PyObject* kv8_append(PyObject*, PyObject* const* args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
-// kv8_read(cache..., lengths, first or None, tokens, programmatic) -> (k, v)
+// kv8_read(cache..., lengths, first or None, tokens) -> (k, v)
 PyObject* kv8_read(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    check_count(count, kCacheArguments + 4, "kv8_read");
+    check_count(count, kCacheArguments + 3, "kv8_read");
     const Cache cache = cache_of(args);
     args += kCacheArguments;
     const at::Tensor& lengths = tensor_of(args[0], "lengths");
     const std::optional<at::Tensor> first = optional_of(args[1], "first");
     const int64_t tokens = integer_of(args[2]);
-    const uint32_t flags = launch_flags(truth_of(args[3]));
+    const uint32_t flags = launch_flags();
     TORCH_CHECK(tokens >= 0, "tokens must not be negative");
     const at::Device device = cache.memory.device();
     const int64_t* length = words_of(lengths, device, cache.parts.batch, "lengths");
@@ -241,17 +250,17 @@ PyObject* kv8_read(PyObject*, PyObject* const* args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
-// kv8_attention(cache..., q, lengths, counts or None, softmax_scale, programmatic) -> Tensor
+// kv8_attention(cache..., q, lengths, counts or None, softmax_scale) -> Tensor
 PyObject* kv8_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    check_count(count, kCacheArguments + 5, "kv8_attention");
+    check_count(count, kCacheArguments + 4, "kv8_attention");
     const Cache cache = cache_of(args);
     args += kCacheArguments;
     const at::Tensor& q = tensor_of(args[0], "q");
     const at::Tensor& lengths = tensor_of(args[1], "lengths");
     const std::optional<at::Tensor> counts = optional_of(args[2], "counts");
     const double softmax_scale = number_of(args[3]);
-    const uint32_t flags = launch_flags(truth_of(args[4]));
+    const uint32_t flags = launch_flags();
     const at::Device device = cache.memory.device();
     const at::ScalarType dtype = dtype_of(cache.parts.type);
     const w4a16_rows q_rows = rows_of(q, device, dtype, "q");

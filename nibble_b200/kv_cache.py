@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from .cuda import _require_extension, programmatic_launch_enabled
+from .cuda import _require_extension
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -43,7 +43,7 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     of ``inv_freq`` (FP32) and ``scale``.  Angles are formed in FP64, the rest in FP32, rounded once.  ``positions`` (int64) has the
     shape of ``x`` without its last two dimensions.  ``out`` may be ``x`` itself, or a tensor that shares no memory with it.
     """
-    return _extension().rotary(x, positions, inv_freq, scale, interleaved, out, programmatic_launch_enabled())
+    return _extension().rotary(x, positions, inv_freq, scale, interleaved, out)
 
 
 class QuantizedKVCache:
@@ -83,15 +83,13 @@ class QuantizedKVCache:
         With ``inv_freq`` the keys are turned to their positions on the way, and so are the queries ``q`` ``[batch, tokens, q_heads,
         head_dim]``, which are returned: the same bits as ``apply_rotary`` in front, in the same launch.
         """
-        return _extension().kv8_append(self.memory, *self._sizes, k, v, start, counts, inv_freq, rope_scale, interleaved, q,
-                                       programmatic_launch_enabled())
+        return _extension().kv8_append(self.memory, *self._sizes, k, v, start, counts, inv_freq, rope_scale, interleaved, q)
 
     def read(self, lengths: torch.Tensor, first: torch.Tensor | None = None,
              tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """What the cache holds: keys and values ``[batch, tokens, kv_heads, head_dim]`` from position ``first[b]`` (default: 0)
         on, of sequences of ``lengths[b]`` tokens; zeros behind the last.  ``tokens`` defaults to ``max_len``."""
-        return _extension().kv8_read(self.memory, *self._sizes, lengths, first, self.max_len if tokens is None else tokens,
-                                     programmatic_launch_enabled())
+        return _extension().kv8_read(self.memory, *self._sizes, lengths, first, self.max_len if tokens is None else tokens)
 
     def attention(self, q: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None,
                   softmax_scale: float | None = None) -> torch.Tensor:
@@ -103,8 +101,7 @@ class QuantizedKVCache:
         rows that see nothing, are zeros.
         """
         return _extension().kv8_attention(self.memory, *self._sizes, q, lengths, counts,
-                                          self.head_dim ** -0.5 if softmax_scale is None else softmax_scale,
-                                          programmatic_launch_enabled())
+                                          self.head_dim ** -0.5 if softmax_scale is None else softmax_scale)
 
     def check(self) -> None:
         """Raises if a call since the last check was given a length, start or count that does not fit, or gave up a bounded wait.
