@@ -194,7 +194,7 @@ rotary_kernel(const RotaryParams p) {
 
 // ------------------------------------------------------------------ tokens into the cache
 
-constexpr int64_t kAppendCtas = 148 * 8;          // two rounds of what the SMs hold
+constexpr int kAppendThreads = 768;               // of an SM: what 80 registers each allow
 
 struct AppendParams {
     KvCache cache;
@@ -315,7 +315,7 @@ __device__ __forceinline__ float scale_of(float top) {
 // the numbers themselves go to the tail, into the slot of the block's parity.  The CTA of the first block reads a tail slot that the
 // newest blocks may write, so it writes that slot itself, after it has read.
 template <typename T, int D, bool ROTARY>
-__global__ void __launch_bounds__(2 * D, (ROTARY ? 768 : 1024) / (2 * D))
+__global__ void __launch_bounds__(2 * D, kAppendThreads / (2 * D))
 kv_append_kernel(const AppendParams p) {
     constexpr int kThreads = 2 * D, kWarps = kThreads / 32;
     extern __shared__ __align__(16) float2 factors[];                              // [32][rotary_dim / 2]
@@ -435,9 +435,24 @@ kv_append_kernel(const AppendParams p) {
     // A newest block of the first one's parity shares its tail slot: the first one's CTA writes it, if it read that slot.
     const int shared = ((newest - first_block) & 1) == 0 ? newest : newest - 1;
     const bool first_reads = begin % kKvBlock != 0 && first_block < newest && shared > first_block;
-    uint32_t k[8], v[8];
+    uint32_t k[8], v[8], next_k[8], next_v[8];
+    // A block ahead (2 x 8191 tokens of 8 heads of 128 written and read back: 42 us, each block fetched in its turn 50; where keys are
+    // turned the cosines take the registers).
+    auto ask = [&](int block) {
+        if (!ROTARY && block * kKvBlock < end) fetch(block, next_k, next_v);
+    };
+    ask(first_block + chunk);
     for (int block = first_block + chunk; block * kKvBlock < end; block += p.chunks) {
-        fetch(block, k, v);
+        if (ROTARY) {
+            fetch(block, k, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                k[i] = next_k[i];
+                v[i] = next_v[i];
+            }
+            ask(block + p.chunks);
+        }
         if (block < newest) {                                             // all of its 32 tokens are there
             unsigned k_bits = __reduce_max_sync(0xffffffffu, magnitude16<T>(k)), v_bits = __reduce_max_sync(0xffffffffu, magnitude16<T>(v));
             if (lane == 0) {
@@ -640,7 +655,8 @@ int launch_kv_append(const w4a16_kv8_cache& cache, const w4a16_rows& k, const w4
     // (tokens beyond the cache are refused on the device; here they would only make CTAs without work)
     const int64_t at_most = tokens < cache.max_len ? tokens : cache.max_len;
     const int64_t pairs = static_cast<int64_t>(cache.batch) * cache.kv_heads, touched = (at_most + 2 * kKvBlock - 2) / kKvBlock;
-    p.chunks = static_cast<int>(std::min(touched, std::max<int64_t>(1, kAppendCtas / pairs)));
+    const int64_t resident = 148 * (kAppendThreads / (2 * cache.head_dim));
+    p.chunks = static_cast<int>(std::min(touched, std::max<int64_t>(1, resident / pairs)));
     int64_t ctas = pairs * p.chunks;
     size_t smem = 0;
     if (rotary != nullptr) {
