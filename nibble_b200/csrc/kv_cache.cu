@@ -6,7 +6,9 @@
 // (interpolated, by parts, with a temperature) change inv_freq and scale and nothing here.  At a position of 10^6 an FP32 angle
 // is off by up to 0.03, so the angle is formed and reduced to a turn in FP64; from there on FP32, rounded once.
 //
-// Bounds: all three are made of one pass over their data, HBM for prompts and launch latency for a token.
+// Bounds: all three are made of one pass over their data, HBM for prompts and launch latency for a token.  Measured, of 6.5 TB/s
+// that a copy reaches: 4096 tokens of 72 heads of 128 turned 28.7 us (5.3 TB/s); 2 x 8191 tokens of 8 heads of 128 written 23 us (4.3);
+// 32768 tokens read back 36 us (5.6); one token turned or read back 2.3 us, written 2.2, turned and written 3.9 with its queries.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

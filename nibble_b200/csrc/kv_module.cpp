@@ -96,7 +96,7 @@ w4a16_rotary_spec spec_of(const at::Tensor& inv_freq, const at::Device& device, 
 
 w4a16_stream_t current_stream() { return reinterpret_cast<w4a16_stream_t>(at::cuda::getCurrentCUDAStream().stream()); }
 
-// (what nibble_b200.cuda.programmatic_launch_enabled() says, which takes Python a third of such a call)
+// (what nibble_b200.cuda.programmatic_launch_enabled() says; asked here, since looking it up in Python shows in a call of 5 us)
 uint32_t launch_flags() {
     const char* knob = std::getenv("W4A16_PDL");
     return knob != nullptr && std::strcmp(knob, "1") == 0 ? W4A16_FLAG_PROGRAMMATIC_LAUNCH : 0u;

@@ -319,7 +319,6 @@ kv_prefill_kernel(const PrefillParams p) {
     __shared__ int odd_tail[4];                          // number of the work (plus one) whose tail's values have an infinity or NaN
     uint8_t* const shared = unaligned + (1024 - (smem_u32(unaligned) & 1023)) % 1024;
     pdl_wait_for_upstream();
-    pdl_release_downstream();
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     if (tid == 0) {
@@ -349,6 +348,7 @@ kv_prefill_kernel(const PrefillParams p) {
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_word;
+    pdl_release_downstream();                  // (behind the allocation: a kernel that starts beside this one may want TMEM too)
     bool healthy = true;
     // Waits for phase number `n` of a barrier; by a converged warp, all of whose lanes then know whether it came.
     auto wait = [&](unsigned long long& bar, int n) {

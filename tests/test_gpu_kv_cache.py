@@ -442,7 +442,95 @@ def test_queries_at_any_stride_and_address():
     cache.append(k[:, :0], v[:, :0], _words(lengths))
 
 
+@pytest.mark.parametrize(("tokens", "kv_heads", "head_dim"), [(1, 4, 64), (20, 2, 128), (5, 3, 64)])
+def test_more_sequences_than_the_machine_holds_at_once(tokens, kv_heads, head_dim):
+    """Runs and units that cross sequences, and rounds of whole units in front of ones that are cut."""
+    g = torch.Generator().manual_seed(tokens)
+    lengths = torch.randint(0, 131, (170,), generator=g).tolist()
+    counts = [min(length, int(torch.randint(0, tokens + 1, (1,), generator=g))) for length in lengths]
+    cache, k, v = _filled(170, kv_heads, 130, head_dim, torch.float16, lengths)
+    q = _draw((170, tokens, 8 * kv_heads, head_dim), torch.float16, 48)
+    _check_attention(cache, k, v, q, lengths, counts)
+    cache.check()
+
+
+def test_offsets_that_pass_32_bits():
+    """Eight heads of 2.2 million positions: codes of 2.25 GB each, of which the last two hundred positions are not zeros."""
+    max_len, d, heads, some = 2_200_000, 128, 8, 203
+    cache = QuantizedKVCache(1, heads, max_len, d)
+    assert cache.memory.numel() > 1 << 32
+    start = (max_len - some) // 32 * 32
+    k, v = _draw((1, some, heads, d), torch.float16, 50), _draw((1, some, heads, d), torch.float16, 51, 100.0)
+    cache.append(k, v, _words([start]))
+    length = start + some
+    for got, x in zip(cache.read(_words([length]), first=_words([start - 5]), tokens=some + 5), (k, v)):
+        assert not got[:, :5].any() and torch.equal(got[:, 5:], _held(x, [some]))
+    for count in (1, 70):
+        # (scores of ten and more, so that the others do not vanish among two million of zero)
+        q = 6.0 * k[:, some - count:some].repeat_interleave(2, 2)
+        got = cache.attention(q, _words([length]), softmax_scale=0.02)
+        kh, vh = oracle.held(k[0], some), oracle.held(v[0], some)
+        for i in range(count):
+            seen = some - count + i + 1
+            score = torch.einsum("hd,thd->ht", q[0, i].double(), kh[:seen].repeat_interleave(2, 1)) * 0.02
+            p = score.exp()
+            p = p / (p.sum(-1, keepdim=True) + start)
+            want = torch.einsum("ht,thd->hd", p, vh[:seen].repeat_interleave(2, 1))
+            weight = torch.einsum("ht,thd->hd", p, vh[:seen].abs().repeat_interleave(2, 1))
+            bound = oracle.attention_bound(want, weight, torch.float16, float(vh.abs().max()) * some)
+            # (and FP32 sums of two million numbers: their own terms' roundings, at most a thousand to a run)
+            assert ((got[0, i].double() - want).abs() <= bound + weight * 2.0 ** -14).all(), i
+    cache.check()
+
+
 # ------------------------------------------------------------------ as they are used together
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_programmatic_launches_change_nothing(head_dim, monkeypatch):
+    """Each kernel started while the one in front ends: steps and chunks in a row, where every call reads what the last one wrote."""
+    inv_freq = (10000.0 ** (-torch.arange(0, head_dim, 2).double() / head_dim)).float().cuda()
+    chunks = [64, 1, 1, 40, 200, 1, 33, 1]
+    rows = _draw((2, sum(chunks), 12, head_dim), torch.float16, 49)
+
+    def run():
+        cache = QuantizedKVCache(2, 2, 360, head_dim)
+        lengths, outs, at = _words([0, 0]), [], 0
+        for tokens in chunks:
+            q, k, v = (part.clone() for part in rows[:, at:at + tokens].split([8, 2, 2], 2))
+            apply_rotary(k, (lengths[:, None] + torch.arange(tokens, device="cuda")), inv_freq, out=k)
+            q = cache.append(k, v, lengths, q=q, inv_freq=torch.zeros_like(inv_freq))
+            lengths += tokens
+            outs += [cache.attention(q, lengths), *cache.read(lengths)]
+            at += tokens
+        cache.check()
+        return outs
+
+    monkeypatch.delenv("W4A16_PDL", raising=False)
+    want = run()
+    monkeypatch.setenv("W4A16_PDL", "1")
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(run(), want))
+    cache = QuantizedKVCache(2, 2, 360, head_dim)
+    lengths = [_words([n, n]) for n in range(0, 351, 50)]
+    parts = [part.contiguous() for part in rows[:, :350].split([8, 2, 2], 2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):                       # seven chunks in a row, nothing between the launches
+        outs = []
+        for i in range(7):
+            q, k, v = (part[:, 50 * i:50 * i + 50] for part in parts)
+            outs.append(cache.attention(cache.append(k, v, lengths[i], q=q, inv_freq=inv_freq), lengths[i + 1]))
+    graph.replay()
+    first = [out.clone() for out in outs]
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(outs, first))
+    monkeypatch.delenv("W4A16_PDL")
+    plain = QuantizedKVCache(2, 2, 360, head_dim)
+    for i in range(7):
+        q, k, v = (part[:, 50 * i:50 * i + 50] for part in parts)
+        assert torch.equal(plain.attention(plain.append(k, v, lengths[i], q=q, inv_freq=inv_freq), lengths[i + 1]), first[i])
+    plain.check()
+    cache.check()
+
 
 def test_a_generation_in_a_captured_graph():
     """Steps of turning, writing and attending, captured once and replayed with the position in device memory, two such graphs by
