@@ -356,6 +356,28 @@ kv_attention_kernel(const AttentionParams p) {
         load_scales(first_block);
 
         const int rows = seg.count * p.group, first_row = seg.tile * kTileRows;
+        // The queries, requested in front of the codes: a thread takes sixteen dims of a row.
+        constexpr int kPieces = (kTileRows * kSteps + kThreads - 1) / kThreads;       // of a thread
+        uint32_t pieces[kPieces][8];
+#pragma unroll
+        for (int e = 0; e < kPieces; ++e) {
+            const int at = tid + e * kThreads, row = first_row + at / kSteps, token = by_group(p, row);
+            const bool there = at < kTileRows * kSteps && row < rows;
+            const T* from = reinterpret_cast<const T*>(p.q) + seg.b * p.q_batch + token * p.q_token +
+                            (seg.head * p.group + row - token * p.group) * p.q_head + at % kSteps * 16;
+            uint32_t (&raw)[8] = pieces[e];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[i] = 0;
+            if (there && p.q_wide) {
+                const uint4 a = *reinterpret_cast<const uint4*>(from), b = *(reinterpret_cast<const uint4*>(from) + 1);
+                raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+                raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
+            } else if (there) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
+            }
+        }
         if (first_segment && member == 0) {        // the ring's first slots: a lane for each, as far as this segment goes
             const int now = min(kSlots, 2 * coded);
             const uint8_t* keys = p.cache.k_codes + (pair * p.cache.blocks + first_block) * Shape::kSlotBytes;
@@ -375,24 +397,13 @@ kv_attention_kernel(const AttentionParams p) {
                 for (int i = now; i < kSlots; ++i) ask();
             }
         }
-        // The queries, as they become the second operand: [8-row tile][two steps of sixteen dims][lane][...], dims in the order of the
-        // codes' bytes.  A thread takes sixteen dims of a row.
-        for (int at = tid; at < kTileRows * kSteps; at += kThreads) {
-            const int tile_row = at / kSteps, chunk = at % kSteps, row = first_row + tile_row;
-            const bool there = row < rows;
-            const int token = by_group(p, row);
-            const T* from = reinterpret_cast<const T*>(p.q) + seg.b * p.q_batch + token * p.q_token +
-                            (seg.head * p.group + row - token * p.group) * p.q_head + chunk * 16;
-            uint32_t raw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (there && p.q_wide) {
-                const uint4 a = *reinterpret_cast<const uint4*>(from), b = *(reinterpret_cast<const uint4*>(from) + 1);
-                raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
-                raw[4] = b.x; raw[5] = b.y; raw[6] = b.z; raw[7] = b.w;
-            } else if (there) {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+        // They become the second operand: [8-row tile][two steps of sixteen dims][lane][...], dims in the order of the codes' bytes.
 #pragma unroll
-                for (int i = 0; i < 8; ++i) raw[i] = h[2 * i] | static_cast<uint32_t>(h[2 * i + 1]) << 16;
-            }
+        for (int e = 0; e < kPieces; ++e) {
+            const int at = tid + e * kThreads;
+            if (at >= kTileRows * kSteps) break;       // (all of a warp)
+            const int tile_row = at / kSteps, chunk = at % kSteps, row = first_row + tile_row;
+            uint32_t (&raw)[8] = pieces[e];
             float back = 1.0f;
             if constexpr (kBf16) {
                 // BF16 queries become FP16 by a power of two of their row's own: a number keeps all its bits unless it is 2^-23
@@ -418,7 +429,7 @@ kv_attention_kernel(const AttentionParams p) {
             }
             if (chunk == 0) {
                 row_scales[tile_row] = p.scale * back;
-                row_places[tile_row] = there ? seg.length - seg.count + token : INT_MAX;      // (a row that is not there: anything goes)
+                row_places[tile_row] = row < rows ? seg.length - seg.count + by_group(p, row) : INT_MAX;      // (a row that is not there: anything goes)
             }
         }
         __syncthreads();
