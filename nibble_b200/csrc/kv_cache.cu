@@ -74,9 +74,10 @@ struct RotaryRows {
     RowView in, out;
     int head_dim, rotary_dim;
     bool interleaved;
-    bool wide;                                   // rows can be read and written 16 bytes at a time
+    bool aligned;                                // rows can be read and written 16 bytes at a time,
+    bool wide;                                   // and so can either half of what is turned
     bool in_place;                               // what is not turned is there already
-    int pieces, piece_bits;                      // of a head, eight numbers or eight pairs each (wide), and bits that number them
+    int pieces, piece_bits;                      // of a head, eight numbers or eight pairs (wide) each, and bits that number them
 };
 
 // Turns `heads` heads from `first_head` on of `tokens` tokens; table[token * rotary_dim / 2 + pair] holds the factors.
@@ -135,12 +136,91 @@ __device__ __forceinline__ void rotate_rows_wide(const RotaryRows& r, const floa
     }
 }
 
+enum class Pairs { kInterleaved, kHalvesOfWords, kHalves };      // neighbours; half a head apart, an even or an odd number of places
+
+// The same where halves begin anywhere: a thread turns eight numbers that lie together, and reads each one's partner for itself.  The
+// pieces of a head are lanes of one warp, which has read all of them before it writes one (rows may be turned in place).  (4096 tokens
+// of 72 heads of 128: 90 numbers turned 49 us, 92 37, 90 in neighbouring pairs 35; number by number 171.)
+template <typename T, Pairs PAIRS>
+__device__ __forceinline__ void rotate_rows_aligned(const RotaryRows& r, const float2* table, long long b, long long first_token, int tokens,
+                                                    int first_head, int heads) {
+    constexpr int kBatch = 2;                    // heads requested together
+    const int half = r.rotary_dim / 2;
+    const int piece = threadIdx.x & ((1 << r.piece_bits) - 1), row = threadIdx.x >> r.piece_bits, rows = blockDim.x >> r.piece_bits;
+    const int d = piece * 8;
+    int abreast = 1;                             // heads that a pass takes side by side
+    while (abreast < heads && abreast < rows) abreast *= 2;
+    const int first = row & (abreast - 1);
+    for (int token_base = 0; token_base < tokens; token_base += rows / abreast) {
+        const int token = token_base + row / abreast;
+        const bool there = piece < r.pieces && token < tokens;
+        float2 f[8];                             // of each number: what it is multiplied with, and its partner
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int pair = PAIRS == Pairs::kInterleaved ? (d + i) / 2 : d + i < half ? d + i : d + i - half;
+            f[i] = there && d + i < r.rotary_dim ? table[token * half + pair] : make_float2(1.0f, 0.0f);
+            if (PAIRS == Pairs::kInterleaved ? i % 2 == 0 : d + i < half) f[i].y = -f[i].y;
+        }
+        const T* const in = row_of<T>(r.in, b, first_token + token, first_head);
+        unsigned place[8];                       // of its partner; numbers that are not turned are read themselves
+#pragma unroll
+        for (int i = 0; i < 8; ++i) place[i] = d + i < half ? d + i + half : d + i < r.rotary_dim ? d + i - half : d + i;
+        T* const out = const_cast<T*>(row_of<T>(r.out, b, first_token + token, first_head)) + d;
+        for (int head_base = 0; head_base < heads; head_base += kBatch * abreast) {
+            uint4 own[kBatch];
+            uint32_t partner[kBatch][4];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int head = head_base + e * abreast + first;
+                if (!there || head >= heads) break;
+                const T* from = in + head * r.in.head;
+                own[e] = *reinterpret_cast<const uint4*>(from + d);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    if (PAIRS == Pairs::kInterleaved) {
+                        partner[e][i / 2] = __byte_perm((&own[e].x)[i / 2], 0, 0x1032);
+                        continue;
+                    }
+                    if (PAIRS == Pairs::kHalvesOfWords) {
+                        partner[e][i / 2] = *reinterpret_cast<const uint32_t*>(from + place[i]);
+                    } else {
+                        const uint16_t* numbers = reinterpret_cast<const uint16_t*>(from);
+                        partner[e][i / 2] = numbers[place[i]] | static_cast<uint32_t>(numbers[place[i + 1]]) << 16;
+                    }
+                }
+            }
+            if (r.in_place) __syncwarp();
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int head = head_base + e * abreast + first;
+                if (!there || head >= heads) break;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    uint32_t& word = (&own[e].x)[i / 2];
+                    const float2 x = widen2<T>(word), y = widen2<T>(partner[e][i / 2]);
+                    // (rotary_first and rotary_second, the sign being in the factor)
+                    const uint32_t turned = narrow2<T>(__fmaf_rn(x.x, f[i].x, __fmul_rn(y.x, f[i].y)),
+                                                       __fmaf_rn(x.y, f[i + 1].x, __fmul_rn(y.y, f[i + 1].y)));
+                    if (d + i < r.rotary_dim) word = turned;      // (an even number of them)
+                }
+                *reinterpret_cast<uint4*>(out + head * r.out.head) = own[e];
+            }
+        }
+    }
+}
+
 template <typename T>
 __device__ void rotate_rows(const RotaryRows& r, const float2* table, long long b, long long first_token, int tokens, int first_head,
                             int heads) {
     if (r.wide) {
         if (r.interleaved) rotate_rows_wide<T, true>(r, table, b, first_token, tokens, first_head, heads);
         else rotate_rows_wide<T, false>(r, table, b, first_token, tokens, first_head, heads);
+        return;
+    }
+    if (r.aligned) {
+        if (r.interleaved) rotate_rows_aligned<T, Pairs::kInterleaved>(r, table, b, first_token, tokens, first_head, heads);
+        else if (r.rotary_dim % 4 == 0) rotate_rows_aligned<T, Pairs::kHalvesOfWords>(r, table, b, first_token, tokens, first_head, heads);
+        else rotate_rows_aligned<T, Pairs::kHalves>(r, table, b, first_token, tokens, first_head, heads);
         return;
     }
     const int half = r.rotary_dim / 2, pieces = half + (r.in_place ? 0 : r.head_dim - r.rotary_dim);      // pairs, and the rest
@@ -605,10 +685,11 @@ RowView view_of(const w4a16_rows& r) {
 }
 
 RotaryRows rotary_rows(const w4a16_rotary_spec& spec, const w4a16_rows& in, const w4a16_rows& out, int head_dim) {
-    RotaryRows rows{view_of(in), view_of(out), head_dim, spec.rotary_dim, spec.interleaved != 0, false, in.data == out.data, 0, 0};
-    rows.wide = wide_rows(in) && wide_rows(out) && head_dim % 8 == 0 &&
-                (spec.interleaved ? spec.rotary_dim : spec.rotary_dim / 2) % 8 == 0 && (head_dim - spec.rotary_dim) % 8 == 0;
-    rows.pieces = spec.rotary_dim / (spec.interleaved ? 8 : 16) + (rows.in_place ? 0 : (head_dim - spec.rotary_dim) / 8);
+    RotaryRows rows{view_of(in), view_of(out), head_dim, spec.rotary_dim, spec.interleaved != 0, false, false, in.data == out.data, 0, 0};
+    rows.aligned = wide_rows(in) && wide_rows(out) && head_dim % 8 == 0;
+    rows.wide = rows.aligned && (spec.interleaved ? spec.rotary_dim : spec.rotary_dim / 2) % 8 == 0;
+    rows.pieces = rows.wide ? spec.rotary_dim / (spec.interleaved ? 8 : 16) + (rows.in_place ? 0 : (head_dim - spec.rotary_dim) / 8)
+                            : (rows.in_place ? spec.rotary_dim + 7 : head_dim) / 8;
     while (1 << rows.piece_bits < rows.pieces) ++rows.piece_bits;
     return rows;
 }

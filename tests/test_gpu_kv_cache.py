@@ -38,7 +38,7 @@ def _held(x, lengths):
 @pytest.mark.parametrize(("shape", "rotary_dim", "interleaved"), [
     ((1, 5, 64), 64, False), ((1, 36, 64), 64, True), ((9, 3, 128), 96, True), ((9, 3, 128), 96, False), ((17, 40, 128), 62, False),
     ((3, 2, 7, 80), 40, False), ((2, 33, 9, 256), 256, True), ((5, 1, 2), 2, False), ((4, 6, 66), 34, True), ((3, 64), 48, False),
-    ((300, 72, 128), 128, False)])
+    ((300, 72, 128), 128, False), ((130, 72, 128), 90, False), ((70, 9, 64), 36, False), ((33, 40, 128), 50, True), ((6, 5, 256), 254, False)])
 def test_rotary_is_its_definition(shape, rotary_dim, interleaved, dtype):
     x = _draw(shape, dtype, sum(shape))
     g = torch.Generator().manual_seed(rotary_dim)
