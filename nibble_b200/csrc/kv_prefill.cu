@@ -25,8 +25,8 @@
 // measured, a step is 4530 with what starting and ending a piece costs (600 a step there), of which MMAs are under way in 3060 and a
 // softmax in 3400.
 //
-// Work split.  As many whole units as make full rounds of the CTAs; what is left of the last round is cut along the tokens, so that
-// all CTAs have a piece, and a small kernel adds the pieces up.  (2048 tokens of 64 heads on 8: 512 units, 148 CTAs.)
+// Work split.  As many whole units as make full rounds of the CTAs; what is left for the last round is cut along the tokens, where that
+// are half as many units as CTAs or fewer, and a small kernel adds the pieces up.  (2048 tokens of 64 heads on 8: 512 units, 148 CTAs.)
 //
 // Every wait is bounded; one that gives up sets the cache's status word, later ones return at once, and the CTA still runs to its
 // TMEM deallocation.
@@ -893,7 +893,8 @@ Split split_of(const w4a16_kv8_cache& cache, int q_heads, int64_t tokens, int sm
     // (a piece is worth two steps or more)
     const int64_t steps = (cache.max_len + kStepTokens - 1) / kStepTokens;
     s.pieces = rest > 0 ? std::max<int64_t>(1, std::min<int64_t>(sms / rest, steps / 2)) : 1;
-    s.grid = s.whole > 0 ? sms : rest * s.pieces;
+    if (s.pieces == 1) s.whole = s.units;            // (nothing to be added up: 128 units of D = 128 take 14 us less)
+    s.grid = s.whole > 0 ? std::min<int64_t>(s.units, sms) : rest * s.pieces;
     return s;
 }
 
