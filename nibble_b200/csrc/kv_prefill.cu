@@ -817,8 +817,9 @@ kv_prefill_kernel(const PrefillParams p) {
     }
 }
 
-// Adds up the pieces of the units that were cut; a warp for a row.
-template <typename T, int D>
+// Adds up the pieces of the units that were cut; a warp for a row, BATCH pieces requested together: two where there are no more (with eight
+// 2048 queries at 8192 take 488 us instead of 476), else eight (40 rows of one sequence of 8000 22 us, one by one 25).
+template <typename T, int D, int BATCH>
 __global__ void __launch_bounds__(128)
 kv_pieces_kernel(const PrefillParams p) {
     pdl_wait_for_upstream();
@@ -833,18 +834,37 @@ kv_pieces_kernel(const PrefillParams p) {
 #pragma unroll
     for (int d = 0; d < kDims; ++d) acc[d] = 0.0f;
     if (row < first.rows) {
-        for (int piece = 0; piece < p.pieces; ++piece) {
-            if (static_cast<long long>(first.stop) * piece / p.pieces == static_cast<long long>(first.stop) * (piece + 1) / p.pieces) continue;
-            const float* part = p.parts + (static_cast<size_t>(unit * p.pieces + piece) * kUnitRows + in_unit) * (D + 4);
-            const float2 state = *reinterpret_cast<const float2*>(part + D);
-            const float best = fmaxf(top, state.x), mine = exp2_fast(top - best), theirs = exp2_fast(state.x - best);
-            top = best;
-            weight = weight * mine + state.y * theirs;
+        for (int begin = 0; begin < p.pieces; begin += BATCH) {
+            float2 state[BATCH], numbers[BATCH][kDims / 2];
+            float best = top;
 #pragma unroll
-            for (int d = 0; d < kDims; d += 2) {
-                const float2 two = *reinterpret_cast<const float2*>(part + lane * kDims + d);
-                acc[d] = acc[d] * mine + two.x * theirs;
-                acc[d + 1] = acc[d + 1] * mine + two.y * theirs;
+            for (int e = 0; e < BATCH; ++e) {
+                const int piece = begin + e;
+                const bool some = piece < p.pieces && static_cast<long long>(first.stop) * piece / p.pieces <
+                                                          static_cast<long long>(first.stop) * (piece + 1) / p.pieces;
+                const float* part = p.parts + (static_cast<size_t>(unit * p.pieces + piece) * kUnitRows + in_unit) * (D + 4);
+                state[e] = some ? *reinterpret_cast<const float2*>(part + D) : make_float2(kNone, 0.0f);
+#pragma unroll
+                for (int d = 0; d < kDims / 2; ++d) {
+                    numbers[e][d] = some ? reinterpret_cast<const float2*>(part + lane * kDims)[d] : make_float2(0.0f, 0.0f);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) best = fmaxf(best, state[e].x);
+            const float mine = exp2_fast(top - best);
+            top = best;
+            weight *= mine;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) acc[d] *= mine;
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const float theirs = exp2_fast(state[e].x - best);
+                weight = fmaf(state[e].y, theirs, weight);
+#pragma unroll
+                for (int d = 0; d < kDims / 2; ++d) {
+                    acc[2 * d] = fmaf(numbers[e][d].x, theirs, acc[2 * d]);
+                    acc[2 * d + 1] = fmaf(numbers[e][d].y, theirs, acc[2 * d + 1]);
+                }
             }
         }
     }
@@ -944,7 +964,7 @@ int launch_kv_prefill(const w4a16_kv8_cache& cache, const w4a16_rows& q, void* o
         const int status = kv_launch(kv_prefill_kernel<T, kD>, dim3(static_cast<unsigned>(s.grid)), dim3(kPrefillThreads),
                                      PrefillShape<kD>::kSharedBytes, programmatic, stream, p);
         if (status != W4A16_OK || rest == 0) return status;
-        return kv_launch(kv_pieces_kernel<T, kD>, dim3(static_cast<unsigned>(rest * (kUnitRows / 4))), dim3(128), 0, true, stream, p);
+        return kv_launch(s.pieces <= 2 ? kv_pieces_kernel<T, kD, 2> : kv_pieces_kernel<T, kD, 8>, dim3(static_cast<unsigned>(rest * (kUnitRows / 4))), dim3(128), 0, true, stream, p);
     };
     using Small = std::integral_constant<int, 64>;
     using Large = std::integral_constant<int, 128>;
