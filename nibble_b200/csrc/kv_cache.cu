@@ -8,7 +8,7 @@
 //
 // Bounds: all three are made of one pass over their data, HBM for prompts and launch latency for a token.  Measured, of 6.5 TB/s
 // that a copy reaches: 4096 tokens of 72 heads of 128 turned 28.7 us (5.3 TB/s); 2 x 8191 tokens of 8 heads of 128 written 23 us (4.3);
-// 32768 tokens read back 36 us (5.6); one token turned or read back 2.3 us, written 2.2, turned and written 3.9 with its queries.
+// 32768 tokens read back 36 us (5.6); one token turned or read back 2.3 us, written 2.2, turned and written 3.0 with its queries.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -35,9 +35,9 @@ __device__ __forceinline__ const T* row_of(const RowView& v, long long b, long l
     return reinterpret_cast<const T*>(v.data) + b * v.batch + i * v.token + h * v.head;
 }
 
-__device__ __forceinline__ float2 rotary_factors(long long position, float inv_freq, float scale) {
-    constexpr double kTurnsPerRadian = 0.15915494309189533577;
-    double turns = static_cast<double>(position) * (static_cast<double>(inv_freq) * kTurnsPerRadian);
+__device__ __forceinline__ double turns_of(float inv_freq) { return static_cast<double>(inv_freq) * 0.15915494309189533577; }      // 1 / (2 pi)
+__device__ __forceinline__ float2 rotary_factors(long long position, double turns_each, float scale) {
+    double turns = static_cast<double>(position) * turns_each;
     turns -= rint(turns);
     float s, c;
     sincospif(static_cast<float>(2.0 * turns), &s, &c);
@@ -247,7 +247,8 @@ constexpr int kMaxRotaryDim = 256;
 
 struct RotaryParams {
     RotaryRows rows;
-    const long long* positions;                  // [batch * tokens]
+    const long long* positions;                  // [batch * tokens]; null: those from start[batch] on
+    const long long* start;
     const float* inv_freq;
     float scale;
     long long tokens;
@@ -267,7 +268,8 @@ rotary_kernel(const RotaryParams p) {
     const int tokens = static_cast<int>(min(static_cast<long long>(kRotaryTokens), p.tokens - first));
     const int half = p.rows.rotary_dim / 2;
     for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
-        table[i] = rotary_factors(p.positions[b * p.tokens + first + i / half], p.inv_freq[i % half], p.scale);
+        const long long token = first + i / half;
+        table[i] = rotary_factors(p.positions != nullptr ? p.positions[b * p.tokens + token] : p.start[b] + token, turns_of(p.inv_freq[i % half]), p.scale);
     }
     __syncthreads();
     const int first_head = part * p.heads_per_cta;
@@ -292,7 +294,7 @@ struct AppendParams {
     int rotary_dim;
     bool interleaved;
     RotaryRows q;
-    int q_heads, q_heads_per_cta, q_parts, q_tiles;        // q_parts == 0: no queries
+    int q_heads, q_heads_per_cta, q_parts;       // q_parts == 0: no queries
 };
 
 // Sixteen numbers of a row, as eight words.
@@ -406,20 +408,27 @@ kv_append_kernel(const AppendParams p) {
     pdl_release_downstream();
     pdl_wait_for_upstream();
     const int tid = threadIdx.x;
+    // The factors of tokens [from, to) of 32 whose first is at position `first`: a thread keeps to one pair, several tokens under way.
+    // (2048 tokens of 8 heads of 128 turned and written: 14.5 us; pairs and tokens numbered through, and partners read one by one, 24.7.)
+    auto form_factors = [&](long long first, int from, int to) {
+        const int half = p.rotary_dim / 2, pair = tid % (D / 2);
+        if (pair >= half) return;
+        const double turns = turns_of(p.inv_freq[pair]);
+#pragma unroll 4
+        for (int token = from + tid / (D / 2); token < to; token += kThreads / (D / 2)) {
+            factors[token * half + pair] = rotary_factors(first + token, turns, p.rope_scale);
+        }
+    };
     const unsigned cache_ctas = static_cast<unsigned>(p.cache.batch) * p.cache.kv_heads * p.chunks;
     if (ROTARY && blockIdx.x >= cache_ctas) {                         // queries
         const unsigned at = blockIdx.x - cache_ctas;
         const int part = at % p.q_parts;
-        const unsigned rest = at / p.q_parts;
-        const long long b = rest / p.q_tiles, first = static_cast<long long>(rest % p.q_tiles) * kKvBlock;
-        const int tokens = static_cast<int>(min(static_cast<long long>(kKvBlock), p.tokens - first)), half = p.rotary_dim / 2;
-        const long long start = p.start[b];
-        for (int i = tid; i < tokens * half; i += kThreads) {
-            factors[i] = rotary_factors(start + first + i / half, p.inv_freq[i % half], p.rope_scale);
-        }
+        const long long b = at / p.q_parts;
+        const int tokens = static_cast<int>(p.tokens);                // (a block's worth at most)
+        form_factors(p.start[b], 0, tokens);
         __syncthreads();
         const int head = part * p.q_heads_per_cta;
-        rotate_rows<T>(p.q, factors, b, first, tokens, head, min(p.q_heads_per_cta, p.q_heads - head));
+        rotate_rows<T>(p.q, factors, b, 0, tokens, head, min(p.q_heads_per_cta, p.q_heads - head));
         return;
     }
     const int chunk = blockIdx.x % p.chunks;
@@ -460,11 +469,7 @@ kv_append_kernel(const AppendParams p) {
         }
         if (ROTARY) {
             __syncthreads();
-            const int half = p.rotary_dim / 2;
-            const int from = max(0, begin - of_block * kKvBlock), to = min(kKvBlock, end - of_block * kKvBlock);      // the new tokens
-            for (int i = from * half + tid; i < to * half; i += kThreads) {
-                factors[i] = rotary_factors(static_cast<long long>(of_block) * kKvBlock + i / half, p.inv_freq[i % half], p.rope_scale);
-            }
+            form_factors(static_cast<long long>(of_block) * kKvBlock, max(0, begin - of_block * kKvBlock), min(kKvBlock, end - of_block * kKvBlock));
             __syncthreads();
         }
         if (whole && t < begin) {
@@ -475,6 +480,22 @@ kv_append_kernel(const AppendParams p) {
             if (ROTARY) {
                 const int half = p.rotary_dim / 2;
                 const float2* f = factors + slot * half;
+                if (!p.interleaved && half % 16 == 0) {               // the partners lie together too
+                    if (d0 >= p.rotary_dim) return;
+                    const bool upper = d0 >= half;
+                    uint32_t partner[8];
+                    load16<T>(from + (upper ? d0 - half : d0 + half), p.wide, partner);
+                    f += upper ? d0 - half : d0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 x = widen2<T>(k[i]), y = widen2<T>(partner[i]);
+                        const float4 two = *reinterpret_cast<const float4*>(f + 2 * i);
+                        const float2 f0 = make_float2(two.x, two.y), f1 = make_float2(two.z, two.w);
+                        k[i] = upper ? narrow2<T>(rotary_second(y.x, x.x, f0), rotary_second(y.y, x.y, f1))
+                                     : narrow2<T>(rotary_first(x.x, y.x, f0), rotary_first(x.y, y.y, f1));
+                    }
+                    return;
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int d = d0 + 2 * i;
@@ -704,11 +725,12 @@ int heads_per_cta(int heads, long long ctas) {
 
 }  // namespace
 
-int launch_rotary(const w4a16_rotary_spec& spec, const w4a16_rows& x, const w4a16_rows& out, int64_t batch, int64_t tokens, int heads,
-                  int head_dim, const long long* positions, bool bf16, bool programmatic, cudaStream_t stream) {
+static int turn_rows(const w4a16_rotary_spec& spec, const w4a16_rows& x, const w4a16_rows& out, int64_t batch, int64_t tokens, int heads,
+                     int head_dim, const long long* positions, const long long* start, bool bf16, bool programmatic, cudaStream_t stream) {
     RotaryParams p{};
     p.rows = rotary_rows(spec, x, out, head_dim);
     p.positions = positions;
+    p.start = start;
     p.inv_freq = spec.inv_freq;
     p.scale = spec.scale;
     p.tokens = tokens;
@@ -722,6 +744,11 @@ int launch_rotary(const w4a16_rotary_spec& spec, const w4a16_rows& x, const w4a1
     const dim3 grid(static_cast<unsigned>(tiles * batch * p.head_parts));
     auto kernel = bf16 ? rotary_kernel<__nv_bfloat16> : rotary_kernel<__half>;
     return kv_launch(kernel, grid, dim3(kRotaryThreads), 0, programmatic, stream, p);
+}
+
+int launch_rotary(const w4a16_rotary_spec& spec, const w4a16_rows& x, const w4a16_rows& out, int64_t batch, int64_t tokens, int heads,
+                  int head_dim, const long long* positions, bool bf16, bool programmatic, cudaStream_t stream) {
+    return turn_rows(spec, x, out, batch, tokens, heads, head_dim, positions, nullptr, bf16, programmatic, stream);
 }
 
 int launch_kv_append(const w4a16_kv8_cache& cache, const w4a16_rows& k, const w4a16_rows& v, int64_t tokens, const long long* start,
@@ -741,6 +768,7 @@ int launch_kv_append(const w4a16_kv8_cache& cache, const w4a16_rows& k, const w4
     const int64_t resident = 148 * (kAppendThreads / (2 * cache.head_dim));
     p.chunks = static_cast<int>(std::min(touched, std::max<int64_t>(1, resident / pairs)));
     int64_t ctas = pairs * p.chunks;
+    const bool bf16 = cache.type == W4A16_TYPE_BF16;
     size_t smem = 0;
     if (rotary != nullptr) {
         p.inv_freq = rotary->inv_freq;
@@ -748,18 +776,22 @@ int launch_kv_append(const w4a16_kv8_cache& cache, const w4a16_rows& k, const w4
         p.rotary_dim = rotary->rotary_dim;
         p.interleaved = rotary->interleaved != 0;
         smem = static_cast<size_t>(kKvBlock) * (rotary->rotary_dim / 2) * sizeof(float2);
-        if (q != nullptr) {
+        if (q != nullptr && tokens > kKvBlock) {
+            // Many queries are turned by a launch of their own (8191 tokens, 64 heads beside 8 of keys: 115 us with that, 127 by CTAs of
+            // the same launch).
+            if (const int status = turn_rows(*rotary, *q, *q_out, cache.batch, tokens, q_heads, cache.head_dim, nullptr, start, bf16, programmatic, stream);
+                status != W4A16_OK) {
+                return status;
+            }
+        } else if (q != nullptr) {
             p.q = rotary_rows(*rotary, *q, *q_out, cache.head_dim);
             p.q_heads = q_heads;
-            const int64_t tiles = (tokens + kKvBlock - 1) / kKvBlock;
-            p.q_heads_per_cta = heads_per_cta(q_heads, tiles * cache.batch);
+            p.q_heads_per_cta = heads_per_cta(q_heads, cache.batch);
             p.q_parts = (q_heads + p.q_heads_per_cta - 1) / p.q_heads_per_cta;
-            p.q_tiles = static_cast<int>(tiles);
-            ctas += tiles * cache.batch * p.q_parts;
+            ctas += static_cast<int64_t>(cache.batch) * p.q_parts;
         }
     }
     if (ctas > INT32_MAX) return W4A16_ERR_TOO_LARGE;
-    const bool bf16 = cache.type == W4A16_TYPE_BF16;
     auto pick = [&](auto turned) {
         constexpr bool kTurned = decltype(turned)::value;
         return cache.head_dim == 64 ? (bf16 ? kv_append_kernel<__nv_bfloat16, 64, kTurned> : kv_append_kernel<__half, 64, kTurned>)

@@ -81,7 +81,7 @@ class QuantizedKVCache:
         positions ``start[b], start[b] + 1, ...``; of sequence ``b`` the first ``counts[b]`` (default: all).
 
         With ``inv_freq`` the keys are turned to their positions on the way, and so are the queries ``q`` ``[batch, tokens, q_heads,
-        head_dim]``, which are returned: the same bits as ``apply_rotary`` in front, in the same launch.
+        head_dim]``, which are returned: the same bits as ``apply_rotary`` in front, for a few tokens in one launch.
         """
         return _extension().kv8_append(self.memory, *self._sizes, k, v, start, counts, inv_freq, rope_scale, interleaved, q)
 
