@@ -17,7 +17,7 @@
 //
 // The tiles share the columns of the scores: a softmax thread takes its row's into registers in one go, and the MMAs of the other
 // tile's scores, which that will want half a round later, follow in their place.  So neither softmax waits for its scores.
-// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 476 us: 1.01 PFLOP/s, of a measured 1.63 for a plain product.
+// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 481 us: 1.00 PFLOP/s, of a measured 1.63 for a plain product.
 // What it was before: 592 with columns for each tile and the probabilities in the scores' place, where a tile's next scores had to
 // wait for its last output, and its softmax for both; 670 with 64 tokens at a time, twice buffered, since MMAs of 64 columns read
 // twice as much shared memory a column; 505 with the maximum of every block sought before its probabilities.  Bounds: on paper MMAs
@@ -276,21 +276,11 @@ __device__ __forceinline__ constexpr int token_of(int column) {
 // 128-byte swizzle: where 16-byte chunk c of row r of a [rows][128 bytes] tile lies.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// What a tail's numbers are multiplied with to become FP16, and the scale that stands for it.  FP16 ones stay as they are.
+// Largest finite magnitude of `count` numbers (an even number of them), by a warp.
 template <typename T>
-__device__ __forceinline__ float tail_power(float top, float& scale) {
-    if constexpr (std::is_same<T, __half>::value) {
-        scale = 1.0f;
-        return 1.0f;
-    }
-    return power_for(top, scale);
-}
-
-// Largest finite magnitude of a warp's share of `numbers` (an even number of them), by all lanes.
-template <typename T>
-__device__ __forceinline__ float finite_top(const T* numbers, int count, int first, int step) {
+__device__ __forceinline__ float finite_top(const T* numbers, int count, int lane) {
     float top = 0.0f;
-    for (int i = first; i < count / 2; i += step) {
+    for (int i = lane; i < count / 2; i += 32) {
         const float2 f = widen2<T>(reinterpret_cast<const uint32_t*>(numbers)[i]);
         const float a = fabsf(f.x), b = fabsf(f.y);
         if (a <= 3.4028235e38f) top = fmaxf(top, a);
@@ -316,6 +306,7 @@ kv_prefill_kernel(const PrefillParams p) {
     // formed only when both tiles' probabilities of step n + 1 are there.
     __shared__ __align__(16) float scales[4][2][kStepBlocks];
     __shared__ float tops[2][4];
+    __shared__ __align__(16) float4 tail_factors[kDequantWarps];      // keys': what makes FP16 of them, the scale of that; values': the same
     __shared__ int odd_tail[4];                          // number of the work (plus one) whose tail's values have an infinity or NaN
     uint8_t* const shared = unaligned + (1024 - (smem_u32(unaligned) & 1023)) % 1024;
     pdl_wait_for_upstream();
@@ -429,7 +420,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 for (int o = 16; o > 0; o >>= 1) unit_scale = fmaxf(unit_scale, __shfl_xor_sync(0xffffffffu, unit_scale, o));
                 if (has_tail) {
                     float scale;
-                    tail_power<T>(kBf16 ? finite_top(v_tail, w.held * D, lane, 32) : 0.0f, scale);
+                    power_for(finite_top(v_tail, w.held * D, lane), scale);
                     unit_scale = fmaxf(unit_scale, scale);
                 }
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");      // (the last work's have been read)
@@ -585,10 +576,10 @@ kv_prefill_kernel(const PrefillParams p) {
         constexpr int kBlockBytes = kKvBlock * D;
         uint8_t* const codes = shared + Shape::kCodesAt + mine * 2 * kBlockBytes;      // of a block's keys, and of its values
         // Asks for a block's codes (which: 0 keys, 1 values), behind all lanes' reads of those before.
-        auto ask = [&](int which, size_t pair, int block) {
+        auto ask = [&](int which, int pair, int block) {
             const unsigned bar = smem_u32(&bars.codes[mine][which]);
             mbar_arrive_expect_tx(bar, kBlockBytes);
-            bulk_load(smem_u32(codes + which * kBlockBytes), (which == 0 ? p.cache.k_codes : p.cache.v_codes) + (pair * p.cache.blocks + block) * kBlockBytes,
+            bulk_load(smem_u32(codes + which * kBlockBytes), (which == 0 ? p.cache.k_codes : p.cache.v_codes) + (static_cast<size_t>(pair) * p.cache.blocks + block) * kBlockBytes,
                       kBlockBytes, bar);
         };
         int steps = 0, read = 0;                         // steps of all, this CTA's works one after the other; blocks of codes
@@ -596,18 +587,29 @@ kv_prefill_kernel(const PrefillParams p) {
         bool asked = false;                              // whether the next step's codes were asked for
         for (int n = 0; work_of(p, n, w); ++n) {
             if (w.stop <= w.begin) continue;
-            const size_t pair = static_cast<size_t>(w.b) * p.cache.kv_heads + w.head;
+            const int pair = w.b * p.cache.kv_heads + w.head;
             // the step behind this work's last
             Work after;
             int follower = n + 1;
             bool follows = work_of(p, follower, after);
             while (follows && after.stop <= after.begin) follows = work_of(p, ++follower, after);
-            const size_t after_pair = static_cast<size_t>(after.b) * p.cache.kv_heads + after.head;
+            const int after_pair = after.b * p.cache.kv_heads + after.head;
             const int after_block = after.begin * kStepBlocks + mine;
             const bool after_coded = follows && after_block < after.full;
             if (!asked && w.begin * kStepBlocks + mine < w.full && lane == 0) {
                 ask(0, pair, w.begin * kStepBlocks + mine);
                 ask(1, pair, w.begin * kStepBlocks + mine);
+            }
+            if (w.held > 0 && w.full % kStepBlocks == mine && w.full / kStepBlocks >= w.begin && w.full / kStepBlocks < w.stop) {
+                // What the numbers of the block that is being filled are multiplied with to become FP16, and the scale that stands for
+                // it.  FP16 keys stay as they are; values are brought to the size of codes, so that probabilities keep as many bits
+                // beside small ones.
+                const size_t tail = (static_cast<size_t>(pair) * 2 + (w.full & 1)) * kKvBlock * D;
+                float4 factors = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane), factors.y);
+                factors.z = power_for(finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane), factors.w);
+                if (lane == 0) tail_factors[mine] = factors;
+                __syncwarp();
             }
 #pragma unroll 1
             for (int step = w.begin; step < w.stop; ++step, ++steps) {
@@ -615,23 +617,26 @@ kv_prefill_kernel(const PrefillParams p) {
                 const bool coded = block < w.full, tail = block == w.full && w.held > 0;
                 const bool last = step + 1 == w.stop;
                 asked = last ? after_coded : block + kStepBlocks < w.full;
-                const size_t next_pair = last ? after_pair : pair;
+                const int next_pair = last ? after_pair : pair;
                 const int next_block = last ? after_block : block + kStepBlocks;
-                const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + (pair * 2 + (block & 1)) * kKvBlock * D;
-                const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (block & 1)) * kKvBlock * D;
+                const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + (static_cast<size_t>(pair) * 2 + (block & 1)) * kKvBlock * D;
+                const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (static_cast<size_t>(pair) * 2 + (block & 1)) * kKvBlock * D;
                 float k_scale = 0.0f, v_scale = 0.0f, k_by = 1.0f, v_by = 1.0f;
                 if (coded) {
-                    k_scale = p.cache.k_scales[pair * p.cache.blocks + block];
-                    v_scale = p.cache.v_scales[pair * p.cache.blocks + block];
+                    k_scale = p.cache.k_scales[static_cast<size_t>(pair) * p.cache.blocks + block];
+                    v_scale = p.cache.v_scales[static_cast<size_t>(pair) * p.cache.blocks + block];
                 } else if (tail) {
-                    k_by = tail_power<T>(kBf16 ? finite_top(k_tail, w.held * D, lane, 32) : 0.0f, k_scale);
-                    v_by = tail_power<T>(kBf16 ? finite_top(v_tail, w.held * D, lane, 32) : 0.0f, v_scale);
+                    const float4 factors = tail_factors[mine];
+                    k_by = factors.x;
+                    k_scale = factors.y;
+                    v_by = factors.z;
+                    v_scale = factors.w;
                 }
                 auto to_half = [&](uint32_t word, float by) {
-                    if constexpr (!kBf16) return word;
                     const float2 f = widen2<T>(word);
                     return pack_half(f.x * by, f.y * by);
                 };
+                auto key_to_half = [&](uint32_t word) { return kBf16 ? to_half(word, k_by) : word; };
                 // keys: row of a token, in the order of the columns (token_of)
                 if (coded) wait(bars.codes[mine][0], read);
                 if (steps >= 2) wait(bars.k_empty[stage], steps / 2 - 1);
@@ -664,7 +669,7 @@ kv_prefill_kernel(const PrefillParams p) {
                                 const uint32_t* raw = reinterpret_cast<const uint32_t*>(k_tail + token * D + i % kHalves * 64 + c * 16);
 #pragma unroll
                                 for (int e = 0; e < 8; e += 2) {
-                                    const uint32_t lo = to_half(raw[e], k_by), hi = to_half(raw[e + 1], k_by);
+                                    const uint32_t lo = key_to_half(raw[e]), hi = key_to_half(raw[e + 1]);
                                     words[e] = prmt(lo, hi, 0x5410);
                                     words[e + 1] = prmt(lo, hi, 0x7632);
                                 }

@@ -403,6 +403,22 @@ def test_what_is_masked_does_not_matter():
     assert got[0, 3, 2].isnan().all() and got[0, 3, 1].isfinite().all() and got[0, 4, 2].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads"), [(1, 8, 2), (5, 8, 2), (90, 8, 2), (300, 64, 1)])
+def test_many_light_tokens_beside_a_heavy_one(tokens, q_heads, kv_heads, dtype):
+    """Half of the result comes of thousands of small probabilities of small values: they keep their bits, whatever the block that is
+    being filled is held as."""
+    length = 8017
+    k = torch.zeros((1, length, kv_heads, 64), dtype=dtype, device="cuda")
+    k[:, 5] = 1.0
+    v = (0.001 * (1.0 + 0.2 * _draw((1, length, kv_heads, 64), torch.float32, 52).clamp(-2, 2))).to(dtype)
+    cache = QuantizedKVCache(1, kv_heads, length + 7, 64, dtype=dtype)
+    cache.append(k, v, _words([0]))
+    q = torch.full((1, tokens, q_heads, 64), 9.0 / 64, dtype=dtype, device="cuda")        # scores of nine, and of zero
+    _check_attention(cache, k, v, q, [length], None, 1.0)
+    cache.check()
+
+
 def test_large_bf16_numbers():
     """Beyond FP16's range, in queries, keys and values, in full blocks and in the tail."""
     k, v = _draw((1, 80, 1, 128), torch.bfloat16, 33, 1e6), _draw((1, 80, 1, 128), torch.bfloat16, 34, 1e9)
