@@ -17,7 +17,7 @@
 //
 // The tiles share the columns of the scores: a softmax thread takes its row's into registers in one go, and the MMAs of the other
 // tile's scores, which that will want half a round later, follow in their place.  So neither softmax waits for its scores.
-// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 481 us: 1.00 PFLOP/s, of a measured 1.63 for a plain product.
+// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 474 us: 1.01 PFLOP/s, of a measured 1.63 for a plain product.
 // What it was before: 592 with columns for each tile and the probabilities in the scores' place, where a tile's next scores had to
 // wait for its last output, and its softmax for both; 670 with 64 tokens at a time, twice buffered, since MMAs of 64 columns read
 // twice as much shared memory a column; 505 with the maximum of every block sought before its probabilities.  Bounds: on paper MMAs
@@ -650,7 +650,7 @@ kv_prefill_kernel(const PrefillParams p) {
                         *reinterpret_cast<uint4*>(at + swizzled(row, 2 * c + 1)) = make_uint4(words[4], words[5], words[6], words[7]);
                     };
                     if (coded) {
-#pragma unroll
+#pragma unroll 4                 // (all eight: 481 us instead of 474)
                         for (int i = 0; i < kVectors; ++i) {
                             const uint4 four = *reinterpret_cast<const uint4*>(codes + i * 512 + lane * 16);
                             uint32_t words[8];
@@ -690,7 +690,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 if (steps >= 2) wait(bars.v_empty[stage], steps / 2 - 1);
                 uint8_t* const to = shared + Shape::kValuesAt + stage * Shape::kValueBytes + mine / 2 * (D * 128);
                 if (coded || !tail) {
-#pragma unroll
+#pragma unroll 4
                     for (int i = 0; i < kVectors; ++i) {         // sixteen dims: [half of them][group of 16 tokens]
                         uint4 four = make_uint4(0u, 0u, 0u, 0u);
                         if (coded) four = *reinterpret_cast<const uint4*>(codes + kBlockBytes + i * 512 + lane * 16);
@@ -823,7 +823,7 @@ kv_prefill_kernel(const PrefillParams p) {
 }
 
 // Adds up the pieces of the units that were cut; a warp for a row, BATCH pieces requested together: two where there are no more (with eight
-// 2048 queries at 8192 take 488 us instead of 476), else eight (40 rows of one sequence of 8000 22 us, one by one 25).
+// 2048 queries at 8192 take 12 us more), else eight (40 rows of one sequence of 8000 22 us, one by one 25).
 template <typename T, int D, int BATCH>
 __global__ void __launch_bounds__(128)
 kv_pieces_kernel(const PrefillParams p) {
