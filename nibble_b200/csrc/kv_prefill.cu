@@ -2,7 +2,7 @@
 //
 // The same definition as kv_attention.cu, and the same arithmetic: codes are exact FP16 integers in both products, the keys' scales
 // multiply FP32 scores, the values' scales enter the probabilities before those are rounded to FP16 (relative to the largest scale
-// of the piece of work, times 2^10), maxima, sums and outputs are FP32.
+// of the piece of work, times 2^10; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
 //
 // A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
 // against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's sixteen warps, one CTA per SM:
@@ -17,7 +17,7 @@
 //
 // The tiles share the columns of the scores: a softmax thread takes its row's into registers in one go, and the MMAs of the other
 // tile's scores, which that will want half a round later, follow in their place.  So neither softmax waits for its scores.
-// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 474 us: 1.01 PFLOP/s, of a measured 1.63 for a plain product.
+// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 486 us: 0.99 PFLOP/s, of a measured 1.63 for a plain product.
 // What it was before: 592 with columns for each tile and the probabilities in the scores' place, where a tile's next scores had to
 // wait for its last output, and its softmax for both; 670 with 64 tokens at a time, twice buffered, since MMAs of 64 columns read
 // twice as much shared memory a column; 505 with the maximum of every block sought before its probabilities.  Bounds: on paper MMAs
@@ -503,14 +503,23 @@ kv_prefill_kernel(const PrefillParams p) {
                     for (int block = 0; block < kStepBlocks; ++block) {
                         uint32_t packed[16];
                         const float with = __log2f(weight[block]) - from;
+                        // Where results are FP16 the sum is of the probabilities as they were rounded, so that what a row's large ones were
+                        // off by goes out of its result: root mean square 1.4 times the result's own rounding at most, where it was up to
+                        // 1.6 (and 474 us, now 486).  Not of a block whose values are so small that its probabilities run out of bits.
+                        const bool as_rounded = !kBf16 && weight[block] >= 1.0f;
                         const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with);
                         uint64_t sums[2] = {0, 0};
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
                             const float2 x = both_of(fma2(pair_of(score[block * 32 + i], score[block * 32 + i + 1]), by2, with2));
-                            const float a = exp2_fast(x.x), b = exp2_fast(x.y);
-                            sums[i / 2 % 2] = add2(sums[i / 2 % 2], pair_of(a, b));
+                            float a = exp2_fast(x.x), b = exp2_fast(x.y);
                             packed[i / 2] = pack_half(a, b);
+                            if (as_rounded) {
+                                const float2 held = widen2<__half>(packed[i / 2]);
+                                a = held.x;
+                                b = held.y;
+                            }
+                            sums[i / 2 % 2] = add2(sums[i / 2 % 2], pair_of(a, b));
                         }
                         const float2 all = both_of(add2(sums[0], sums[1]));
                         largest_sum = fmaxf(largest_sum, all.x + all.y);
@@ -650,7 +659,7 @@ kv_prefill_kernel(const PrefillParams p) {
                         *reinterpret_cast<uint4*>(at + swizzled(row, 2 * c + 1)) = make_uint4(words[4], words[5], words[6], words[7]);
                     };
                     if (coded) {
-#pragma unroll 4                 // (all eight: 481 us instead of 474)
+#pragma unroll 4                 // (all eight: 7 us more)
                         for (int i = 0; i < kVectors; ++i) {
                             const uint4 four = *reinterpret_cast<const uint4*>(codes + i * 512 + lane * 16);
                             uint32_t words[8];

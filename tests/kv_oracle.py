@@ -67,8 +67,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, length: int, co
 
 
 def attention_bound(out: torch.Tensor, weight: torch.Tensor, dtype: torch.dtype, top: float) -> torch.Tensor:
-    """How far a kernel may be off: a probability is rounded to FP16, off by half a step, 2^-11 of itself; scores are FP32 sums of
-    exact products and their exponentials good to some 2^-18 of themselves (scores below 100: 100 * 2^-24 from each of a handful of
-    roundings), for which there is 2^-13; the result is rounded once to its type; and probabilities far below the largest are held in
-    steps of 2^-35 of it (``top`` is the largest |v| times the number of tokens)."""
-    return weight * (2.0 ** -11 + 2.0 ** -13) + out.abs() * torch.finfo(dtype).eps / 2 + top * 2.0 ** -34
+    """How far a kernel may be off: a probability is rounded to FP16, off by half a step, 2^-11 of itself, and where the sum is of the
+    rounded ones it is off by as much (sum p_i (1 + e_i) v_i / sum p_i (1 + e_i) with |e_i| <= 2^-11 differs from sum p_i v_i by
+    sum p_i e_i (v_i - out) to first order, at most 2^-11 of sum p |v| and 2^-11 of |out|); scores are FP32 sums of exact products
+    and their exponentials good to some 2^-18 of themselves (scores below 100: 100 * 2^-24 from each of a handful of roundings), for
+    which there is 2^-13; the result is rounded once to its type; and probabilities far below the largest are held in steps of 2^-35
+    of it (``top`` is the largest |v| times the number of tokens)."""
+    return weight * (2.0 ** -11 + 2.0 ** -13) + out.abs() * (2.0 ** -11 + torch.finfo(dtype).eps / 2) + top * 2.0 ** -34

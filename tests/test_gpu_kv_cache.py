@@ -419,6 +419,20 @@ def test_many_light_tokens_beside_a_heavy_one(tokens, q_heads, kv_heads, dtype):
     cache.check()
 
 
+@pytest.mark.parametrize("spread", [1.0, 3.0])
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads", "head_dim", "length"), [
+    (1, 32, 4, 64, 500), (1, 8, 1, 128, 3001), (4, 8, 1, 128, 700), (5, 16, 2, 64, 999)])
+def test_fp16_results_are_off_by_their_own_rounding(tokens, q_heads, kv_heads, head_dim, length, spread):
+    """Few rows: what a probability's rounding leaves is not lost, so that the bound's parts for it fall away."""
+    cache, k, v = _filled(1, kv_heads, length, head_dim, torch.float16, [length])
+    q = _draw((1, tokens, q_heads, head_dim), torch.float16, 53, spread)
+    got = cache.attention(q, _words([length]))[0].double()
+    kh, vh = oracle.held(k[0], length), oracle.held(v[0], length)
+    want, weight = oracle.attention(q[0], kh, vh, length, tokens, head_dim ** -0.5)
+    bound = oracle.attention_bound(want, weight, torch.float16, float(vh.abs().max()) * length) - (weight + want.abs()) * 2.0 ** -11
+    assert ((got - want).abs() <= bound).all()
+
+
 def test_large_bf16_numbers():
     """Beyond FP16's range, in queries, keys and values, in full blocks and in the tail."""
     k, v = _draw((1, 80, 1, 128), torch.bfloat16, 33, 1e6), _draw((1, 80, 1, 128), torch.bfloat16, 34, 1e9)
