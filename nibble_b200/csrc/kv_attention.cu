@@ -19,8 +19,8 @@
 // run has of a sequence and head goes to the workspace, and a second kernel, which starts beside the first, adds those parts up in
 // order and attends over the block that is being filled.
 //
-// Measured (64 query heads on 8, D = 128, in a graph): one token over 65501 29.4 us = 4.6 TB/s, of a measured 6.5 for a copy, of which
-// 5 us go by before the first block has arrived and 4 after the last; 48 sequences of up to 8192 tokens 72.7 us = 5.5 TB/s.  Short
+// Measured (64 query heads on 8, D = 128, in a graph): one token over 65501 29.7 us = 4.5 TB/s, of a measured 6.5 for a copy, of which
+// 5 us go by before the first block has arrived and 4 after the last; 48 sequences of up to 8192 tokens 73.0 us = 5.5 TB/s.  Short
 // contexts are latency: 500 tokens of 32 heads on 4, D = 64, 6.9 us, of which two kernels that do nothing would take 4.7.  (A warp that
 // went over a block that is not there while the first lengths are on their way, to have the loop's code at hand, made them 8.0.)
 #include <cuda_bf16.h>
@@ -213,8 +213,8 @@ struct AttentionShape {
 };
 
 // 8-row tiles of a warp in the variants for 32 and 64 rows: as many as its registers hold, since they share what makes FP16 of codes.
-// (D = 64, 32 query heads on 4: eight sequences of 8000 tokens, 40 rows: four tiles and two warps to a ring 37.4 us, two and four
-// 46.0; 24 rows 25.7 and 29.2; short sequences the same within 1 us.)
+// (D = 64, 32 query heads on 4, without the second product: eight sequences of 8000 tokens, 40 rows: four tiles and two warps to a ring
+// 37.4 us, two and four 46.0; 24 rows 25.7 and 29.2; short sequences the same within 1 us.)
 template <int D>
 constexpr int kWide = D == 64 ? 4 : 2;
 
