@@ -276,16 +276,20 @@ __device__ __forceinline__ constexpr int token_of(int column) {
 // 128-byte swizzle: where 16-byte chunk c of row r of a [rows][128 bytes] tile lies.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// Largest finite magnitude of `count` numbers (an even number of them), by a warp.
+// Largest finite magnitude of `count` numbers (an even number of them), by a warp; and whether one of them is an infinity or NaN.
 template <typename T>
-__device__ __forceinline__ float finite_top(const T* numbers, int count, int lane) {
+__device__ __forceinline__ float finite_top(const T* numbers, int count, int lane, bool* odd = nullptr) {
     float top = 0.0f;
+    bool strange = false;
     for (int i = lane; i < count / 2; i += 32) {
         const float2 f = widen2<T>(reinterpret_cast<const uint32_t*>(numbers)[i]);
         const float a = fabsf(f.x), b = fabsf(f.y);
         if (a <= 3.4028235e38f) top = fmaxf(top, a);
+        else strange = true;
         if (b <= 3.4028235e38f) top = fmaxf(top, b);
+        else strange = true;
     }
+    if (odd != nullptr) *odd = __any_sync(0xffffffffu, strange);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     return top;
@@ -307,7 +311,10 @@ kv_prefill_kernel(const PrefillParams p) {
     __shared__ __align__(16) float scales[4][2][kStepBlocks];
     __shared__ float tops[2][4];
     __shared__ __align__(16) float4 tail_factors[kDequantWarps];      // keys': what makes FP16 of them, the scale of that; values': the same
-    __shared__ int odd_tail[4];                          // number of the work (plus one) whose tail's values have an infinity or NaN
+    // Whether the values of a step's block that is being filled have an infinity or NaN: by steps like the scales, written and read at the
+    // same places.  (By works it would be overwritten: works without a step are passed over at once, and one tile may be at the end
+    // of a work while the other is in the next but three.)
+    __shared__ bool odd_tail[4][kStepBlocks];
     uint8_t* const shared = unaligned + (1024 - (smem_u32(unaligned) & 1023)) % 1024;
     pdl_wait_for_upstream();
     const int tid = threadIdx.x, lane = tid & 31;
@@ -324,7 +331,6 @@ kv_prefill_kernel(const PrefillParams p) {
             mbar_init(smem_u32(&bars.p_full[t]), 4);
             mbar_init(smem_u32(&bars.o_done[t]), 1);
         }
-        for (int i = 0; i < 4; ++i) odd_tail[i] = 0;
         for (int i = 0; i < kDequantWarps; ++i) {
             mbar_init(smem_u32(&bars.codes[i][0]), 1);
             mbar_init(smem_u32(&bars.codes[i][1]), 1);
@@ -369,6 +375,7 @@ kv_prefill_kernel(const PrefillParams p) {
             const bool has_tail = active && w.held > 0 && w.stop * kStepBlocks > w.full;
             const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (w.full & 1)) * kKvBlock * D;
             float top = kNone, sum = 0.0f, unit_scale = 0.0f, q_scale = p.scale;
+            bool odd = false;                            // the tail's values have an infinity or NaN
             if (active) {
                 // the row of queries: [half][row][128 bytes], dims in the order of the codes' bytes
                 uint8_t* const to = shared + t * Shape::kQueryBytes;
@@ -441,6 +448,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 // (and out of the sum again).  Either may be NaN; a row that sees nothing of the block is kept out of that.
                 const float4 k_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][0]);
                 const float4 v_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][1]);
+                if (has_tail && step + 1 == w.stop) odd = odd_tail[(steps_of_all + step - w.begin) & 3][w.full % kStepBlocks];
                 float by[kStepBlocks] = {k_scale.x, k_scale.y, k_scale.z, k_scale.w};
                 float weight[kStepBlocks] = {v_scale.x, v_scale.y, v_scale.z, v_scale.w};
                 const bool masked = (step + 1) * kStepTokens - 1 > lowest;
@@ -540,11 +548,9 @@ kv_prefill_kernel(const PrefillParams p) {
             const bool write = to_part ? active : row < p.tokens * p.group;
             T* out = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(w.b) * p.tokens + token) * p.q_heads + q_head) * D;
             const float by = to_part ? unit_scale / kHeadroom : sum > 0.0f ? unit_scale / kHeadroom / sum : sum;
-            bool odd = false;
             if (active) {
                 wait(bars.o_done[t], steps_done - 1);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                odd = has_tail && *const_cast<volatile int*>(&odd_tail[n & 3]) == n + 1;
             }
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
@@ -594,6 +600,7 @@ kv_prefill_kernel(const PrefillParams p) {
         int steps = 0, read = 0;                         // steps of all, this CTA's works one after the other; blocks of codes
         Work w;
         bool asked = false;                              // whether the next step's codes were asked for
+        bool odd_values = false;                         // of the tail, where it is this warp's
         for (int n = 0; work_of(p, n, w); ++n) {
             if (w.stop <= w.begin) continue;
             const int pair = w.b * p.cache.kv_heads + w.head;
@@ -616,7 +623,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 const size_t tail = (static_cast<size_t>(pair) * 2 + (w.full & 1)) * kKvBlock * D;
                 float4 factors = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
                 if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane), factors.y);
-                factors.z = power_for(finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane), factors.w);
+                factors.z = power_for(finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane, &odd_values), factors.w);
                 if (lane == 0) tail_factors[mine] = factors;
                 __syncwarp();
             }
@@ -690,6 +697,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 if (lane == 0) {
                     scales[steps & 3][0][mine] = k_scale;
                     scales[steps & 3][1][mine] = v_scale;
+                    if (tail) odd_tail[steps & 3][mine] = odd_values;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.k_full[stage]);
@@ -713,7 +721,6 @@ kv_prefill_kernel(const PrefillParams p) {
                         }
                     }
                 } else {
-                    bool odd_values = false;
                     for (int i = lane; i < 8 * (D / 8); i += 32) {      // eight dims of four tokens
                         const int quad = i / (D / 8), d0 = i % (D / 8) * 8;
                         uint32_t raw[4][4];
@@ -725,8 +732,8 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll
                             for (int f = 0; f < 4; ++f) {
                                 const float2 v = widen2<T>(raw[e][f]);
-                                if (!(fabsf(v.x) <= 3.4028235e38f)) raw[e][f] &= 0xffff0000u, odd_values = true;
-                                if (!(fabsf(v.y) <= 3.4028235e38f)) raw[e][f] &= 0x0000ffffu, odd_values = true;
+                                if (!(fabsf(v.x) <= 3.4028235e38f)) raw[e][f] &= 0xffff0000u;
+                                if (!(fabsf(v.y) <= 3.4028235e38f)) raw[e][f] &= 0x0000ffffu;
                                 raw[e][f] = to_half(raw[e][f], v_by);
                             }
                         }
@@ -741,7 +748,6 @@ kv_prefill_kernel(const PrefillParams p) {
                             }
                         }
                     }
-                    if (__any_sync(0xffffffffu, odd_values) && lane == 0) odd_tail[n & 3] = n + 1;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.v_full[stage]);
