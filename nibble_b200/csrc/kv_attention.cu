@@ -190,13 +190,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t pair) {
     return out;
 }
 
-// A power of two that brings `top` to between 2^9 and 2^10 (1 for zero), and its inverse.
-__device__ __forceinline__ float power_for(float top, float& inverse) {
-    const int exponent = top > 0.0f ? max(-100, min(100, 9 - ilogbf(top))) : 0;
-    inverse = __int_as_float((127 - exponent) << 23);
-    return __int_as_float((127 + exponent) << 23);
-}
-
 // A team of MT warps shares a ring; each has 8 * NT rows of its own, and the kWarps / MT teams take the blocks in turn.
 template <typename T, int D, int NT, int MT>
 struct AttentionShape {

@@ -121,6 +121,14 @@ __device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float a, float b) {
 // The power of two at or above a positive normal number.
 __device__ __forceinline__ float next_power(float x) { return __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0xff800000u); }
 
+// A power of two that brings `top`, finite and not negative, to between 2^9 and 2^10 (1 for zero), and its inverse.  Both are normal
+// numbers for all that FP32 has down to 2^-109; what is below that comes to less than 2^9, which loses none of its bits.
+__device__ __forceinline__ float power_for(float top, float& inverse) {
+    const int exponent = top > 0.0f ? min(118, 9 - ilogbf(top)) : 0;
+    inverse = __int_as_float((127 - exponent) << 23);
+    return __int_as_float((127 + exponent) << 23);
+}
+
 template <typename... Params, typename... Args>
 int kv_launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, bool programmatic, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t launch = {};

@@ -1,14 +1,15 @@
 // Attention of many new tokens (a prompt, or a chunk of one) over the 8-bit cache, on the 5th-generation tensor cores.
 //
-// The same definition as kv_attention.cu, and the same arithmetic: codes are exact FP16 integers in both products, the keys' scales
-// multiply FP32 scores, the values' scales enter the probabilities before those are rounded to FP16 (relative to the largest scale
-// of the piece of work, times 2^10; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
+// The same definition as kv_attention.cu, and the same arithmetic: codes are exact integers in both products (of FP16; scores of BF16
+// caches are products of BF16, so that queries and keys of any size keep their bits), the keys' scales multiply FP32 scores, the
+// values' scales enter the probabilities before those are rounded to FP16 (relative to the largest scale of the piece of work, times
+// 2^10; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
 //
 // A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
 // against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's sixteen warps, one CTA per SM:
 //   warps 0-3, 4-7   softmax of tile A and of tile B: a thread per row.  Stages its row of queries, then in every step takes the
 //                    row's 128 scores out of TMEM, leaves the probabilities there, and in the end takes the output.
-//   warps 8-11       make FP16 operands in shared memory of a block's codes each (which they have copied in a step ahead), swizzled by
+//   warps 8-11       make 16-bit operands in shared memory of a block's codes each (which they have copied in a step ahead), swizzled by
 //                    128 bytes: keys [token][d], values [d][token]; of the block that is being filled, of its 16-bit numbers; zeros
 //                    behind the last.
 //   warp 12          (13-15: nothing) allocates TMEM and issues the MMAs: S = Q K^T with both operands in shared memory, O += P V
@@ -186,14 +187,20 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float power_for(float top, float& inverse) {
-    const int exponent = top > 0.0f ? max(-100, min(100, 9 - ilogbf(top))) : 0;
-    inverse = __int_as_float((127 - exponent) << 23);
-    return __int_as_float((127 + exponent) << 23);
-}
 __device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& even, uint32_t& odd) {
     even = hsub2_u32(and_xor(word, 0x00ff00ffu, 0x64806480u), 0x64806480u);
     odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
+}
+// The same as BF16, whose seven bits behind the point hold a code's lower seven beside 128: the bit of its sign is what 256 has and 128 has
+// not.  (128 + lower seven) - (128 or 256).
+__device__ __forceinline__ uint32_t two_codes_to_bf16(uint32_t word) {
+    const uint32_t lower = (word & 0x007f007fu) | 0x43004300u, sign = (word & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 codes = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lower), *reinterpret_cast<const __nv_bfloat162*>(&sign));
+    return *reinterpret_cast<const uint32_t*>(&codes);
+}
+__device__ __forceinline__ void codes_to_bf16(uint32_t word, uint32_t& even, uint32_t& odd) {
+    even = two_codes_to_bf16(word);
+    odd = two_codes_to_bf16(word >> 8);
 }
 
 __device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
@@ -399,8 +406,7 @@ kv_prefill_kernel(const PrefillParams p) {
                     unit_scale = fmaxf(unit_scale, v_scales[block]);
                 }
                 if constexpr (kBf16) {
-                    // BF16 becomes FP16 by a power of two of the row's own: a number keeps all its bits unless it is 2^-23 of the
-                    // row's largest or less
+                    // by a power of two of the row's own, so that no product is beyond FP32 that the definition has within
                     uint32_t largest = 0;
 #pragma unroll
                     for (int i = 0; i < D / 2; ++i) largest = max(largest, max(raw[i] << 16 & 0x7fffffffu, raw[i] & 0x7fff0000u));
@@ -410,7 +416,7 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll
                     for (int i = 0; i < D / 2; ++i) {
                         const float2 f = widen2<T>(raw[i]);
-                        raw[i] = pack_half(f.x * by, f.y * by);
+                        raw[i] = narrow2<T>(f.x * by, f.y * by);
                     }
                 }
 #pragma unroll
@@ -617,9 +623,9 @@ kv_prefill_kernel(const PrefillParams p) {
                 ask(1, pair, w.begin * kStepBlocks + mine);
             }
             if (w.held > 0 && w.full % kStepBlocks == mine && w.full / kStepBlocks >= w.begin && w.full / kStepBlocks < w.stop) {
-                // What the numbers of the block that is being filled are multiplied with to become FP16, and the scale that stands for
-                // it.  FP16 keys stay as they are; values are brought to the size of codes, so that probabilities keep as many bits
-                // beside small ones.
+                // What the numbers of the block that is being filled are multiplied with, and the scale that stands for it.  FP16 keys
+                // stay as they are, BF16 ones stay BF16; values, which become FP16, are brought to the size of codes, so that
+                // probabilities keep as many bits beside small ones.
                 const size_t tail = (static_cast<size_t>(pair) * 2 + (w.full & 1)) * kKvBlock * D;
                 float4 factors = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
                 if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane), factors.y);
@@ -652,7 +658,15 @@ kv_prefill_kernel(const PrefillParams p) {
                     const float2 f = widen2<T>(word);
                     return pack_half(f.x * by, f.y * by);
                 };
-                auto key_to_half = [&](uint32_t word) { return kBf16 ? to_half(word, k_by) : word; };
+                auto key_operand = [&](uint32_t word) {
+                    if (!kBf16) return word;
+                    const float2 f = widen2<T>(word);
+                    return narrow2<T>(f.x * k_by, f.y * k_by);
+                };
+                auto key_codes = [&](uint32_t word, uint32_t& even, uint32_t& odd) {
+                    if (kBf16) codes_to_bf16(word, even, odd);
+                    else codes_to_half(word, even, odd);
+                };
                 // keys: row of a token, in the order of the columns (token_of)
                 if (coded) wait(bars.codes[mine][0], read);
                 if (steps >= 2) wait(bars.k_empty[stage], steps / 2 - 1);
@@ -670,10 +684,10 @@ kv_prefill_kernel(const PrefillParams p) {
                         for (int i = 0; i < kVectors; ++i) {
                             const uint4 four = *reinterpret_cast<const uint4*>(codes + i * 512 + lane * 16);
                             uint32_t words[8];
-                            codes_to_half(four.x, words[0], words[1]);
-                            codes_to_half(four.y, words[2], words[3]);
-                            codes_to_half(four.z, words[4], words[5]);
-                            codes_to_half(four.w, words[6], words[7]);
+                            key_codes(four.x, words[0], words[1]);
+                            key_codes(four.y, words[2], words[3]);
+                            key_codes(four.z, words[4], words[5]);
+                            key_codes(four.w, words[6], words[7]);
                             store(i, words);
                         }
                     } else {
@@ -685,7 +699,7 @@ kv_prefill_kernel(const PrefillParams p) {
                                 const uint32_t* raw = reinterpret_cast<const uint32_t*>(k_tail + token * D + i % kHalves * 64 + c * 16);
 #pragma unroll
                                 for (int e = 0; e < 8; e += 2) {
-                                    const uint32_t lo = key_to_half(raw[e]), hi = key_to_half(raw[e + 1]);
+                                    const uint32_t lo = key_operand(raw[e]), hi = key_operand(raw[e + 1]);
                                     words[e] = prmt(lo, hi, 0x5410);
                                     words[e + 1] = prmt(lo, hi, 0x7632);
                                 }
@@ -761,7 +775,8 @@ kv_prefill_kernel(const PrefillParams p) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssuerRegisters));
         // ---------------------------------------------------------------- MMAs
         constexpr uint32_t kCommon = (1u << 4) | (static_cast<uint32_t>(kRows >> 4) << 24);      // FP32 sums of FP16, 128 rows, K-major
-        constexpr uint32_t kScoreDesc = kCommon | (static_cast<uint32_t>(kStepTokens >> 3) << 17);
+        constexpr uint32_t kOfBf16 = kBf16 ? (1u << 7) | (1u << 10) : 0u;                        // both operands
+        constexpr uint32_t kScoreDesc = kCommon | kOfBf16 | (static_cast<uint32_t>(kStepTokens >> 3) << 17);
         constexpr uint32_t kOutputDesc = kCommon | (static_cast<uint32_t>(D >> 3) << 17);
         const bool chosen = elect_one();
         int steps = 0, works[2] = {0, 0};                // steps of all, up to this work; works of each tile

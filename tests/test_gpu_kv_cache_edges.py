@@ -7,7 +7,7 @@ import torch
 
 import kv_oracle as oracle
 from nibble_b200 import QuantizedKVCache, apply_rotary
-from test_gpu_kv_cache import _draw, _held, _words
+from test_gpu_kv_cache import _check_attention, _draw, _held, _words
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,29 @@ def test_infinities_of_the_newest_block_are_seen_beside_works_without_a_step(row
             assert (got[b, sees, :, 7] == float("inf")).all(), b
             assert got[b, ~sees].isfinite().all() and got[b, :, :, :7].isfinite().all() and got[b, :, :, 8:].isfinite().all(), b
     cache.check()
+
+
+@pytest.mark.parametrize("length", [20, 64, 90])
+@pytest.mark.parametrize(("tokens", "q_heads", "head_dim"), [(1, 4, 128), (5, 8, 64), (20, 16, 128), (20, 16, 64)])
+@pytest.mark.parametrize(("q_size", "k_size", "v_size"), [(120, -120, 117), (-122, 121, 0), (0, 0, -100), (118, -118, 1)])
+def test_bf16_numbers_of_any_size(q_size, k_size, v_size, tokens, q_heads, head_dim, length):
+    """Powers of two that all but use up the type's range, in few rows and many, in full blocks and in the one being filled."""
+    dtype = torch.bfloat16
+    k, v = (_draw((1, length, 1, head_dim), dtype, seed, 2.0 ** size) for seed, size in ((5, k_size), (6, v_size)))
+    q = _draw((1, tokens, q_heads, head_dim), dtype, 7, 2.0 ** q_size)
+    cache = QuantizedKVCache(1, 1, length + 3, head_dim, dtype=dtype)
+    cache.append(k, v, _words([0]))
+    _check_attention(cache, k, v, q, [length], None)
+    cache.check()
+
+
+@pytest.mark.parametrize(("tokens", "q_heads"), [(4, 8), (40, 8)])
+def test_a_key_far_out_does_not_cost_others_their_bits(tokens, q_heads):
+    """The block that is being filled, BF16, numbers of one key 10^12 times the others, which meet zeros in the queries."""
+    length = 50
+    k, v, q = (_draw((1, n, heads, 64), torch.bfloat16, seed) for n, heads, seed in ((length, 1, 8), (length, 1, 9), (tokens, q_heads, 10)))
+    k[:, length - 3, :, :8] *= 1e12
+    q[..., :8] = 0.0
+    cache = QuantizedKVCache(1, 1, 64, 64, dtype=torch.bfloat16)
+    cache.append(k, v, _words([0]))
+    _check_attention(cache, k, v, q, [length], None)
