@@ -473,13 +473,12 @@ kv_attention_kernel(const AttentionParams p) {
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    // relative to the maximum so far, or to zero while the row has seen nothing
-                    const bool fresh = top[n][r] == kNone;
-                    const float by = k_scale * q_scale[n][r], from = fresh ? 0.0f : -top[n][r], limit = fresh ? -INFINITY : kMaxLag;
+                    // (rounded here and the maximum taken off later: what is off by a rounding of 10^12 is then so for equal scores alike)
+                    const float by = k_scale * q_scale[n][r], limit = top[n][r] == kNone ? -INFINITY : top[n][r] + kMaxLag;
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
                         float& x = score[n][t >> 1][(t & 1) * 2 + r];
-                        x = fmaf(x, by, from);
+                        x *= by;
                         lag = lag || x > limit;
                     }
                 }
@@ -508,18 +507,14 @@ kv_attention_kernel(const AttentionParams p) {
                     float shrink[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const bool fresh = top[n][r] == kNone;
                         float more = fmaxf(fmaxf(score[n][0][r], score[n][0][2 + r]), fmaxf(score[n][1][r], score[n][1][2 + r]));
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) more = fmaxf(more, __shfl_xor_sync(0xffffffffu, more, o));
-                        if (!fresh) more = fmaxf(more, 0.0f);
-                        if (more == -INFINITY) more = 0.0f;               // still nothing seen
-                        else top[n][r] = fresh ? more : top[n][r] + more;
-                        shrink[r] = fresh ? 1.0f : exp2_fast(-more);
+                        more = fmaxf(more, top[n][r]);                    // (kNone while nothing has been seen)
+                        shrink[r] = top[n][r] == kNone ? 1.0f : exp2_fast(top[n][r] - more);
+                        top[n][r] = more;
                         sum[n][r] *= shrink[r];
                         shrink[r] *= unit_change;
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) score[n][t >> 1][(t & 1) * 2 + r] -= more;
                     }
 #pragma unroll
                     for (int j = 0; j < kSteps; ++j) {
@@ -541,12 +536,14 @@ kv_attention_kernel(const AttentionParams p) {
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                // relative to the maximum so far, or to zero while the row has seen nothing
+                const float from[2] = {top[n][0] == kNone ? 0.0f : top[n][0], top[n][1] == kNone ? 0.0f : top[n][1]};
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     float w[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float e = exp2_fast(score[n][t >> 1][(t & 1) * 2 + r]);
+                        const float e = exp2_fast(score[n][t >> 1][(t & 1) * 2 + r] - from[r]);
                         sum[n][r] += e;
                         w[r] = e * weight;
                     }

@@ -62,6 +62,7 @@ static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 
 constexpr float kNone = -1.0e30f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;
+constexpr float kFar = 0x1p16f;                 // a score that is so large is rounded before the maximum is taken off
 constexpr float kLargestSum = 65000.0f;         // of a block's probabilities times their values' scale: none is beyond FP16 then
 
 struct PrefillParams {
@@ -382,6 +383,7 @@ kv_prefill_kernel(const PrefillParams p) {
             const bool has_tail = active && w.held > 0 && w.stop * kStepBlocks > w.full;
             const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (w.full & 1)) * kKvBlock * D;
             float top = kNone, sum = 0.0f, unit_scale = 0.0f, q_scale = p.scale;
+            bool far = false;                            // a row of the warp has a maximum beyond kFar
             bool odd = false;                            // the tail's values have an infinity or NaN
             if (active) {
                 // the row of queries: [half][row][128 bytes], dims in the order of the codes' bytes
@@ -478,7 +480,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 // The maximum is looked for in the first step, and where the probabilities relative to the last one have become too
                 // large for FP16: then once more, relative to the new one.
                 float step_sum = 0.0f;
-                bool anew = step == w.begin;
+                bool anew = step == w.begin || far;
 #pragma unroll 1
                 for (int attempt = 0; attempt < 2; ++attempt) {
                     if (anew) {
@@ -509,8 +511,21 @@ kv_prefill_kernel(const PrefillParams p) {
                             }
                         }
                         anew = false;
+                        far = __any_sync(0xffffffffu, top > kNone && fabsf(top) > kFar);
                     }
-                    const float from = top > kNone ? top : 0.0f;      // (a row that has seen nothing yet: all it meets is masked)
+                    float from = top > kNone ? top : 0.0f;      // (a row that has seen nothing yet: all it meets is masked)
+                    if (far) {
+                        // Product and difference in one rounding would leave the product's own, which for 10^12 is some 10^4: equal
+                        // scores would be beyond or below their maximum.  (The maximum is that of this step, so that there is no
+                        // second attempt.)
+#pragma unroll
+                        for (int i = 0; i < kStepTokens; ++i) {
+                            score[i] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(score[i]), by[i / kKvBlock]), -from));
+                        }
+#pragma unroll
+                        for (int block = 0; block < kStepBlocks; ++block) by[block] = 1.0f;
+                        from = 0.0f;
+                    }
                     step_sum = 0.0f;
                     float largest_sum = 0.0f;
 #pragma unroll

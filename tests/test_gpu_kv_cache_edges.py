@@ -63,3 +63,35 @@ def test_a_key_far_out_does_not_cost_others_their_bits(tokens, q_heads):
     cache = QuantizedKVCache(1, 1, 64, 64, dtype=torch.bfloat16)
     cache.append(k, v, _words([0]))
     _check_attention(cache, k, v, q, [length], None)
+
+
+def _equal_scores(dtype, tokens, q_heads, head_dim, length, q_size, k_size, seed):
+    """A cache all of whose keys are the same, exactly so as codes and as they came, and queries of one number."""
+    k = torch.full((1, length, 1, head_dim), 127.0 * 2.0 ** k_size, dtype=dtype, device="cuda")
+    v = _draw((1, length, 1, head_dim), dtype, seed)
+    cache = QuantizedKVCache(1, 1, length + 3, head_dim, dtype=dtype)
+    cache.append(k, v, _words([0]))
+    return cache, k, v, torch.full((1, tokens, q_heads, head_dim), q_size, dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("length", [20, 64, 90, 700])
+@pytest.mark.parametrize(("tokens", "q_heads", "head_dim"), [(1, 4, 128), (1, 8, 64), (5, 8, 64), (20, 16, 128), (20, 16, 64)])
+def test_equal_scores_of_any_size_count_alike(tokens, q_heads, head_dim, length, sign, dtype):
+    """Scores of 3 * 10^10 and more: what a row of them gives is the mean."""
+    cache, k, v, q = _equal_scores(dtype, tokens, q_heads, head_dim, length, sign * 2.0 ** 14, 8, 11)
+    _check_attention(cache, k, v, q, [length], None, 1.0)
+    _check_attention(cache, k, v, q, [length], None, 0.7)
+    cache.check()
+
+
+@pytest.mark.parametrize(("tokens", "q_heads"), [(1, 8), (4, 8), (40, 8)])
+@pytest.mark.parametrize("length", [50, 333])
+def test_a_score_far_out(tokens, q_heads, length):
+    """One key 10^12 times the others: it is all that a query sees, or nothing of it."""
+    k, v = _draw((1, length, 1, 64), torch.bfloat16, 12), _draw((1, length, 1, 64), torch.bfloat16, 13)
+    k[:, length - 3] *= 1e12
+    cache = QuantizedKVCache(1, 1, length, 64, dtype=torch.bfloat16)
+    cache.append(k, v, _words([0]))
+    _check_attention(cache, k, v, _draw((1, tokens, q_heads, 64), torch.bfloat16, 14), [length], None)
