@@ -45,7 +45,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMinRun = 4;                      // blocks that are worth a CTA: one a warp (500 tokens 6.9 us; with eight 8.0)
 constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
-constexpr float kNone = -1.0e30f;               // the maximum of nothing
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;            // probabilities are held in FP16 times this: 2^10,
 constexpr float kMaxLag = 3.0f;                 // times 2^3 where the maximum has not been followed yet,

@@ -28,6 +28,7 @@ namespace w4a16 {
 constexpr int kKvBlock = 32;           // tokens that share a scale
 constexpr unsigned kKvBadLength = 1;   // status: a length or count outside the cache
 constexpr unsigned kKvGaveUp = 2;      // status: a bounded wait ran out
+constexpr float kNone = -3.4028235e38f;      // the maximum of nothing: no score is below it but minus infinity
 
 // Offset of a number among a full block's codes.
 template <int D>

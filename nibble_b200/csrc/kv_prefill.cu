@@ -59,7 +59,6 @@ constexpr int kPrefillThreads = (kMmaWarp + 4) * 32;      // (registers are hand
 // scores, is short of.
 constexpr int kSoftmaxRegisters = 208, kDequantRegisters = 64, kIssuerRegisters = 32;
 static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 * 128);
-constexpr float kNone = -1.0e30f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kHeadroom = 1024.0f;
 constexpr float kFar = 0x1p16f;                 // a score that is so large is rounded before the maximum is taken off

@@ -95,3 +95,13 @@ def test_a_score_far_out(tokens, q_heads, length):
     cache = QuantizedKVCache(1, 1, length, 64, dtype=torch.bfloat16)
     cache.append(k, v, _words([0]))
     _check_attention(cache, k, v, _draw((1, tokens, q_heads, 64), torch.bfloat16, 14), [length], None)
+
+
+@pytest.mark.parametrize("length", [20, 64, 90, 700])
+@pytest.mark.parametrize(("tokens", "q_heads", "head_dim"), [(1, 4, 128), (1, 8, 64), (5, 8, 64), (20, 16, 128), (20, 16, 64)])
+def test_scores_near_the_ends_of_fp32(tokens, q_heads, head_dim, length):
+    """Scores of some -10^37, all equal: the mean, not a row that sees nothing."""
+    for sign in (-1.0, 1.0):
+        cache, k, v, q = _equal_scores(torch.bfloat16, tokens, q_heads, head_dim, length, sign * 2.0 ** 60, 49, 15)
+        _check_attention(cache, k, v, q, [length], None, 1.0)
+        cache.check()
