@@ -7,8 +7,8 @@
 // for each key/value head fills a tile.  (With the queries as the sixteen rows half of
 // every tile was empty.)  Codes enter the products as exact FP16 integers, made of bytes by XOR-ing them into 1024 + 128 (one LOP3 for two,
 // then 1152 is subtracted); the key's scale multiplies the FP32 score, the value's goes into the probability before that is rounded to
-// FP16, both relative to the block at which the accumulator was last rescaled.  FP16 has its eleven bits for probabilities down to
-// 2^-24 of the largest (they are held times 2^10).  Where the results are BF16 that is all; where they are FP16 what the rounding left
+// FP16.  What is rounded, a probability times the scale of its values, is held relative to the largest of those that the row has seen,
+// times 2^10, whatever the largest probability: FP16 has its eleven bits down to 2^-24 of that.  Where the results are BF16 that is all; where they are FP16 what the rounding left
 // takes part in a second product, so that results are off by their own rounding alone (without it by 1.4 to 1.5 times that, root mean
 // square, and one token over 65501 takes 29.7 us instead of 29.9, 8 sequences of 8000 with 32 rows 60 instead of 69).  Scores, maxima,
 // sums and outputs are FP32.
@@ -46,9 +46,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kMinRun = 4;                      // blocks that are worth a CTA: one a warp (500 tokens 6.9 us; with eight 8.0)
 constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHeadroom = 1024.0f;            // probabilities are held in FP16 times this: 2^10,
+constexpr float kHeadroom = 10.0f;              // weights are held in FP16 times 2^10,
 constexpr float kMaxLag = 3.0f;                 // times 2^3 where the maximum has not been followed yet,
-constexpr float kMaxRatio = 4.0f;               // times 4 where the values' scale has not: below 65504 in all
+constexpr float kMaxRise = 2.0f;                // times 2^2 where the values' scale has not: below 65504 in all
+constexpr float kLightest = -100.0f;            // values' scales below 2^-100 count as that where weights are compared
 
 struct AttentionParams {
     KvCache cache;
@@ -451,22 +452,24 @@ kv_attention_kernel(const AttentionParams p) {
         const int lowest = row_places[member * NT * 8];        // (positions go up with the rows)
 
         float acc[NT][kSteps][4];                  // dims 16 j + g and + 8, rows 2c and 2c + 1
-        float top[NT][2], sum[NT][2];              // the sum is of this lane's tokens
+        // The largest score so far, the sum of the probabilities relative to it (of this lane's tokens), and the logarithm of what a
+        // probability times its values' scale is multiplied with for the product: what brings the largest of those that the row has
+        // seen to 2^10, wherever the largest probability is.
+        float top[NT][2], sum[NT][2], level[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.0f;
             top[n][0] = top[n][1] = kNone;
-            sum[n][0] = sum[n][1] = 0.0f;
+            sum[n][0] = sum[n][1] = level[n][0] = level[n][1] = 0.0f;
         }
-        float unit_scale = 0x1p-100f;               // of the accumulators: values are acc * unit_scale / kHeadroom
-        float per_scale = kHeadroom / 0x1p-100f;    // kHeadroom / unit_scale
 
         // Scores of a block, [group of 16 tokens][token 2g: rows 2c, 2c + 1; token 2g + 1: the same], and the probabilities that come
         // of them, as operands of the second product: row g, tokens 4c, 4c + 2 and 4c + 1, 4c + 3 of each group.
         uint32_t prob[NT][2][2], rest[NT][2][2];       // (of FP16 caches)
         auto probabilities = [&](float (&score)[NT][2][4], int block, float k_scale, float v_scale) {
             const int token = block * kKvBlock + 2 * g;
+            const float v_log = __log2f(v_scale);   // (minus infinity for a block of zeros, or NaN)
             bool lag = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -480,6 +483,7 @@ kv_attention_kernel(const AttentionParams p) {
                         x *= by;
                         lag = lag || x > limit;
                     }
+                    lag = lag || level[n][r] + v_log > kHeadroom + kMaxRise;
                 }
             }
             if ((block + 1) * kKvBlock - 1 > lowest) {
@@ -492,28 +496,24 @@ kv_attention_kernel(const AttentionParams p) {
                     }
                 }
             }
-            const bool new_unit = v_scale > kMaxRatio * unit_scale;
-            if (__any_sync(0xffffffffu, lag || new_unit)) {
-                float unit_change = 1.0f;
-                if (new_unit) {                     // (a power of two, which has no part in how probabilities are rounded)
-                    const float now = next_power(v_scale);
-                    unit_change = unit_scale / now;
-                    unit_scale = now;
-                    per_scale = kHeadroom / now;
-                }
+            if (__any_sync(0xffffffffu, lag)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float shrink[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        float more = fmaxf(fmaxf(score[n][0][r], score[n][0][2 + r]), fmaxf(score[n][1][r], score[n][1][2 + r]));
+                        float here = fmaxf(fmaxf(score[n][0][r], score[n][0][2 + r]), fmaxf(score[n][1][r], score[n][1][2 + r]));
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) more = fmaxf(more, __shfl_xor_sync(0xffffffffu, more, o));
-                        more = fmaxf(more, top[n][r]);                    // (kNone while nothing has been seen)
-                        shrink[r] = top[n][r] == kNone ? 1.0f : exp2_fast(top[n][r] - more);
-                        top[n][r] = more;
-                        sum[n][r] *= shrink[r];
-                        shrink[r] *= unit_change;
+                        for (int o = 4; o < 32; o <<= 1) here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, o));
+                        const bool fresh = top[n][r] == kNone;
+                        const float now = fmaxf(here, top[n][r]);         // (kNone while nothing has been seen)
+                        // the largest weight, relative to the largest score: the one so far, and this block's
+                        const float held = fresh ? -INFINITY : kHeadroom - level[n][r] + (top[n][r] - now);
+                        const float largest = fmaxf(held, here - now + fmaxf(v_log, kLightest));
+                        shrink[r] = fresh ? 1.0f : exp2_fast(held - largest);
+                        sum[n][r] *= fresh ? 1.0f : exp2_fast(top[n][r] - now);
+                        level[n][r] = now == kNone ? 0.0f : kHeadroom - largest;
+                        top[n][r] = now;
                     }
 #pragma unroll
                     for (int j = 0; j < kSteps; ++j) {
@@ -524,9 +524,8 @@ kv_attention_kernel(const AttentionParams p) {
                     }
                 }
             }
-            float weight = v_scale * per_scale;
-            if (weight != weight) {                 // the block's values are NaN, for the rows that see any of them
-                weight = 0.0f;
+            const bool spoilt = v_scale != v_scale;  // the block's values are NaN, for the rows that see any of them
+            if (spoilt) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (block * kKvBlock <= place[n][0]) sum[n][0] = __int_as_float(0x7fc00000);
@@ -536,7 +535,12 @@ kv_attention_kernel(const AttentionParams p) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 // relative to the maximum so far, or to zero while the row has seen nothing
-                const float from[2] = {top[n][0] == kNone ? 0.0f : top[n][0], top[n][1] == kNone ? 0.0f : top[n][1]};
+                float from[2], weight[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    from[r] = top[n][r] == kNone ? 0.0f : top[n][r];
+                    weight[r] = spoilt ? 0.0f : exp2_fast(fminf(level[n][r] + v_log, 126.0f));
+                }
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     float w[2];
@@ -544,7 +548,7 @@ kv_attention_kernel(const AttentionParams p) {
                     for (int r = 0; r < 2; ++r) {
                         const float e = exp2_fast(score[n][t >> 1][(t & 1) * 2 + r] - from[r]);
                         sum[n][r] += e;
-                        w[r] = e * weight;
+                        w[r] = e * weight[r];
                     }
                     const uint32_t rounded = pack_half(w[0], w[1]);
                     prob[n][t >> 1][t & 1] = transpose8x8(rounded);
@@ -612,7 +616,6 @@ kv_attention_kernel(const AttentionParams p) {
         if (!healthy) break;
 
         // rows of this segment: a row's sums, then the teams' results
-        const float to_value = unit_scale / kHeadroom;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -626,6 +629,7 @@ kv_attention_kernel(const AttentionParams p) {
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
+                const float to_value = exp2_fast(-level[n][r]);
                 float* to = merge + (team * kTileRows + member * 8 * NT + n * 8 + 2 * c + r) * (D + 2);
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j) {

@@ -2,8 +2,8 @@
 //
 // The same definition as kv_attention.cu, and the same arithmetic: codes are exact integers in both products (of FP16; scores of BF16
 // caches are products of BF16, so that queries and keys of any size keep their bits), the keys' scales multiply FP32 scores, the
-// values' scales enter the probabilities before those are rounded to FP16 (relative to the largest scale of the piece of work, times
-// 2^10; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
+// values' scales enter the probabilities before those are rounded to FP16 (relative to the largest such weight that the row has seen,
+// times 2^10; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
 //
 // A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
 // against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's sixteen warps, one CTA per SM:
@@ -60,9 +60,11 @@ constexpr int kPrefillThreads = (kMmaWarp + 4) * 32;      // (registers are hand
 constexpr int kSoftmaxRegisters = 208, kDequantRegisters = 64, kIssuerRegisters = 32;
 static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 * 128);
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHeadroom = 1024.0f;
+constexpr float kHeadroom = 10.0f;              // weights are held in FP16 times 2^10
+constexpr float kLightest = -100.0f;            // BF16 values' scales below 2^-100 count as that where weights are compared,
+constexpr float kLightestHalf = -40.0f;         // FP16 ones, all of which are above it but zero, as this
 constexpr float kFar = 0x1p16f;                 // a score that is so large is rounded before the maximum is taken off
-constexpr float kLargestSum = 65000.0f;         // of a block's probabilities times their values' scale: none is beyond FP16 then
+constexpr float kLargestSum = 65000.0f;         // of a block's weights: none is beyond FP16 then
 
 struct PrefillParams {
     KvCache cache;
@@ -77,7 +79,7 @@ struct PrefillParams {
     const long long* counts;
     float scale;                                 // |softmax scale| * log2 e
     bool negate;                                 // the softmax scale is negative: the queries are taken with the other sign
-    float* parts;                                // [piece][256][D + 4]: sums, maximum, sum of weights
+    float* parts;                                // [piece][256][D + 4]: sums, what they are relative to (as two logarithms), sum of probabilities
     int units, whole, pieces;                    // units in all; those of full rounds; pieces of each of the others
 };
 
@@ -171,6 +173,11 @@ __device__ __forceinline__ float2 both_of(uint64_t pair) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -285,7 +292,7 @@ __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (
 
 // Largest finite magnitude of `count` numbers (an even number of them), by a warp; and whether one of them is an infinity or NaN.
 template <typename T>
-__device__ __forceinline__ float finite_top(const T* numbers, int count, int lane, bool* odd = nullptr) {
+__device__ __forceinline__ float finite_top(const T* numbers, int count, int lane, bool& odd) {
     float top = 0.0f;
     bool strange = false;
     for (int i = lane; i < count / 2; i += 32) {
@@ -296,7 +303,7 @@ __device__ __forceinline__ float finite_top(const T* numbers, int count, int lan
         if (b <= 3.4028235e38f) top = fmaxf(top, b);
         else strange = true;
     }
-    if (odd != nullptr) *odd = __any_sync(0xffffffffu, strange);
+    odd = __any_sync(0xffffffffu, strange);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     return top;
@@ -315,8 +322,8 @@ kv_prefill_kernel(const PrefillParams p) {
     __shared__ unsigned tmem_word;
     // Of a step's blocks, keys' and values', four steps: operands are made two steps ahead of the scores, and those of step n + 2 are
     // formed only when both tiles' probabilities of step n + 1 are there.
-    __shared__ __align__(16) float scales[4][2][kStepBlocks];
-    __shared__ float tops[2][4];
+    // (Keys' scales; logarithms of the values' scales; and, for FP16, the inverses of what those are the logarithms of.)
+    __shared__ __align__(16) float scales[4][3][kStepBlocks];
     __shared__ __align__(16) float4 tail_factors[kDequantWarps];      // keys': what makes FP16 of them, the scale of that; values': the same
     // Whether the values of a step's block that is being filled have an infinity or NaN: by steps like the scales, written and read at the
     // same places.  (By works it would be overwritten: works without a step are passed over at once, and one tile may be at the end
@@ -381,7 +388,11 @@ kv_prefill_kernel(const PrefillParams p) {
             const bool active = w.stop > w.begin && w.rows > w.first_row + t * kRows;      // this tile has rows, and they see something
             const bool has_tail = active && w.held > 0 && w.stop * kStepBlocks > w.full;
             const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (w.full & 1)) * kKvBlock * D;
-            float top = kNone, sum = 0.0f, unit_scale = 0.0f, q_scale = p.scale;
+            // What this row's weights, exp2(score) times the scale of the values, are relative to: the largest that it has seen (or a
+            // little less).  FP16: `top` is that one's score and `level` the logarithm of its scale, and the sum is relative to it
+            // too.  BF16, whose scales lie so far apart that weights which count for nothing can be those of the largest
+            // probabilities: `top` is the largest score, which the sum is relative to, and `level` the weight relative to it.
+            float top = kNone, level = 0.0f, sum = 0.0f, q_scale = p.scale;
             bool far = false;                            // a row of the warp has a maximum beyond kFar
             bool odd = false;                            // the tail's values have an infinity or NaN
             if (active) {
@@ -401,10 +412,6 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) raw[i + e] = h[2 * e] | static_cast<uint32_t>(h[2 * e + 1]) << 16;
                     }
-                }
-                const float* v_scales = p.cache.v_scales + pair * p.cache.blocks;
-                for (int block = w.begin * kStepBlocks + row_in_tile; block < min(w.stop * kStepBlocks, w.full); block += kRows) {
-                    unit_scale = fmaxf(unit_scale, v_scales[block]);
                 }
                 if constexpr (kBf16) {
                     // by a power of two of the row's own, so that no product is beyond FP32 that the definition has within
@@ -428,21 +435,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.q_full[t]);
-                // What the accumulator's numbers are relative to: the largest scale of the values that this work meets.  Rounded up to a
-                // power of two, so that what a row does not see has no part in how its probabilities are rounded.
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) unit_scale = fmaxf(unit_scale, __shfl_xor_sync(0xffffffffu, unit_scale, o));
-                if (has_tail) {
-                    float scale;
-                    power_for(finite_top(v_tail, w.held * D, lane), scale);
-                    unit_scale = fmaxf(unit_scale, scale);
-                }
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");      // (the last work's have been read)
-                if (lane == 0) tops[t][warp % 4] = unit_scale;
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-                unit_scale = next_power(fmaxf(fmaxf(fmaxf(tops[t][0], tops[t][1]), fmaxf(tops[t][2], tops[t][3])), 1.0e-30f));
             }
-            const float per_scale = kHeadroom / unit_scale;
             const int lowest = __reduce_min_sync(0xffffffffu, row < w.rows ? place : INT_MAX);
             for (int step = w.begin; active && step < w.stop; ++step, ++steps_done) {
                 wait(bars.s_full[t], steps_done);
@@ -451,22 +444,25 @@ kv_prefill_kernel(const PrefillParams p) {
                 tmem_load128(score_at, score);
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 arrive(bars.s_taken[t]);                 // the other tile's scores may come in their place
-                // Of each block: a score's factor, not negative, and the logarithm of a probability's factor, which goes into the exponent
-                // (and out of the sum again).  Either may be NaN; a row that sees nothing of the block is kept out of that.
+                // Of each block: a score's factor, not negative, and the logarithm of its values' scale, which goes into the exponent (and out
+                // of the sum again; BF16: beside it).  Either may be NaN; a row that sees nothing of the block is kept out of that.
                 const float4 k_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][0]);
-                const float4 v_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][1]);
+                const float4 v_log = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][1]);
+                const float4 v_inverse = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][2]);
                 if (has_tail && step + 1 == w.stop) odd = odd_tail[(steps_of_all + step - w.begin) & 3][w.full % kStepBlocks];
                 float by[kStepBlocks] = {k_scale.x, k_scale.y, k_scale.z, k_scale.w};
-                float weight[kStepBlocks] = {v_scale.x, v_scale.y, v_scale.z, v_scale.w};
+                float value[kStepBlocks] = {v_log.x, v_log.y, v_log.z, v_log.w};
+                float inverse[kStepBlocks] = {v_inverse.x, v_inverse.y, v_inverse.z, v_inverse.w};
                 const bool masked = (step + 1) * kStepTokens - 1 > lowest;
                 const int last = place - step * kStepTokens;             // tokens of the step up to it are seen
 #pragma unroll
                 for (int block = 0; block < kStepBlocks; ++block) {
                     by[block] *= q_scale;
-                    weight[block] *= per_scale;
                     if (by[block] == 0.0f) by[block] = 0x1p-100f;
-                    if (weight[block] < 0x1p-80f) weight[block] = 0x1p-80f;
-                    if (masked && block * kKvBlock > last) by[block] = weight[block] = 1.0f;
+                    if (masked && block * kKvBlock > last) {
+                        by[block] = inverse[block] = 1.0f;
+                        value[block] = 0.0f;
+                    }
                 }
                 if (masked) {
 #pragma unroll
@@ -476,28 +472,53 @@ kv_prefill_kernel(const PrefillParams p) {
                 }
                 if (steps_done > 0) wait(bars.o_done[t], steps_done - 1);      // the probabilities before these have been used
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                // The maximum is looked for in the first step, and where the probabilities relative to the last one have become too
-                // large for FP16: then once more, relative to the new one.
+                // The largest weight is looked for in the first step, and where the weights relative to the last one have become too large
+                // for FP16: then once more, relative to the new one.
                 float step_sum = 0.0f;
                 bool anew = step == w.begin || far;
 #pragma unroll 1
                 for (int attempt = 0; attempt < 2; ++attempt) {
                     if (anew) {
-                        float more = kNone;
+                        float largest[kStepBlocks];
 #pragma unroll
                         for (int block = 0; block < kStepBlocks; ++block) {
                             const float* x = reinterpret_cast<const float*>(score + block * 32);
-                            float largest[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
+                            float two[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
 #pragma unroll
                             for (int i = 6; i < 30; i += 4) {
-                                largest[0] = max3(largest[0], x[i], x[i + 1]);
-                                largest[1] = max3(largest[1], x[i + 2], x[i + 3]);
+                                two[0] = max3(two[0], x[i], x[i + 1]);
+                                two[1] = max3(two[1], x[i + 2], x[i + 3]);
                             }
-                            more = fmaxf(more, max3(max3(largest[0], x[30], x[31]), largest[1], largest[1]) * by[block]);
+                            largest[block] = max3(max3(two[0], x[30], x[31]), two[1], two[1]) * by[block];
                         }
-                        const float shrink = more > top && top > kNone ? exp2_fast(top - more) : 1.0f;
-                        top = fmaxf(top, more);
-                        sum *= shrink;
+                        float now = top, shrink = 1.0f;
+                        if constexpr (kBf16) {
+                            float most = kNone;
+#pragma unroll
+                            for (int block = 0; block < kStepBlocks; ++block) now = fmaxf(now, largest[block]);
+                            const float before = top > kNone ? level + (top - now) : -INFINITY;
+#pragma unroll
+                            for (int block = 0; block < kStepBlocks; ++block) most = fmaxf(most, largest[block] - now + fmaxf(value[block], kLightest));
+                            most = fmaxf(most, before);
+                            if (top > kNone) {
+                                shrink = exp2_fast(before - most);
+                                sum *= exp2_fast(top - now);
+                            }
+                            level = now > kNone ? most : 0.0f;
+                        } else {
+                            float of_now = level;
+#pragma unroll
+                            for (int block = 0; block < kStepBlocks; ++block) {
+                                if (largest[block] - now + (value[block] - of_now) > 0.0f) {
+                                    now = largest[block];
+                                    of_now = value[block];
+                                }
+                            }
+                            if (top > kNone) shrink = exp2_fast(top - now + (level - of_now));
+                            sum *= shrink;
+                            level = of_now;
+                        }
+                        top = now;
                         if (step > w.begin) {
 #pragma unroll 1
                             for (int d = 0; d < D; d += 32) {
@@ -530,28 +551,36 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll
                     for (int block = 0; block < kStepBlocks; ++block) {
                         uint32_t packed[16];
-                        const float with = __log2f(weight[block]) - from;
-                        // Where results are FP16 the sum is of the probabilities as they were rounded, so that what a row's large ones were
+                        const float rise = value[block] - level + kHeadroom;
+                        const float with = kBf16 ? -from : rise - from;
+                        const float factor = kBf16 ? exp2_fast(rise > 126.0f ? 126.0f : rise) : inverse[block];      // (NaN stays)
+                        // Where results are FP16 the sum is of the weights as they were rounded, so that what a row's large ones were
                         // off by goes out of its result: root mean square 1.4 times the result's own rounding at most, where it was up to
-                        // 1.6 (and 474 us, now 486).  Not of a block whose values are so small that its probabilities run out of bits.
-                        const bool as_rounded = !kBf16 && weight[block] >= 1.0f;
-                        const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with);
+                        // 1.6 (and 474 us, now 486).  Not of a block whose values are so small that its weights run out of bits.
+                        const bool as_rounded = !kBf16 && rise >= kHeadroom - 4.0f;
+                        const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with), factor2 = pair_of(factor, factor);
                         uint64_t sums[2] = {0, 0};
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
                             const float2 x = both_of(fma2(pair_of(score[block * 32 + i], score[block * 32 + i + 1]), by2, with2));
                             float a = exp2_fast(x.x), b = exp2_fast(x.y);
-                            packed[i / 2] = pack_half(a, b);
-                            if (as_rounded) {
-                                const float2 held = widen2<__half>(packed[i / 2]);
-                                a = held.x;
-                                b = held.y;
+                            if constexpr (kBf16) {
+                                const float2 weights = both_of(mul2(pair_of(a, b), factor2));
+                                packed[i / 2] = pack_half(weights.x, weights.y);
+                            } else {
+                                packed[i / 2] = pack_half(a, b);
+                                if (as_rounded) {
+                                    const float2 held = widen2<__half>(packed[i / 2]);
+                                    a = held.x;
+                                    b = held.y;
+                                }
                             }
                             sums[i / 2 % 2] = add2(sums[i / 2 % 2], pair_of(a, b));
                         }
                         const float2 all = both_of(add2(sums[0], sums[1]));
-                        largest_sum = fmaxf(largest_sum, all.x + all.y);
-                        step_sum = fmaf(all.x + all.y, __fdividef(1.0f, weight[block]), step_sum);
+                        const float block_sum = all.x + all.y;
+                        largest_sum = fmaxf(largest_sum, kBf16 ? fmaxf(block_sum, block_sum * factor) : block_sum);
+                        step_sum = kBf16 ? step_sum + block_sum : fmaf(block_sum, factor, step_sum);
                         tmem_store16(prob_at + block * 16, packed);
                     }
                     anew = __any_sync(0xffffffffu, largest_sum > kLargestSum);
@@ -567,7 +596,7 @@ kv_prefill_kernel(const PrefillParams p) {
             float* part = p.parts + (static_cast<size_t>(blockIdx.x) * kUnitRows + t * kRows + row_in_tile) * (D + 4);
             const bool write = to_part ? active : row < p.tokens * p.group;
             T* out = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(w.b) * p.tokens + token) * p.q_heads + q_head) * D;
-            const float by = to_part ? unit_scale / kHeadroom : sum > 0.0f ? unit_scale / kHeadroom / sum : sum;
+            const float unit = kBf16 ? exp2_fast(level - kHeadroom) : 1.0f, by = to_part ? unit : sum > 0.0f ? unit / sum : sum;
             if (active) {
                 wait(bars.o_done[t], steps_done - 1);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -600,7 +629,7 @@ kv_prefill_kernel(const PrefillParams p) {
                     }
                 }
             }
-            if (write && to_part) *reinterpret_cast<float2*>(part + D) = make_float2(top, sum);
+            if (write && to_part) *reinterpret_cast<float4*>(part + D) = make_float4(top, kBf16 ? 0.0f : level, sum, 0.0f);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // (the next work's first arrival lets O be overwritten)
         }
     } else if (warp < kMmaWarp) {
@@ -638,12 +667,22 @@ kv_prefill_kernel(const PrefillParams p) {
             }
             if (w.held > 0 && w.full % kStepBlocks == mine && w.full / kStepBlocks >= w.begin && w.full / kStepBlocks < w.stop) {
                 // What the numbers of the block that is being filled are multiplied with, and the scale that stands for it.  FP16 keys
-                // stay as they are, BF16 ones stay BF16; values, which become FP16, are brought to the size of codes, so that
-                // probabilities keep as many bits beside small ones.
+                // stay as they are, BF16 ones stay BF16.  FP16 values, where they are smaller, are brought to the size of codes, so that
+                // weights keep as many bits beside small ones; all stay exact.  BF16 values become FP16 just below its largest: they
+                // keep their bits down to 2^-32 of the block's largest, and below 2^-40 of it count as zero.  (As codes they count as zero
+                // below 2^-8 of it.)
                 const size_t tail = (static_cast<size_t>(pair) * 2 + (w.full & 1)) * kKvBlock * D;
                 float4 factors = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane), factors.y);
-                factors.z = power_for(finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane, &odd_values), factors.w);
+                if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane, odd_values), factors.y);
+                const float largest = finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane, odd_values);
+                factors.z = power_for(largest, factors.w);
+                if (kBf16) {
+                    factors.z *= 64.0f;
+                    factors.w *= 1.0f / 64.0f;
+                } else if (factors.z < 1.0f) {
+                    factors.z = factors.w = 1.0f;
+                }
+                if (largest == 0.0f) factors.w = 0.0f;       // (it counts for no more than a full block of zeros)
                 if (lane == 0) tail_factors[mine] = factors;
                 __syncwarp();
             }
@@ -724,7 +763,9 @@ kv_prefill_kernel(const PrefillParams p) {
                 }
                 if (lane == 0) {
                     scales[steps & 3][0][mine] = k_scale;
-                    scales[steps & 3][1][mine] = v_scale;
+                    const float v_log = !kBf16 && v_scale < 0x1p-40f ? kLightestHalf : __log2f(v_scale);
+                    scales[steps & 3][1][mine] = v_log;
+                    if (!kBf16) scales[steps & 3][2][mine] = exp2_fast(-v_log);
                     if (tail) odd_tail[steps & 3][mine] = odd_values;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -879,36 +920,43 @@ kv_pieces_kernel(const PrefillParams p) {
     const int row = first.first_row + in_unit;
     if (row >= p.tokens * p.group) return;
     constexpr int kDims = D / 32;
-    float top = kNone, weight = 0.0f, acc[kDims];
+    float top = kNone, level = 0.0f, weight = 0.0f, acc[kDims];
 #pragma unroll
     for (int d = 0; d < kDims; ++d) acc[d] = 0.0f;
     if (row < first.rows) {
         for (int begin = 0; begin < p.pieces; begin += BATCH) {
-            float2 state[BATCH], numbers[BATCH][kDims / 2];
-            float best = top;
+            float4 state[BATCH];                          // what its numbers are relative to, and its sum
+            float2 numbers[BATCH][kDims / 2];
+            float best = top, of_best = level;
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
                 const int piece = begin + e;
                 const bool some = piece < p.pieces && static_cast<long long>(first.stop) * piece / p.pieces <
                                                           static_cast<long long>(first.stop) * (piece + 1) / p.pieces;
                 const float* part = p.parts + (static_cast<size_t>(unit * p.pieces + piece) * kUnitRows + in_unit) * (D + 4);
-                state[e] = some ? *reinterpret_cast<const float2*>(part + D) : make_float2(kNone, 0.0f);
+                state[e] = some ? *reinterpret_cast<const float4*>(part + D) : make_float4(kNone, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int d = 0; d < kDims / 2; ++d) {
                     numbers[e][d] = some ? reinterpret_cast<const float2*>(part + lane * kDims)[d] : make_float2(0.0f, 0.0f);
                 }
             }
 #pragma unroll
-            for (int e = 0; e < BATCH; ++e) best = fmaxf(best, state[e].x);
-            const float mine = exp2_fast(top - best);
+            for (int e = 0; e < BATCH; ++e) {
+                if (state[e].x - best + (state[e].y - of_best) > 0.0f) {
+                    best = state[e].x;
+                    of_best = state[e].y;
+                }
+            }
+            const float mine = exp2_fast(top - best + (level - of_best));
             top = best;
+            level = of_best;
             weight *= mine;
 #pragma unroll
             for (int d = 0; d < kDims; ++d) acc[d] *= mine;
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
-                const float theirs = exp2_fast(state[e].x - best);
-                weight = fmaf(state[e].y, theirs, weight);
+                const float theirs = exp2_fast(state[e].x - best + (state[e].y - of_best));
+                weight = fmaf(state[e].z, theirs, weight);
 #pragma unroll
                 for (int d = 0; d < kDims / 2; ++d) {
                     acc[2 * d] = fmaf(numbers[e][d].x, theirs, acc[2 * d]);

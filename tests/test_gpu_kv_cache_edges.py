@@ -105,3 +105,79 @@ def test_scores_near_the_ends_of_fp32(tokens, q_heads, head_dim, length):
         cache, k, v, q = _equal_scores(torch.bfloat16, tokens, q_heads, head_dim, length, sign * 2.0 ** 60, 49, 15)
         _check_attention(cache, k, v, q, [length], None, 1.0)
         cache.check()
+
+
+def _block_tops(v, length):
+    """The largest magnitude of each token's block (of its own, where the block is being filled): [length, heads]."""
+    tops = v[:length].double().abs().amax(-1)
+    full = length // 32 * 32
+    tops[:full] = tops[:full].view(-1, 32, v.shape[1]).amax(1, keepdim=True).expand(-1, 32, -1).reshape(full, -1)
+    return tops
+
+
+def _check_seen(cache, k, v, q, length, scale):
+    """Attention against its definition, within what the tokens that a query sees allow: a weight (probability times its values' scale)
+    is held in FP16 times 2^10 relative to the largest one seen, M / 127 at most with M the largest p x (largest of the token's block).
+    What is below FP16's normal numbers is off by half a step, 2^-25: times a code of 127 at most that is 2^-35 of M for each token;
+    times a number of the block being filled, held up to 2^16, 2^-25 x 2^-10 x 2^16 / 127 < 2^-25 of it, 31 of them 2^-20.  A sum of rounded
+    weights is off by 2^-31 of itself for each of them at most (their scale is 2^-4 of the largest's or more).  The rest is
+    kv_oracle.attention_bound's."""
+    got = cache.attention(q, _words([length]), softmax_scale=scale)[0].double()
+    tokens, q_heads, _ = q.shape[1:]
+    group = q_heads // v.shape[2]
+    kb, vb = oracle.held(k[0], length)[:length], oracle.held(v[0], length)[:length]
+    want, weight = oracle.attention(q[0], kb, vb, length, tokens, scale)
+    tops = _block_tops(v[0], length)
+    hidden = torch.arange(length, device="cuda")[None, :] > (length - tokens + torch.arange(tokens, device="cuda"))[:, None]
+    for head in range(v.shape[2]):
+        rows = slice(head * group, (head + 1) * group)
+        scores = torch.einsum("ihd,td->iht", q[0, :, rows].double(), kb[:, head]) * scale
+        p = torch.softmax(scores.masked_fill(hidden[:, None, :], float("-inf")), -1)
+        most = (p * tops[:, head]).amax(-1, keepdim=True)
+        bound = oracle.attention_bound(want[:, rows], weight[:, rows], q.dtype, 0.0)
+        bound = bound + most * (length * 2.0 ** -35 + 2.0 ** -20) + want[:, rows].abs() * length * 2.0 ** -31
+        off = (got[:, rows] - want[:, rows]).abs()
+        assert (off <= bound).all(), (head, float((off / bound).max()))
+    cache.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads"), [(1, 8, 2), (5, 8, 2), (3, 32, 2), (90, 8, 2), (300, 64, 1)])
+@pytest.mark.parametrize("where", ["unseen", "unseen in a full block", "unlikely", "unlikely and near"])
+def test_values_far_out_do_not_cost_others_their_bits(where, tokens, q_heads, kv_heads, dtype):
+    """Half of a row's result comes of thousands of small probabilities of small values, beside a value that is millions of times as large:
+    behind the queries, or of a token that counts for nothing."""
+    length = 8032 if where == "unseen in a full block" else 8017
+    large = 60000.0 if dtype == torch.float16 else 1e6
+    k = torch.zeros((1, length, kv_heads, 64), dtype=dtype, device="cuda")
+    heavy = length - 5 if where == "unlikely and near" and tokens == 1 else 5
+    k[:, heavy] = 1.0
+    v = (0.01 * (1.0 + 0.2 * _draw((1, length, kv_heads, 64), torch.float32, 16).clamp(-2, 2))).to(dtype)
+    if where.startswith("unseen"):
+        v[:, length - 1, :, ::2] = large
+    else:
+        at = length - 9 if where == "unlikely and near" else 40
+        k[:, at] = -60.0 / 9
+        v[:, at, :, ::2] = large
+    cache = QuantizedKVCache(1, kv_heads, length + 7, 64, dtype=dtype)
+    cache.append(k, v, _words([0]))
+    q = torch.full((1, tokens, q_heads, 64), 9.0 / 64, dtype=dtype, device="cuda")        # scores of nine, of zero, of -60
+    _check_seen(cache, k, v, q, length, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "q_heads", "head_dim"), [(1, 8, 64), (6, 8, 128), (40, 8, 64), (400, 8, 128)])
+def test_blocks_of_values_of_every_size(tokens, q_heads, head_dim, dtype):
+    """Sizes that go up and down by thousands from block to block, some zero, with scores that do the same: the reference of the weights
+    moves in either way, and pieces of a row meet with different ones."""
+    length = 1500
+    g = torch.Generator().manual_seed(17)
+    low, high = (-16, 13) if dtype == torch.float16 else (-60, 90)
+    sizes = 2.0 ** torch.randint(low, high, (47,), generator=g).double() * (torch.rand((47,), generator=g) > 0.1)
+    sizes = sizes.cuda().repeat_interleave(32)[:length, None, None]
+    k = _draw((1, length, 1, head_dim), dtype, 18)
+    v = (_draw((1, length, 1, head_dim), torch.float32, 19).double() * sizes)[...].to(dtype)
+    cache = QuantizedKVCache(1, 1, length + 9, head_dim, dtype=dtype)
+    cache.append(k, v, _words([0]))
+    for spread in (0.3, 2.0, 6.0):
+        _check_seen(cache, k, v, _draw((1, tokens, q_heads, head_dim), dtype, 20, spread), length, head_dim ** -0.5)
