@@ -629,12 +629,12 @@ kv_attention_kernel(const AttentionParams p) {
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float to_value = exp2_fast(-level[n][r]);
+                const float to_value = exp2_fast(-level[n][r]), shrink = kBf16 ? kShrink : 1.0f;
                 float* to = merge + (team * kTileRows + member * 8 * NT + n * 8 + 2 * c + r) * (D + 2);
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j) {
-                    to[j * 16 + g] = acc[n][j][r] * to_value;
-                    to[j * 16 + 8 + g] = acc[n][j][2 + r] * to_value;
+                    to[j * 16 + g] = acc[n][j][r] * shrink * to_value;
+                    to[j * 16 + 8 + g] = acc[n][j][2 + r] * shrink * to_value;
                 }
                 if (g == 0) *reinterpret_cast<float2*>(to + D) = make_float2(top[n][r], sum[n][r]);
             }
@@ -680,6 +680,7 @@ kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
     constexpr int kRows = kWarps / ROW_WARPS;            // at a time
     constexpr int kDims = D / 32;                        // of a lane
     constexpr int kStride = D + 8;                       // of a token's numbers in shared memory
+    constexpr float kHeld = std::is_same<T, __nv_bfloat16>::value ? kShrink : 1.0f;      // what sums of values are held times
     __shared__ __align__(16) T keys[kKvBlock * kStride];
     __shared__ __align__(16) T values[kKvBlock * D];
     __shared__ __align__(16) float queries[kRows][D];
@@ -761,7 +762,7 @@ kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
             for (int o = 16; o > 0; o >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, o);
 #pragma unroll 4
             for (int t = 0; t < seen; ++t) {
-                const float w = __shfl_sync(0xffffffffu, mine, t);
+                const float w = __shfl_sync(0xffffffffu, mine, t) * kHeld;
                 const T* v = values + t * D + lane * kDims;
 #pragma unroll
                 for (int e = 0; e < kDims; e += 2) {
@@ -849,7 +850,7 @@ kv_finish_kernel(const AttentionParams p, int rows_per_cta) {
             }
         }
         if (row < last_row && share == 0) {
-            const float by = weight > 0.0f ? 1.0f / weight : weight;       // (no weight: nothing is seen)
+            const float by = weight > 0.0f ? 1.0f / kHeld / weight : weight;       // (no weight: nothing is seen)
             T* to = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(b) * p.tokens + i) * p.q_heads + q_head) * D + lane * kDims;
 #pragma unroll
             for (int e = 0; e < kDims; e += 2) *reinterpret_cast<uint32_t*>(to + e) = narrow2<T>(acc[e] * by, acc[e + 1] * by);

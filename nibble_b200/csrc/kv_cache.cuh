@@ -28,6 +28,7 @@ namespace w4a16 {
 constexpr int kKvBlock = 32;           // tokens that share a scale
 constexpr unsigned kKvBadLength = 1;   // status: a length or count outside the cache
 constexpr unsigned kKvGaveUp = 2;      // status: a bounded wait ran out
+constexpr float kShrink = 0x1p-32f;      // BF16: sums of values over tokens are held times this, so that those of its largest are finite
 constexpr float kNone = -3.4028235e38f;      // the maximum of nothing: no score is below it but minus infinity
 
 // Offset of a number among a full block's codes.

@@ -597,6 +597,7 @@ kv_prefill_kernel(const PrefillParams p) {
             const bool write = to_part ? active : row < p.tokens * p.group;
             T* out = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(w.b) * p.tokens + token) * p.q_heads + q_head) * D;
             const float unit = kBf16 ? exp2_fast(level - kHeadroom) : 1.0f, by = to_part ? unit : sum > 0.0f ? unit / sum : sum;
+            const float shrink = kBf16 && to_part ? kShrink : 1.0f;
             if (active) {
                 wait(bars.o_done[t], steps_done - 1);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -606,7 +607,7 @@ kv_prefill_kernel(const PrefillParams p) {
                 uint32_t o[32];
                 if (active) tmem_load32(out_at + d, o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = active && row < w.rows ? __float_as_uint(__uint_as_float(o[i]) * by) : 0u;
+                for (int i = 0; i < 32; ++i) o[i] = active && row < w.rows ? __float_as_uint(__uint_as_float(o[i]) * shrink * by) : 0u;
                 if (odd) {                               // infinities and NaN of the tail, which were kept out of the products
                     for (int i = 0; i < w.held; ++i) {
                         if (w.full * kKvBlock + i > place) break;
@@ -965,7 +966,8 @@ kv_pieces_kernel(const PrefillParams p) {
             }
         }
     }
-    const float by = weight > 0.0f ? 1.0f / weight : weight;
+    constexpr float kHeld = std::is_same<T, __nv_bfloat16>::value ? kShrink : 1.0f;      // what the sums are held times
+    const float by = weight > 0.0f ? 1.0f / kHeld / weight : weight;
     const int token = by_group(p, row), q_head = first.head * p.group + row - token * p.group;
     T* to = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(first.b) * p.tokens + token) * p.q_heads + q_head) * D + lane * kDims;
 #pragma unroll

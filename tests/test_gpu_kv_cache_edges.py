@@ -181,3 +181,21 @@ def test_blocks_of_values_of_every_size(tokens, q_heads, head_dim, dtype):
     cache.append(k, v, _words([0]))
     for spread in (0.3, 2.0, 6.0):
         _check_seen(cache, k, v, _draw((1, tokens, q_heads, head_dim), dtype, 20, spread), length, head_dim ** -0.5)
+
+
+@pytest.mark.parametrize("length", [20, 90, 3000])
+@pytest.mark.parametrize(("tokens", "q_heads", "head_dim"), [(1, 8, 64), (6, 8, 128), (20, 16, 64), (300, 8, 128)])
+def test_means_of_the_largest_values(tokens, q_heads, head_dim, length):
+    """BF16 values as large as they come: their sums are beyond FP32, their means are not."""
+    top = torch.finfo(torch.bfloat16).max
+    k = _draw((1, length, 1, head_dim), torch.bfloat16, 21, 0.1)
+    sign = torch.where(torch.arange(head_dim, device="cuda") % 3 == 0, -1.0, 1.0)
+    v = (top * sign).to(torch.bfloat16).expand(1, length, 1, head_dim)
+    cache = QuantizedKVCache(1, 1, length + 3, head_dim, dtype=torch.bfloat16)
+    cache.append(k, v, _words([0]))
+    got = cache.attention(_draw((1, tokens, q_heads, head_dim), torch.bfloat16, 22), _words([length]))
+    first = max(0, tokens - length)
+    # (a sum of rounded numbers over one of others: 2^-8 of the mean for all of them, which is a step of BF16 at most)
+    assert got.isfinite().all() and not got[0, :first].any()
+    assert ((got[0, first:].double() / (top * sign) - 1.0).abs() <= 2.0 ** -7).all()
+    cache.check()
