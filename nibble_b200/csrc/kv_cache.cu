@@ -395,9 +395,9 @@ __device__ __forceinline__ float scale_of(float top) {
 }
 
 // A CTA takes blocks of one sequence and key/value head that the new tokens touch: a thread owns sixteen numbers of a key and of a
-// value.  A block that becomes full is read (older tokens from the tail), its codes and scales are written; of the newest two blocks
-// the numbers themselves go to the tail, into the slot of the block's parity.  The CTA of the first block reads a tail slot that the
-// newest blocks may write, so it writes that slot itself, after it has read.
+// value.  A block that becomes full is read (older tokens from the tail), its codes and scales are written; of the last token's block and
+// the one before it the numbers themselves go to the tail, into the slot of the block's parity.  The CTA of the first block reads a tail
+// slot that one of those two may write, so it writes that slot itself, after it has read.
 template <typename T, int D, bool ROTARY>
 __global__ void __launch_bounds__(2 * D, kAppendThreads / (2 * D))
 kv_append_kernel(const AppendParams p) {
@@ -441,8 +441,9 @@ kv_append_kernel(const AppendParams p) {
         return;
     }
     const int begin = static_cast<int>(start), end = begin + static_cast<int>(count);
-    const int first_block = begin / kKvBlock, newest = end / kKvBlock;   // `newest`: the one that the next token goes to
     if (count == 0) return;
+    const int first_block = begin / kKvBlock, newest = end / kKvBlock;   // `newest`: the one that the next token goes to
+    const int last_block = (end - 1) / kKvBlock;                         // the last token's
     // this thread's token and sixteen dims of the keys: byte tid * 16 of the block's key codes
     constexpr int kRuns = D / 64, kChunks = D / 16;
     const int line = tid / 32, lane = tid % 32;
@@ -535,8 +536,9 @@ kv_append_kernel(const AppendParams p) {
         }
     };
 
-    // A newest block of the first one's parity shares its tail slot: the first one's CTA writes it, if it read that slot.
-    const int shared = ((newest - first_block) & 1) == 0 ? newest : newest - 1;
+    // The one of the last two blocks that has the first one's parity shares its tail slot: the first one's CTA writes it, if it read
+    // that slot.
+    const int shared = ((last_block - first_block) & 1) == 0 ? last_block : last_block - 1;
     const bool first_reads = begin % kKvBlock != 0 && first_block < newest && shared > first_block;
     uint32_t k[8], v[8], next_k[8], next_v[8];
     // A block ahead (2 x 8191 tokens of 8 heads of 128 written and read back: 42 us, each block fetched in its turn 50; where keys are
@@ -598,8 +600,8 @@ kv_append_kernel(const AppendParams p) {
             __syncthreads();
             *reinterpret_cast<uint4*>(p.cache.v_codes + at * (kKvBlock * D) + tid * 16) = turned_codes[value_piece(line, lane)];
         }
-        if (block >= newest - 1 && !(first_reads && block == shared)) keep(block, k, v);
-        if (first_reads && block == first_block && shared * kKvBlock < end) {
+        if (block >= last_block - 1 && !(first_reads && block == shared)) keep(block, k, v);
+        if (first_reads && block == first_block) {
             __syncthreads();                                              // all of the old slot has been read
             fetch(shared, k, v);
             keep(shared, k, v);

@@ -199,3 +199,39 @@ def test_means_of_the_largest_values(tokens, q_heads, head_dim, length):
     assert got.isfinite().all() and not got[0, :first].any()
     assert ((got[0, first:].double() / (top * sign) - 1.0).abs() <= 2.0 ** -7).all()
     cache.check()
+
+
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize(("dtype", "head_dim"), [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("pieces", [[64], [20, 44], [20, 12, 32], [1] * 64, [96], [40, 56], [5, 91], [96 - 31, 31], [32], [31, 1], [128], [50, 78],
+                                    [33], [70], [20, 57]])
+def test_a_length_falls_to_the_block_before_the_last_tokens(pieces, dtype, head_dim, turned):
+    """Whatever the last append ended on, and however the tokens came: read, attended over, and written on from there."""
+    reached = sum(pieces)
+    k, v, other = (_draw((2, 176, 2, head_dim), dtype, seed) for seed in (23, 24, 25))
+    q = _draw((2, 1, 4, head_dim), dtype, 26)
+    inv_freq = torch.zeros((head_dim // 2,), device="cuda") if turned else None           # (by no angle at all)
+
+    def fill(cache):
+        at = 0
+        for piece in pieces:
+            cache.append(k[:, at:at + piece], v[:, at:at + piece], _words([at, at]), inv_freq=inv_freq)
+            at += piece
+        return cache
+
+    low = ((reached - 1) // 32 - 1) * 32
+    for back in sorted({max(0, low), max(0, low) + 1, max(0, low) + 20, max(0, low) + 31, max(1, low + 32), reached}):
+        if back > reached:
+            continue
+        cache = fill(QuantizedKVCache(2, 2, 176, head_dim, dtype=dtype))
+        for got, x in zip(cache.read(_words([back, back])), (k, v)):
+            assert torch.equal(got, _held(x, [back, back])), back
+        fresh = QuantizedKVCache(2, 2, 176, head_dim, dtype=dtype)
+        fresh.append(k[:, :back], v[:, :back], _words([0, 0]))
+        assert torch.equal(cache.attention(q, _words([back, back])), fresh.attention(q, _words([back, back])))
+        for piece in (7, 40):
+            cache = fill(QuantizedKVCache(2, 2, 176, head_dim, dtype=dtype))
+            cache.append(other[:, :piece], other[:, :piece], _words([back, back]), inv_freq=inv_freq)
+            mixed = torch.cat((v[:, :back], other[:, :piece], v[:, back + piece:]), 1)
+            assert torch.equal(cache.read(_words([back + piece] * 2))[1], _held(mixed, [back + piece] * 2)), (back, piece)
+        cache.check()
