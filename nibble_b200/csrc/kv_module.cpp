@@ -1,13 +1,14 @@
 // The native side of nibble_b200/kv_cache.py: checks tensors, allocates outputs and workspaces from the caching allocator, and
 // hands pointers plus the current stream of the tensors' device to the C ABI.  Every violation is a TORCH_CHECK, i.e. a
 // RuntimeError.  (Messages hold no numbers: with this image's compiler, formatting one through a stream crashes.)  Nothing here takes
-// part in autograd: a call whose input asks for a gradient is refused.
+// part in autograd: a call whose input asks for a gradient, or carries a forward-mode tangent, is refused.
 #include "kv_module.h"
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
@@ -28,6 +29,8 @@ const at::Tensor& tensor_of(PyObject* object, const char* name) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()),
                 name, " requires a gradient, which this operator does not form; detach it or use torch.no_grad()");
+    TORCH_CHECK(!(at::isFloatingType(t.scalar_type()) && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined()),
+                name, " carries a tangent of forward-mode differentiation, which this operator does not pass on");
     return t;
 }
 std::optional<at::Tensor> optional_of(PyObject* object, const char* name) {

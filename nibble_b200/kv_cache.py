@@ -10,7 +10,7 @@ each number is rounded once.  A block with an infinity or NaN in it reads back a
 
 Lengths, starts and counts are int64 tensors on the device, so that a captured CUDA graph serves every step; one that does not fit
 the cache leaves that sequence alone (its outputs are zeros) and is reported by ``check()``.  None of these operators forms
-gradients: an input that requires one is refused.  All of them run on the current stream of the tensors' device.
+gradients: an input that requires one, or carries a forward-mode tangent, is refused.  All of them run on the current stream of the tensors' device.
 """
 from __future__ import annotations
 

@@ -235,3 +235,28 @@ def test_a_length_falls_to_the_block_before_the_last_tokens(pieces, dtype, head_
             mixed = torch.cat((v[:, :back], other[:, :piece], v[:, back + piece:]), 1)
             assert torch.equal(cache.read(_words([back + piece] * 2))[1], _held(mixed, [back + piece] * 2)), (back, piece)
         cache.check()
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation and transformed tensors: no result that has lost them."""
+    cache = QuantizedKVCache(1, 2, 64, 64)
+    x, at, inv_freq = _draw((1, 3, 2, 64), torch.float16, 27), _words([0]), torch.ones((32,), device="cuda")
+    places = _words([[0, 1, 2]])
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: apply_rotary(dual, places, inv_freq), lambda: apply_rotary(x, places, inv_freq, out=dual),
+                     lambda: apply_rotary(x, places, torch.autograd.forward_ad.make_dual(inv_freq, inv_freq)),
+                     lambda: cache.append(dual, x, at), lambda: cache.append(x, dual[:, :, :], at),
+                     lambda: cache.append(x, x, at, q=dual, inv_freq=inv_freq), lambda: cache.attention(dual, at)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        with torch.autograd.forward_ad._set_fwd_grad_enabled(False):
+            assert torch.equal(apply_rotary(dual, places, inv_freq), apply_rotary(x, places, inv_freq))
+        assert torch.equal(cache.attention(torch.autograd.forward_ad.unpack_dual(dual).primal, at), torch.zeros_like(x))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: apply_rotary(t, places, inv_freq), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: apply_rotary(t, places, inv_freq))(x[None])
+    torch.cuda.synchronize()
+    cache.check()
+    assert not cache.memory.any()
