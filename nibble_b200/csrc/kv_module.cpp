@@ -159,6 +159,8 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
                                   x.scalar_type() == at::kBFloat16 ? W4A16_TYPE_BF16 : W4A16_TYPE_F16, flags, current_stream()),
                      "apply_rotary");
     }
+    // (so that autograd, and whoever else goes by versions, sees that a tensor given as `out` has changed)
+    if (given.has_value() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }

@@ -237,6 +237,7 @@ def test_a_length_falls_to_the_block_before_the_last_tokens(pieces, dtype, head_
         cache.check()
 
 
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_tangents_are_refused():
     """Forward-mode differentiation and transformed tensors: no result that has lost them."""
     cache = QuantizedKVCache(1, 2, 64, 64)
@@ -260,3 +261,43 @@ def test_tangents_are_refused():
     torch.cuda.synchronize()
     cache.check()
     assert not cache.memory.any()
+
+
+def test_turning_in_place_counts_as_a_change():
+    """A tensor saved for a backward pass, and the fused layers' memory of their last input."""
+    from nibble_b200 import QuantizedLinear, fuse_parallel_linears
+
+    x, places, inv_freq = _draw((3, 4, 64), torch.float16, 28), _words([5, 6, 7]), torch.ones((32,), device="cuda")
+    weight = _draw((64, 64), torch.float16, 29).requires_grad_()
+    out = x @ weight
+    before = x._version
+    with torch.no_grad():
+        apply_rotary(x, places, inv_freq, out=x)
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    into = torch.empty_like(x)
+    kept = (x._version, into._version)
+    apply_rotary(x, places, inv_freq, out=into)
+    assert x._version == kept[0] and into._version > kept[1]
+    with torch.inference_mode():
+        plain = x.clone()
+        assert torch.equal(apply_rotary(plain, places, inv_freq, out=plain), into)
+        apply_rotary(x, places, inv_freq, out=into)
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            for seed, name in enumerate(("q_proj", "k_proj", "v_proj")):
+                linear = torch.nn.Linear(256, 128, bias=False)
+                linear.weight.data = _draw((128, 256), torch.float32, 30 + seed, 0.02).cpu()
+                setattr(self, name, QuantizedLinear.from_float(linear, group_size=128).cuda())
+
+    block = Block()
+    fuse_parallel_linears(block)
+    rows = _draw((3, 256), torch.float16, 33)
+    block.q_proj(rows)
+    apply_rotary(rows.view(3, 4, 64), places, inv_freq, out=rows.view(3, 4, 64))
+    got = block.k_proj(rows)
+    block.q_proj(torch.zeros_like(rows))
+    assert torch.equal(got, block.k_proj(rows.clone()))
