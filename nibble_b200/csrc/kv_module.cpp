@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <optional>
@@ -111,6 +112,49 @@ bool truth_of(PyObject* object) {
     return value != 0;
 }
 
+// Whether integers i_d, |i_d| < sizes[d], can make sum i_d * strides[d] equal to `offset`; strides falling from `dim` on.  True where
+// finding out would take long, as with strides that do not nest.
+bool reachable(const int64_t (&sizes)[4], const int64_t (&strides)[4], int dim, int64_t offset) {
+    if (dim == 4) return offset == 0;
+    int64_t within = 0;                                  // what the dimensions behind this one reach
+    for (int d = dim + 1; d < 4; ++d) within += (sizes[d] - 1) * strides[d];
+    const int64_t stride = strides[dim], most = sizes[dim] - 1;
+    if (most == 0 || stride == 0) return reachable(sizes, strides, dim + 1, offset);
+    // i * stride from offset - within to offset + within
+    int64_t low = offset - within, high = offset + within;
+    low = low >= 0 ? (low + stride - 1) / stride : -(-low / stride);
+    high = high >= 0 ? high / stride : -((-high + stride - 1) / stride);
+    low = std::max(low, -most);
+    high = std::min(high, most);
+    if (high - low > 3) return true;
+    for (int64_t i = low; i <= high; ++i) {
+        if (reachable(sizes, strides, dim + 1, offset - i * stride)) return true;
+    }
+    return false;
+}
+
+// Whether two tensors of the same sizes (four dimensions at most) and 16-bit type may share memory: by their extents, and where those
+// meet and the strides are the same, as of two parts of a fused row, exactly.
+bool may_share(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0) return false;
+    auto past = [](const at::Tensor& t) {
+        int64_t numbers = 1;
+        for (int64_t d = 0; d < t.dim(); ++d) numbers += (t.size(d) - 1) * t.stride(d);
+        return reinterpret_cast<uintptr_t>(t.const_data_ptr()) + static_cast<uintptr_t>(numbers) * 2;
+    };
+    const auto begin_a = reinterpret_cast<uintptr_t>(a.const_data_ptr()), begin_b = reinterpret_cast<uintptr_t>(b.const_data_ptr());
+    if (past(a) <= begin_b || past(b) <= begin_a) return false;
+    if (a.strides() != b.strides() || (begin_a - begin_b) % 2 != 0) return true;
+    int64_t sizes[4] = {1, 1, 1, 1}, strides[4] = {0, 0, 0, 0};
+    int order[4] = {0, 1, 2, 3};
+    std::sort(order, order + a.dim(), [&](int x, int y) { return a.stride(x) > a.stride(y); });
+    for (int64_t d = 0; d < a.dim(); ++d) {
+        sizes[d] = a.size(order[d]);
+        strides[d] = a.stride(order[d]);
+    }
+    return reachable(sizes, strides, 0, (static_cast<int64_t>(begin_a) - static_cast<int64_t>(begin_b)) / 2);
+}
+
 }  // namespace
 
 // rotary(x, positions, inv_freq, scale, interleaved, out or None) -> Tensor
@@ -134,14 +178,14 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
     at::Tensor out;
     if (given.has_value()) {
         out = *given;
+        TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type(), "out must be on the device of x and of its dtype");
         TORCH_CHECK(out.sizes() == x.sizes(), "out must have the shape of x");
         at::assert_no_internal_overlap(out);
         const bool in_place = out.data_ptr() == x.data_ptr() && out.strides() == x.strides();
-        TORCH_CHECK(in_place || at::get_overlap_status(out, x) == at::MemOverlapStatus::No, "out must be x itself or share no memory with it");
+        TORCH_CHECK(in_place || !may_share(out, x), "out must be x itself or share no memory with it");
     } else {
         out = at::detail::empty_cuda(x.sizes(), x.scalar_type(), x.device(), c10::nullopt);
     }
-    TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type(), "out must be on the device of x and of its dtype");
     TORCH_CHECK(x.numel() == 0 || (x.stride(-1) == 1 && out.stride(-1) == 1), "the last dimension of x and out must be contiguous");
     // (as [batch, tokens, heads, head_dim], dimensions that are not there having one entry)
     const int64_t missing = 4 - x.dim();

@@ -301,3 +301,39 @@ def test_turning_in_place_counts_as_a_change():
     got = block.k_proj(rows)
     block.q_proj(torch.zeros_like(rows))
     assert torch.equal(got, block.k_proj(rows.clone()))
+
+
+def test_turned_into_another_place():
+    """``out`` beside ``x``: memory of its own, rows with gaps, another part of the same rows; and what overlaps is refused."""
+    d, inv_freq = 64, (10000.0 ** (-torch.arange(0, 64, 2).double() / 64)).float().cuda()
+    places = _words([[4, 5, 6], [90, 91, 92]])
+    row = _draw((2, 3, 20 * d), torch.float16, 34)
+    q, k = row[..., :6 * d].unflatten(-1, (6, d)), row[..., 6 * d:12 * d].unflatten(-1, (6, d))
+    want = apply_rotary(q.contiguous(), places, inv_freq)
+    apart = torch.zeros((2, 3, 6, d), dtype=torch.float16, device="cuda")
+    assert apply_rotary(q, places, inv_freq, out=apart) is apart and torch.equal(apart, want)
+    slot = torch.zeros((2, 3, 9, d + 8), dtype=torch.float16, device="cuda")
+    apply_rotary(q, places, inv_freq, out=slot[:, :, 2:8, :d])
+    assert torch.equal(slot[:, :, 2:8, :d], want) and not slot[:, :, :2].any() and not slot[:, :, 8:].any() and not slot[..., d:].any()
+    by_head = torch.zeros((2, 6, 3, d), dtype=torch.float16, device="cuda").transpose(1, 2)
+    assert torch.equal(apply_rotary(q, places, inv_freq, out=by_head), want)
+    kept = row.clone()
+    apply_rotary(q, places, inv_freq, out=k)                                       # the same rows, the part behind
+    assert torch.equal(k, want) and torch.equal(row[..., :6 * d], kept[..., :6 * d]) and torch.equal(row[..., 12 * d:], kept[..., 12 * d:])
+    apply_rotary(q[:, :1], places[:, :1].contiguous(), inv_freq, out=q[:, 1:2])     # the next token's row
+    assert torch.equal(q[:, 1:2], want[:, :1])
+    one = row[0, 0].view(20, d)
+    kept = one.clone()
+    apply_rotary(one[0:16:2], _words(7), inv_freq, out=one[1:17:2])                # every other head into its neighbour
+    assert torch.equal(one[0:16:2], kept[0:16:2]) and torch.equal(one[17:], kept[17:])
+    assert torch.equal(one[1:17:2], apply_rotary(kept[0:16:2], _words(7), inv_freq))
+    kept = row.clone()
+    for into in (row[..., d:7 * d].unflatten(-1, (6, d)), row[..., 1:6 * d + 1].unflatten(-1, (6, d)), row[..., 5 * d:11 * d].unflatten(-1, (6, d)),
+                 row[..., :12 * d].unflatten(-1, (6, 2 * d))[..., :d], row.view(-1).as_strided((2, 3, 6, d), (3 * 20 * d, 20 * d, d, 1), 8),
+                 q.float(), q.bfloat16(), q[:, :, :5], q.cpu()):
+        with pytest.raises(RuntimeError):
+            apply_rotary(q, places, inv_freq, out=into)
+    with pytest.raises(RuntimeError):
+        apply_rotary(q[:, :2], places[:, :2].contiguous(), inv_freq, out=q[:, 1:])
+    torch.cuda.synchronize()
+    assert torch.equal(row, kept)
