@@ -305,7 +305,7 @@ kv_attention_kernel(const AttentionParams p) {
         }
         const unsigned slot = feed.fill % kSlots;
         if (MT > 1 && feed.fill >= kSlots &&
-            !mbar_wait(smem_u32(&bars[team][slot][1]), (feed.fill / kSlots - 1) & 1, kKvGaveUp, p.cache.status)) {
+            !mbar_wait<false, true>(smem_u32(&bars[team][slot][1]), (feed.fill / kSlots - 1) & 1, kKvGaveUp, p.cache.status)) {
             healthy = false;
             return;
         }
@@ -320,7 +320,7 @@ kv_attention_kernel(const AttentionParams p) {
     // A slot, once it has been filled; null if that did not happen.
     auto arrived = [&](unsigned number) -> const uint8_t* {
         const unsigned slot = number % kSlots;
-        healthy = mbar_wait(smem_u32(&bars[team][slot][0]), (number / kSlots) & 1, kKvGaveUp, p.cache.status) && healthy;
+        healthy = mbar_wait<false, true>(smem_u32(&bars[team][slot][0]), (number / kSlots) & 1, kKvGaveUp, p.cache.status) && healthy;
         healthy = __all_sync(0xffffffffu, healthy);
         return healthy ? ring + slot * Shape::kSlotBytes : nullptr;
     };
@@ -666,7 +666,7 @@ kv_attention_kernel(const AttentionParams p) {
     }
     if (!healthy && feeder) {                       // wait, within limits, for copies that are still on their way
         for (unsigned s = take; s < feed.fill; ++s) {
-            mbar_wait(smem_u32(&bars[team][s % kSlots][0]), (s / kSlots) & 1, kKvGaveUp, p.cache.status);
+            mbar_wait<false, true>(smem_u32(&bars[team][s % kSlots][0]), (s / kSlots) & 1, kKvGaveUp, p.cache.status);
         }
     }
 }

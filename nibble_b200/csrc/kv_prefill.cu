@@ -363,7 +363,7 @@ kv_prefill_kernel(const PrefillParams p) {
     bool healthy = true;
     // Waits for phase number `n` of a barrier; by a converged warp, all of whose lanes then know whether it came.
     auto wait = [&](unsigned long long& bar, int n) {
-        if (healthy) healthy = mbar_wait(smem_u32(&bar), n & 1, kKvGaveUp, p.cache.status);
+        if (healthy) healthy = mbar_wait<false, true>(smem_u32(&bar), n & 1, kKvGaveUp, p.cache.status);
         healthy = __all_sync(0xffffffffu, healthy);
     };
     // This warp's arrival, behind its writes to shared memory for the tensor core.
@@ -825,7 +825,7 @@ kv_prefill_kernel(const PrefillParams p) {
             }
         }
         if (!healthy && lane == 0) {                     // wait, within limits, for copies that may still be on their way
-            for (int which = 0; which < 2; ++which) mbar_wait(smem_u32(&bars.codes[mine][which]), read & 1, kKvGaveUp, p.cache.status);
+            for (int which = 0; which < 2; ++which) mbar_wait<false, true>(smem_u32(&bars.codes[mine][which]), read & 1, kKvGaveUp, p.cache.status);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssuerRegisters));
@@ -897,7 +897,7 @@ kv_prefill_kernel(const PrefillParams p) {
         }
         // nothing may be in flight when TMEM goes
         for (int t = 0; t < 2; ++t) {
-            if (used[t] > 0) mbar_wait(smem_u32(&bars.o_done[t]), (used[t] - 1) & 1, kKvGaveUp, p.cache.status);
+            if (used[t] > 0) mbar_wait<false, true>(smem_u32(&bars.o_done[t]), (used[t] - 1) & 1, kKvGaveUp, p.cache.status);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

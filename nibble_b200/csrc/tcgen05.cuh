@@ -31,8 +31,8 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(unsigned bar, unsigned byt
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // Bounded wait for the phase with the given parity to complete.  False (and a status code) on give-up.  `kCluster`: of a barrier at
-// which threads or copies of the cluster's other CTAs arrive.
-template <bool kCluster = false>
+// which threads or copies of the cluster's other CTAs arrive.  `kBits`: the status word is one of bits, of which the code is one.
+template <bool kCluster = false, bool kBits = false>
 __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, unsigned code, unsigned* status) {
     for (unsigned spin = 0; spin < kSpinLimit; ++spin) {
         unsigned done;
@@ -55,7 +55,8 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, unsigne
         }
         if (done) return true;
     }
-    atomicMax(status, code);
+    if constexpr (kBits) atomicOr(status, code);
+    else atomicMax(status, code);
     return false;
 }
 // Whether that phase has completed, without waiting.
