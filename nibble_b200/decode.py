@@ -307,6 +307,14 @@ class LlamaDecodeRunner:
                 torch._foreach_copy_(kept, copies)
             self._graph.replay()
 
+    def _check_caches(self) -> None:
+        """Raises if 8-bit caches report a position that did not fit, or a wait that gave up, since the last ``reset``."""
+        if self.caches is not None:
+            words = int(torch.cat(self._cache_status).bitwise_and(3).amax().item())
+            if words != 0:
+                raise RuntimeError("a decode step ran past the end of the KV cache" if words == 1 else
+                                   "attention over the 8-bit cache gave up waiting; its output is incomplete")
+
     def reset(self) -> None:
         self.position.zero_()
         self.status.zero_()
@@ -340,7 +348,8 @@ class LlamaDecodeRunner:
         self.position.fill_(count)
         from .cuda import check_device_status
 
-        check_device_status()      # the batched forward ran the prefill kernels: none of their waits may have given up
+        check_device_status()      # the batched forward ran the prefill kernels: none of their waits may have given up,
+        self._check_caches()       # nor one of the attention over 8-bit caches
 
     # Tokens of a prompt that go through the model together with an 8-bit cache: enough to fill the machine, and activations stay small.
     PREFILL_CHUNK = 2048
@@ -385,11 +394,7 @@ class LlamaDecodeRunner:
                 self.step()
         if int(self.status.item()) != 0:
             raise RuntimeError("a decode step ran past the end of the KV cache")
-        if self.caches is not None:
-            words = int(torch.cat(self._cache_status).bitwise_and(3).amax().item())
-            if words != 0:
-                raise RuntimeError("a decode step ran past the end of the KV cache" if words == 1 else
-                                   "attention over the 8-bit cache gave up waiting; its output is incomplete")
+        self._check_caches()
         if self.persistent and int(self.step_status.item()) != 0:
             code = int(self.step_status.item())
             raise RuntimeError("a decode step ran past the end of the KV cache" if code == 1 else
