@@ -644,10 +644,9 @@ kv_read_kernel(const ReadParams p) {
     const int b = pair / p.cache.kv_heads, head = pair % p.cache.kv_heads;
     long long length = p.lengths[b];
     long long first = p.first == nullptr ? 0 : p.first[b];
-    if (length < 0 || length > p.cache.max_len || first < 0) {
+    if (length < 0 || length > p.cache.max_len || first < 0 || first > p.cache.max_len) {
         if (tid == 0) atomicOr(p.cache.status, kKvBadLength);
-        length = 0;
-        first = max(first, 0ll);
+        length = first = 0;
     }
     const long long block = first / kKvBlock + chunk;
     const int slot = line / kRuns / 2 * 16 + lane / 4 * 2 + line / kRuns % 2;

@@ -337,3 +337,20 @@ def test_turned_into_another_place():
         apply_rotary(q[:, :2], places[:, :2].contiguous(), inv_freq, out=q[:, 1:])
     torch.cuda.synchronize()
     assert torch.equal(row, kept)
+
+
+@pytest.mark.parametrize("length", [40, 64, 70])
+def test_reading_from_a_place_beyond_the_cache(length):
+    """Zeros, and reported, as for a length or start that does not fit; up to the cache's end there is nothing to report."""
+    x = _draw((3, 70, 1, 64), torch.float16, 35)
+    cache = QuantizedKVCache(3, 1, 70, 64)
+    cache.append(x, x, _words([0, 0, 0]))
+    lengths = _words([length] * 3)
+    got, _ = cache.read(lengths, first=_words([70, length, 0]), tokens=40)
+    assert not got[:2].any() and torch.equal(got[2], _held(x, [length] * 3)[2, :40])
+    cache.check()
+    for first in (71, 1 << 33, (1 << 63) - 1, (1 << 63) - 40, -1, -(1 << 63)):
+        for part in cache.read(lengths, first=_words([first, 0, first]), tokens=40):
+            assert not part[0].any() and not part[2].any() and torch.equal(part[1], _held(x, [length] * 3)[1, :40]), first
+        with pytest.raises(RuntimeError, match="did not fit"):
+            cache.check()
