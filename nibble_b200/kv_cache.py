@@ -106,11 +106,9 @@ class QuantizedKVCache:
     def check(self) -> None:
         """Raises if a call since the last check was given a length, start or count that does not fit, or gave up a bounded wait.
         Synchronises; clears what it reports."""
-        with torch.inference_mode():                 # (in which a cache made under it may be written too)
-            word = self.memory[:4].view(torch.int32)
-            status = int(word.item())
-            if status:
-                word.zero_()
+        word = self.memory[:4].view(torch.int32)
+        status = int(word.item())
         if status:
+            word.zero_()
             raise RuntimeError("attention over the 8-bit cache gave up waiting; its output is incomplete" if status & 2 else
                                "a length, start or count did not fit the 8-bit cache")

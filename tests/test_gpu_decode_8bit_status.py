@@ -40,14 +40,3 @@ def test_a_prompt_in_chunks_reports_what_its_caches_do(word, what):
     runner.prefill(prompt)
     for cache in runner.caches:
         cache.check()
-
-
-def test_a_cache_made_under_inference_mode_reports_outside_of_it():
-    x = torch.zeros((1, 1, 1, 64), dtype=torch.float16, device="cuda")
-    with torch.inference_mode():
-        cache = QuantizedKVCache(1, 1, 64, 64)
-    cache.append(x, x, torch.tensor([64], device="cuda"))
-    with pytest.raises(RuntimeError, match="did not fit"):
-        cache.check()
-    cache.check()
-    assert not cache.memory.any()
