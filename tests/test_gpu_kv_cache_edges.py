@@ -354,3 +354,72 @@ def test_reading_from_a_place_beyond_the_cache(length):
             assert not part[0].any() and not part[2].any() and torch.equal(part[1], _held(x, [length] * 3)[1, :40]), first
         with pytest.raises(RuntimeError, match="did not fit"):
             cache.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads", "head_dim", "length", "spread"), [
+    (1, 64, 8, 64, 900, 1.0), (5, 32, 8, 128, 2000, 2.0), (64, 16, 4, 64, 1000, 1.0), (150, 16, 2, 128, 3000, 1.0), (150, 16, 2, 128, 700, 3.0),
+    (600, 8, 1, 64, 600, 0.3)])
+def test_errors_are_of_the_size_of_their_roundings(tokens, q_heads, kv_heads, head_dim, length, spread, dtype):
+    """The root of the mean square of what results are off by, against that of the roundings they are made with: the result's own, evenly
+    spread over a step (step^2 / 12), and a weight's to FP16, evenly spread over 2^-11 of it to either side at most (a third of that
+    squared).  Few FP16 rows: the result's alone.  Where the sum is of the rounded weights (many FP16 rows) an error of p_t moves the result by
+    p_t e_t (v_t - out), elsewhere by p_t e_t v_t.  1.03 for what is not in the sum: FP32's roundings, some 2^-18 of p, and the sample."""
+    k, v = _draw((1, length, kv_heads, head_dim), dtype, 36), _draw((1, length, kv_heads, head_dim), dtype, 37)
+    cache = QuantizedKVCache(1, kv_heads, length, head_dim, dtype=dtype)
+    cache.append(k, v, _words([0]))
+    q = _draw((1, tokens, q_heads, head_dim), dtype, 38, spread)
+    got = cache.attention(q, _words([length]))[0].double()
+    group, few = q_heads // kv_heads, tokens * q_heads // kv_heads <= 32
+    kb, vb = oracle.held(k[0], length), oracle.held(v[0], length)
+    hidden = torch.arange(length, device="cuda")[None, :] > (length - tokens + torch.arange(tokens, device="cuda"))[:, None]
+    off = allowed = 0.0
+    for head in range(kv_heads):
+        rows = slice(head * group, (head + 1) * group)
+        scores = torch.einsum("ihd,td->iht", q[0, :, rows].double(), kb[:, head]) * head_dim ** -0.5
+        p = torch.softmax(scores.masked_fill(hidden[:, None, :], float("-inf")), -1)
+        values = vb[:, head]
+        out = p @ values
+        off += float((got[:, rows] - out).square().sum())
+        step = torch.finfo(dtype).eps * 2.0 ** out.abs().clamp_min(2.0 ** -14).log2().floor()
+        allowed += float(step.square().sum()) / 12
+        if few and dtype == torch.float16:
+            continue
+        moved = p.square() @ values.square()
+        if dtype == torch.float16:
+            moved = moved - 2 * out * (p.square() @ values) + out.square() * p.square().sum(-1, keepdim=True)
+        allowed += float(moved.sum()) * 2.0 ** -22 / 3
+    assert off ** 0.5 <= 1.03 * allowed ** 0.5, (off / allowed) ** 0.5
+
+
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads", "head_dim", "length"), [
+    (1, 32, 4, 64, 500), (1, 8, 1, 128, 3001), (5, 16, 2, 64, 999), (90, 8, 2, 64, 1500), (200, 16, 2, 128, 700)])
+@pytest.mark.parametrize("spread", [1.0, 3.0])
+def test_bf16_sums_are_of_weights_that_are_not_rounded(tokens, q_heads, kv_heads, head_dim, length, spread):
+    """So that of the bound on a kernel's error the part for a rounded sum, 2^-11 of the result, falls away."""
+    k, v = _draw((1, length, kv_heads, head_dim), torch.bfloat16, 39), _draw((1, length, kv_heads, head_dim), torch.bfloat16, 40)
+    cache = QuantizedKVCache(1, kv_heads, length, head_dim, dtype=torch.bfloat16)
+    cache.append(k, v, _words([0]))
+    q = _draw((1, tokens, q_heads, head_dim), torch.bfloat16, 41, spread)
+    got = cache.attention(q, _words([length]))[0].double()
+    kb, vb = oracle.held(k[0], length), oracle.held(v[0], length)
+    want, weight = oracle.attention(q[0], kb, vb, length, tokens, head_dim ** -0.5)
+    bound = oracle.attention_bound(want, weight, torch.bfloat16, float(vb.abs().max()) * length) - want.abs() * 2.0 ** -11
+    assert ((got - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads", "head_dim"), [(1, 8, 2, 64), (5, 8, 1, 128), (12, 8, 2, 64), (90, 8, 2, 64), (300, 16, 1, 128)])
+def test_a_cache_far_larger_than_what_it_holds(tokens, q_heads, kv_heads, head_dim, dtype):
+    """Runs and pieces are cut for the longest sequence that a cache takes; short and long ones in one of 50000 tokens, and in one that is
+    full."""
+    lengths = [tokens, 500, 33, 40, 1203]
+    k, v = _draw((5, 1203, kv_heads, head_dim), dtype, 42), _draw((5, 1203, kv_heads, head_dim), dtype, 43)
+    q = _draw((5, tokens, q_heads, head_dim), dtype, 44)
+    for max_len in (1203, 50000):
+        cache = QuantizedKVCache(5, kv_heads, max_len, head_dim, dtype=dtype)
+        cache.append(k, v, _words([0] * 5), _words(lengths))
+        first = _check_attention(cache, k, v, q, lengths, None)
+        for _ in range(3):
+            assert torch.equal(cache.attention(q, _words(lengths)), first)
+        cache.check()
