@@ -668,21 +668,15 @@ kv_prefill_kernel(const PrefillParams p) {
             }
             if (w.held > 0 && w.full % kStepBlocks == mine && w.full / kStepBlocks >= w.begin && w.full / kStepBlocks < w.stop) {
                 // What the numbers of the block that is being filled are multiplied with, and the scale that stands for it.  FP16 keys
-                // stay as they are, BF16 ones stay BF16.  FP16 values, where they are smaller, are brought to the size of codes, so that
-                // weights keep as many bits beside small ones; all stay exact.  BF16 values become FP16 just below its largest: they
-                // keep their bits down to 2^-32 of the block's largest, and below 2^-40 of it count as zero.  (As codes they count as zero
-                // below 2^-8 of it.)
+                // stay as they are, BF16 ones stay BF16; values, which become FP16, are brought to the size of codes, so that weights
+                // keep as many bits beside small ones.  Values keep their bits down to 2^-23 of the block's largest (BF16 2^-26), and
+                // below 2^-34 of it count as zero.  (As codes they count as zero below 2^-8 of it; with more room for them weights
+                // would have less, 2^-18 of a row's largest instead of 2^-24.)
                 const size_t tail = (static_cast<size_t>(pair) * 2 + (w.full & 1)) * kKvBlock * D;
                 float4 factors = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
                 if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane, odd_values), factors.y);
                 const float largest = finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane, odd_values);
                 factors.z = power_for(largest, factors.w);
-                if (kBf16) {
-                    factors.z *= 64.0f;
-                    factors.w *= 1.0f / 64.0f;
-                } else if (factors.z < 1.0f) {
-                    factors.z = factors.w = 1.0f;
-                }
                 if (largest == 0.0f) factors.w = 0.0f;       // (it counts for no more than a full block of zeros)
                 if (lane == 0) tail_factors[mine] = factors;
                 __syncwarp();

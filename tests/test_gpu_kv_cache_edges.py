@@ -111,7 +111,7 @@ def _block_tops(v, length):
     """The largest magnitude of each token's block (of its own, where the block is being filled): [length, heads]."""
     tops = v[:length].double().abs().amax(-1)
     full = length // 32 * 32
-    tops[:full] = tops[:full].view(-1, 32, v.shape[1]).amax(1, keepdim=True).expand(-1, 32, -1).reshape(full, -1)
+    tops[:full] = tops[:full].view(full // 32, 32, v.shape[1]).amax(1, keepdim=True).expand(-1, 32, -1).reshape(full, v.shape[1])
     return tops
 
 
@@ -119,7 +119,8 @@ def _check_seen(cache, k, v, q, length, scale):
     """Attention against its definition, within what the tokens that a query sees allow: a weight (probability times its values' scale)
     is held in FP16 times 2^10 relative to the largest one seen, M / 127 at most with M the largest p x (largest of the token's block).
     What is below FP16's normal numbers is off by half a step, 2^-25: times a code of 127 at most that is 2^-35 of M for each token;
-    times a number of the block being filled, held up to 2^16, 2^-25 x 2^-10 x 2^16 / 127 < 2^-25 of it, 31 of them 2^-20.  A sum of rounded
+    times a number of the block being filled, held up to 2^10, 2^-25 x 2^-10 x 2^10 / 127 < 2^-31 of it, 31 of them 2^-26; and such a number
+    itself is off by 2^-34 of the block's largest (2^-25 of 2^9), which a query may not see, times its probability.  A sum of rounded
     weights is off by 2^-31 of itself for each of them at most (their scale is 2^-4 of the largest's or more).  The rest is
     kv_oracle.attention_bound's."""
     got = cache.attention(q, _words([length]), softmax_scale=scale)[0].double()
@@ -135,7 +136,10 @@ def _check_seen(cache, k, v, q, length, scale):
         p = torch.softmax(scores.masked_fill(hidden[:, None, :], float("-inf")), -1)
         most = (p * tops[:, head]).amax(-1, keepdim=True)
         bound = oracle.attention_bound(want[:, rows], weight[:, rows], q.dtype, 0.0)
-        bound = bound + most * (length * 2.0 ** -35 + 2.0 ** -20) + want[:, rows].abs() * length * 2.0 ** -31
+        bound = bound + most * (length * 2.0 ** -35 + 2.0 ** -26) + want[:, rows].abs() * length * 2.0 ** -31
+        full = length // 32 * 32
+        if full < length:
+            bound = bound + p[..., full:].sum(-1, keepdim=True) * float(v[0, full:length, head].abs().max()) * 2.0 ** -34
         off = (got[:, rows] - want[:, rows]).abs()
         assert (off <= bound).all(), (head, float((off / bound).max()))
     cache.check()
