@@ -45,11 +45,9 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMinRun = 4;                      // blocks that are worth a CTA: one a warp (500 tokens 6.9 us; with eight 8.0)
 constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHeadroom = 10.0f;              // weights are held in FP16 times 2^10,
+// (weights are held in FP16 times 2^kHeadroom)
 constexpr float kMaxLag = 3.0f;                 // times 2^3 where the maximum has not been followed yet,
 constexpr float kMaxRise = 2.0f;                // times 2^2 where the values' scale has not: below 65504 in all
-constexpr float kLightest = -100.0f;            // values' scales below 2^-100 count as that where weights are compared
 
 struct AttentionParams {
     KvCache cache;
@@ -66,15 +64,6 @@ struct AttentionParams {
     float* parts;                                // workspace: see part_of()
     int grid;                                    // CTAs of the first kernel
 };
-
-// row / group; rows are fewer than 2^24, so that the quotient in FP32 is off by one at most.
-__device__ __forceinline__ int by_group(const AttentionParams& p, int row) {
-    int quotient = static_cast<int>(static_cast<float>(row) * p.per_group);
-    const int rest = row - quotient * p.group;
-    if (rest < 0) --quotient;
-    if (rest >= p.group) ++quotient;
-    return quotient;
-}
 
 struct Sequence {
     int length, count, blocks, row_tiles;        // full blocks; tiles of this sequence's queries
@@ -154,33 +143,10 @@ __device__ __forceinline__ bool next_segment(const AttentionParams& p, int end, 
     return false;
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Four codes of a word as (c0, c2) and (c1, c3).
-__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& even, uint32_t& odd) {
-    even = hsub2_u32(and_xor(word, 0x00ff00ffu, 0x64806480u), 0x64806480u);
-    odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
-}
-
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
 }
 
 // A matrix of 8 x 8 16-bit numbers, two of a row in each lane, transposed across the warp.
@@ -938,7 +904,7 @@ int launch_shape(const AttentionParams& p, const Shape& s, bool programmatic, cu
     // Behind the first kernel always programmatic: it waits for that one itself.  Four warps a row while rows are few.
     const int64_t pairs = static_cast<int64_t>(p.cache.batch) * p.cache.kv_heads, rows = p.tokens * static_cast<int64_t>(p.group);
     const bool few = pairs * rows <= 1024;
-    const int rows_per_cta = few ? 1 : rows <= 64 ? 4 : 32;
+    const int rows_per_cta = few ? 1 : 4;
     const int64_t ctas = pairs * ((rows + rows_per_cta - 1) / rows_per_cta);
     return kv_launch(few ? kv_finish_kernel<T, D, 4> : kv_finish_kernel<T, D, 1>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), 0,
                      s.grid > 0 || programmatic, stream, p, rows_per_cta);

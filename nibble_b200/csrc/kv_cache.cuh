@@ -22,12 +22,16 @@
 #include <stdint.h>
 
 #include "kernels.h"
+#include "unpack.cuh"
 
 namespace w4a16 {
 
 constexpr int kKvBlock = 32;           // tokens that share a scale
 constexpr unsigned kKvBadLength = 1;   // status: a length or count outside the cache
 constexpr unsigned kKvGaveUp = 2;      // status: a bounded wait ran out
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHeadroom = 10.0f;           // weights of attention's second product, exp2(score) times the values' scale, are held in FP16 times 2^10
+constexpr float kLightest = -100.0f;         // values' scales below 2^-100 count as that where weights are compared
 constexpr float kShrink = 0x1p-32f;      // BF16: sums of values over tokens are held times this, so that those of its largest are finite
 constexpr float kNone = -3.4028235e38f;      // the maximum of nothing: no score is below it but minus infinity
 
@@ -120,15 +124,43 @@ __device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The power of two at or above a positive normal number.
-__device__ __forceinline__ float next_power(float x) { return __uint_as_float((__float_as_uint(x) + 0x007fffffu) & 0xff800000u); }
-
 // A power of two that brings `top`, finite and not negative, to between 2^9 and 2^10 (1 for zero), and its inverse.  Both are normal
 // numbers for all that FP32 has down to 2^-109; what is below that comes to less than 2^9, which loses none of its bits.
 __device__ __forceinline__ float power_for(float top, float& inverse) {
     const int exponent = top > 0.0f ? min(118, 9 - ilogbf(top)) : 0;
     inverse = __int_as_float((127 - exponent) << 23);
     return __int_as_float((127 + exponent) << 23);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) { return narrow2<__half>(a, b); }
+
+// Four codes of a word as (c0, c2) and (c1, c3).
+__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& even, uint32_t& odd) {
+    even = hsub2_u32(and_xor(word, 0x00ff00ffu, 0x64806480u), 0x64806480u);
+    odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
+}
+
+// row / group, for attention's parameters of either kernel; rows are fewer than 2^24, so that the quotient in FP32 is off by one at most.
+template <typename Params>
+__device__ __forceinline__ int by_group(const Params& p, int row) {
+    int quotient = static_cast<int>(static_cast<float>(row) * p.per_group);
+    const int rest = row - quotient * p.group;
+    if (rest < 0) --quotient;
+    if (rest >= p.group) ++quotient;
+    return quotient;
+}
+
+// A copy into shared memory that counts its bytes on an mbarrier; addresses and size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 template <typename... Params, typename... Args>

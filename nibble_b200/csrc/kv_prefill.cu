@@ -59,10 +59,7 @@ constexpr int kPrefillThreads = (kMmaWarp + 4) * 32;      // (registers are hand
 // scores, is short of.
 constexpr int kSoftmaxRegisters = 208, kDequantRegisters = 64, kIssuerRegisters = 32;
 static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 * 128);
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHeadroom = 10.0f;              // weights are held in FP16 times 2^10
-constexpr float kLightest = -100.0f;            // BF16 values' scales below 2^-100 count as that where weights are compared,
-constexpr float kLightestHalf = -40.0f;         // FP16 ones, all of which are above it but zero, as this
+constexpr float kLightestHalf = -40.0f;         // the same for FP16 (kLightest): all scales are above it but zero
 constexpr float kFar = 0x1p16f;                 // a score that is so large is rounded before the maximum is taken off
 constexpr float kLargestSum = 65000.0f;         // of a block's weights: none is beyond FP16 then
 
@@ -82,14 +79,6 @@ struct PrefillParams {
     float* parts;                                // [piece][256][D + 4]: sums, what they are relative to (as two logarithms), sum of probabilities
     int units, whole, pieces;                    // units in all; those of full rounds; pieces of each of the others
 };
-
-__device__ __forceinline__ int by_group(const PrefillParams& p, int row) {
-    int quotient = static_cast<int>(static_cast<float>(row) * p.per_group);
-    const int rest = row - quotient * p.group;
-    if (rest < 0) --quotient;
-    if (rest >= p.group) ++quotient;
-    return quotient;
-}
 
 // A unit or a piece of one: steps [begin, stop) of its visible tokens.
 struct Work {
@@ -153,11 +142,6 @@ struct PrefillBarriers {
     unsigned long long codes[kDequantWarps][2];
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // Two FP32 operations an instruction.
 __device__ __forceinline__ uint64_t pair_of(uint32_t a, uint32_t b) {
     uint64_t d;
@@ -190,15 +174,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& even, uint32_t& odd) {
-    even = hsub2_u32(and_xor(word, 0x00ff00ffu, 0x64806480u), 0x64806480u);
-    odd = hsub2_u32(and_xor(word >> 8, 0x00ff00ffu, 0x64806480u), 0x64806480u);
-}
-// The same as BF16, whose seven bits behind the point hold a code's lower seven beside 128: the bit of its sign is what 256 has and 128 has
+// codes_to_half() as BF16, whose seven bits behind the point hold a code's lower seven beside 128: the bit of its sign is what 256 has and 128 has
 // not.  (128 + lower seven) - (128 or 256).
 __device__ __forceinline__ uint32_t two_codes_to_bf16(uint32_t word) {
     const uint32_t lower = (word & 0x007f007fu) | 0x43004300u, sign = (word & 0x00800080u) | 0x43004300u;
@@ -208,12 +184,6 @@ __device__ __forceinline__ uint32_t two_codes_to_bf16(uint32_t word) {
 __device__ __forceinline__ void codes_to_bf16(uint32_t word, uint32_t& even, uint32_t& odd) {
     even = two_codes_to_bf16(word);
     odd = two_codes_to_bf16(word >> 8);
-}
-
-__device__ __forceinline__ void bulk_load(unsigned dst, const void* src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
 }
 
 // D (TMEM) += A (shared memory) x B (shared memory).

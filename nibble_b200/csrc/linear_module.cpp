@@ -233,15 +233,15 @@ PyMethodDef methods[] = {
     {"quantize_pack", method(quantize_pack), METH_FASTCALL, "quantize_pack(weights, group_size) -> (Tensor, Tensor) or NotImplemented"},
     {"uses_fused_kernel", method(rule), METH_FASTCALL, "uses_fused_kernel(rows, out_features, in_features, group_size) -> bool"},
     {"rotary", method(w4a16::rotary), METH_FASTCALL,
-     "rotary(x, positions, inv_freq, scale, interleaved, out or None, programmatic) -> Tensor"},
+     "rotary(x, positions, inv_freq, scale, interleaved, out or None) -> Tensor"},
     {"kv8_bytes", method(w4a16::kv8_bytes), METH_FASTCALL, "kv8_bytes(batch, kv_heads, max_len, head_dim) -> int, 0 where they do not fit"},
     {"kv8_append", method(w4a16::kv8_append), METH_FASTCALL,
      "kv8_append(memory, batch, kv_heads, max_len, head_dim, type, k, v, start, counts or None, inv_freq or None, rope_scale, interleaved, "
-     "q or None, programmatic) -> turned q or None"},
+     "q or None) -> turned q or None"},
     {"kv8_read", method(w4a16::kv8_read), METH_FASTCALL,
-     "kv8_read(memory, batch, kv_heads, max_len, head_dim, type, lengths, first or None, tokens, programmatic) -> (Tensor, Tensor)"},
+     "kv8_read(memory, batch, kv_heads, max_len, head_dim, type, lengths, first or None, tokens) -> (Tensor, Tensor)"},
     {"kv8_attention", method(w4a16::kv8_attention), METH_FASTCALL,
-     "kv8_attention(memory, batch, kv_heads, max_len, head_dim, type, q, lengths, counts or None, softmax_scale, programmatic) -> Tensor"},
+     "kv8_attention(memory, batch, kv_heads, max_len, head_dim, type, q, lengths, counts or None, softmax_scale) -> Tensor"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_C", "Native side of nibble_b200: torch operators and QuantizedLinear.forward.", -1,
