@@ -1,15 +1,14 @@
 // Attention of many new tokens (a prompt, or a chunk of one) over the 8-bit cache, on the 5th-generation tensor cores.
 //
-// The same definition as kv_attention.cu, and the same arithmetic: codes are exact integers in both products (of FP16; scores of BF16
-// caches are products of BF16, so that queries and keys of any size keep their bits), the keys' scales multiply FP32 scores, the
-// values' scales enter the probabilities before those are rounded to FP16 (relative to the largest such weight that the row has seen,
-// times 2^10; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
+// The same definition as kv_attention.cu, and the same arithmetic: codes are exact FP16 integers in both products, the keys' scales
+// multiply FP32 scores, the values' scales enter the probabilities before those are rounded to FP16 (relative to the largest such weight that the row has seen,
+// times 2^9; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
 //
 // A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
 // against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's sixteen warps, one CTA per SM:
 //   warps 0-3, 4-7   softmax of tile A and of tile B: a thread per row.  Stages its row of queries, then in every step takes the
 //                    row's 128 scores out of TMEM, leaves the probabilities there, and in the end takes the output.
-//   warps 8-11       make 16-bit operands in shared memory of a block's codes each (which they have copied in a step ahead), swizzled by
+//   warps 8-11       make FP16 operands in shared memory of a block's codes each (which they have copied in a step ahead), swizzled by
 //                    128 bytes: keys [token][d], values [d][token]; of the block that is being filled, of its 16-bit numbers; zeros
 //                    behind the last.
 //   warp 12          (13-15: nothing) allocates TMEM and issues the MMAs: S = Q K^T with both operands in shared memory, O += P V
@@ -56,11 +55,20 @@ constexpr int kSoftmaxWarps = 8, kDequantWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kDequantWarps;
 constexpr int kPrefillThreads = (kMmaWarp + 4) * 32;      // (registers are handed over by four warps at a time)
 // Registers of a thread: of 128 at launch the makers of operands and the issuer give up what the softmax, which holds a row's 128
-// scores, is short of.
-constexpr int kSoftmaxRegisters = 208, kDequantRegisters = 64, kIssuerRegisters = 32;
-static_assert(2 * kSoftmaxRegisters + kDequantRegisters + kIssuerRegisters <= 4 * 128);
+// scores, is short of.  FP16 at D = 128 leaves the makers more (2048 queries at 8192: 488 us, with the others' split 503); the others do not
+// (D = 64 FP16 229 and 222, BF16 94 and 92; D = 128 BF16 255 and 248).
+template <typename T, int D>
+struct PrefillRegisters {
+    static constexpr bool kMakersMore = std::is_same<T, __half>::value && D == 128;
+    static constexpr int kSoftmax = kMakersMore ? 200 : 208, kDequant = kMakersMore ? 80 : 64, kIssuer = 32;
+    static_assert(2 * kSoftmax + kDequant + kIssuer <= 4 * 128);
+};
+constexpr float kHeadroom = 9.0f;               // weights are held in FP16 times 2^9 (times 2^10 they outgrow it sooner: 3 % at D = 64)
 constexpr float kLightestHalf = -40.0f;         // the same for FP16 (kLightest): all scales are above it but zero
 constexpr float kFar = 0x1p16f;                 // a score that is so large is rounded before the maximum is taken off
+// What is noted of the block that is being filled: values that are infinite or NaN; BF16 keys or values that lie so far apart that the
+// small ones would not keep their bits beside the largest.
+constexpr unsigned kOddValues = 1, kApart = 2;
 constexpr float kLargestSum = 65000.0f;         // of a block's weights: none is beyond FP16 then
 
 struct PrefillParams {
@@ -174,18 +182,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// codes_to_half() as BF16, whose seven bits behind the point hold a code's lower seven beside 128: the bit of its sign is what 256 has and 128 has
-// not.  (128 + lower seven) - (128 or 256).
-__device__ __forceinline__ uint32_t two_codes_to_bf16(uint32_t word) {
-    const uint32_t lower = (word & 0x007f007fu) | 0x43004300u, sign = (word & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 codes = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lower), *reinterpret_cast<const __nv_bfloat162*>(&sign));
-    return *reinterpret_cast<const uint32_t*>(&codes);
-}
-__device__ __forceinline__ void codes_to_bf16(uint32_t word, uint32_t& even, uint32_t& odd) {
-    even = two_codes_to_bf16(word);
-    odd = two_codes_to_bf16(word >> 8);
-}
-
 // D (TMEM) += A (shared memory) x B (shared memory).
 __device__ __forceinline__ void umma_f16_shared(unsigned tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instr_desc,
                                                 uint32_t accumulate) {
@@ -260,24 +256,94 @@ __device__ __forceinline__ constexpr int token_of(int column) {
 // 128-byte swizzle: where 16-byte chunk c of row r of a [rows][128 bytes] tile lies.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// Largest finite magnitude of `count` numbers (an even number of them), by a warp; and whether one of them is an infinity or NaN.
+// Of `count` numbers (a multiple of eight, 16-byte aligned), by a warp: the largest finite magnitude, and the smallest of the eights' largest
+// that is not zero (infinite, if there is none).  Sets `odd` if one of them is an infinity or NaN.
 template <typename T>
-__device__ __forceinline__ float finite_top(const T* numbers, int count, int lane, bool& odd) {
-    float top = 0.0f;
+__device__ __forceinline__ float2 range_of(const T* numbers, int count, int lane, bool& odd) {
+    float top = 0.0f, least = INFINITY;
     bool strange = false;
-    for (int i = lane; i < count / 2; i += 32) {
-        const float2 f = widen2<T>(reinterpret_cast<const uint32_t*>(numbers)[i]);
-        const float a = fabsf(f.x), b = fabsf(f.y);
-        if (a <= 3.4028235e38f) top = fmaxf(top, a);
-        else strange = true;
-        if (b <= 3.4028235e38f) top = fmaxf(top, b);
-        else strange = true;
+#pragma unroll 2
+    for (int i = lane; i < count / 8; i += 32) {
+        const uint4 eight = reinterpret_cast<const uint4*>(numbers)[i];
+        const uint32_t words[4] = {eight.x, eight.y, eight.z, eight.w};
+        float most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = widen2<T>(words[e]);
+            const float a = fabsf(f.x), b = fabsf(f.y);
+            if (a <= 3.4028235e38f) most = fmaxf(most, a);
+            else strange = true;
+            if (b <= 3.4028235e38f) most = fmaxf(most, b);
+            else strange = true;
+        }
+        top = fmaxf(top, most);
+        if (most > 0.0f) least = fminf(least, most);
     }
     odd = __any_sync(0xffffffffu, strange);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    return top;
+    for (int o = 16; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+    }
+    return make_float2(top, least);
 }
+// Adds the block that is being filled, of BF16 numbers that lie far apart, to a row's results: all in FP32 from the numbers as they came, a
+// thread for its row, as the kernel for few rows does.  `top`, `level` and `sum` are the row's, its numbers lie in TMEM; by a whole warp.
+template <int D>
+__device__ __forceinline__ void add_tail(const __nv_bfloat16* q, const __nv_bfloat16* keys, const __nv_bfloat16* values, int seen, float scale,
+                                         unsigned out_at, float& top, float& level, float& sum) {
+    float scores[kKvBlock];
+    for (int t = 0; t < kKvBlock; ++t) scores[t] = 0.0f;
+    for (int d = 0; d < D; d += 8) {
+        float row[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) row[e] = seen > 0 ? __bfloat162float(q[d + e]) : 0.0f;
+        for (int t = 0; t < seen; ++t) {
+            const uint4 eight = *reinterpret_cast<const uint4*>(keys + t * D + d);
+            const uint32_t words[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 k = widen2<__nv_bfloat16>(words[e]);
+                scores[t] = fmaf(row[2 * e], k.x, fmaf(row[2 * e + 1], k.y, scores[t]));
+            }
+        }
+    }
+    float now = top;
+    for (int t = 0; t < seen; ++t) {
+        scores[t] = __fmul_rn(scores[t], scale);
+        now = fmaxf(now, scores[t]);
+    }
+    const float shrink = top > kNone ? exp2_fast(top - now) : 1.0f, factor = exp2_fast(level - kHeadroom) * kShrink * shrink;
+    sum *= shrink;
+    for (int t = 0; t < seen; ++t) {
+        scores[t] = exp2_fast(scores[t] - now);
+        sum += scores[t];
+    }
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+        uint32_t o[32];
+        tmem_load32(out_at + d, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+        for (int t = 0; t < seen; ++t) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const float v = __bfloat162float(values[t * D + d + e]);
+                // (infinities and NaN are added in the end)
+                if (fabsf(v) <= 3.4028235e38f) o[e] = __float_as_uint(fmaf(scores[t] * kShrink, v, __uint_as_float(o[e])));
+            }
+        }
+        tmem_store16(out_at + d, o);
+        tmem_store16(out_at + d + 16, o + 16);
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    static_assert(kShrink == 0x1p-32f);
+    top = now;
+    level = kHeadroom + 32.0f;                           // TMEM holds sums times kShrink
+}
+
+// The inverse of a power of two.
+__device__ __forceinline__ float inverse_power(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
@@ -293,12 +359,11 @@ kv_prefill_kernel(const PrefillParams p) {
     // Of a step's blocks, keys' and values', four steps: operands are made two steps ahead of the scores, and those of step n + 2 are
     // formed only when both tiles' probabilities of step n + 1 are there.
     // (Keys' scales; logarithms of the values' scales; and, for FP16, the inverses of what those are the logarithms of.)
-    __shared__ __align__(16) float scales[4][3][kStepBlocks];
-    __shared__ __align__(16) float4 tail_factors[kDequantWarps];      // keys': what makes FP16 of them, the scale of that; values': the same
-    // Whether the values of a step's block that is being filled have an infinity or NaN: by steps like the scales, written and read at the
-    // same places.  (By works it would be overwritten: works without a step are passed over at once, and one tile may be at the end
-    // of a work while the other is in the next but three.)
-    __shared__ bool odd_tail[4][kStepBlocks];
+    __shared__ __align__(16) float4 scales[4][kStepBlocks];
+    // What there is to note of a step's block that is being filled: by steps like the factors, written and read at the same places.  (By
+    // works it would be overwritten: works without a step are passed over at once, and one tile may be at the end of a work while the
+    // other is in the next but three.)
+    __shared__ uint8_t tail_notes[4][kStepBlocks];
     uint8_t* const shared = unaligned + (1024 - (smem_u32(unaligned) & 1023)) % 1024;
     pdl_wait_for_upstream();
     const int tid = threadIdx.x, lane = tid & 31;
@@ -343,7 +408,7 @@ kv_prefill_kernel(const PrefillParams p) {
     };
 
     if (warp < kSoftmaxWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PrefillRegisters<T, D>::kSoftmax));
         // ---------------------------------------------------------------- softmax: one row a thread
         const int t = warp / 4, row_in_tile = tid & (kRows - 1);
         const unsigned lanes = static_cast<unsigned>(warp % 4 * 32) << 16;
@@ -358,6 +423,7 @@ kv_prefill_kernel(const PrefillParams p) {
             const bool active = w.stop > w.begin && w.rows > w.first_row + t * kRows;      // this tile has rows, and they see something
             const bool has_tail = active && w.held > 0 && w.stop * kStepBlocks > w.full;
             const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (pair * 2 + (w.full & 1)) * kKvBlock * D;
+            const T* q_row = reinterpret_cast<const T*>(p.q) + w.b * p.q_batch + token * p.q_token + q_head * p.q_head;
             // What this row's weights, exp2(score) times the scale of the values, are relative to: the largest that it has seen (or a
             // little less).  FP16: `top` is that one's score and `level` the logarithm of its scale, and the sum is relative to it
             // too.  BF16, whose scales lie so far apart that weights which count for nothing can be those of the largest
@@ -365,26 +431,27 @@ kv_prefill_kernel(const PrefillParams p) {
             float top = kNone, level = 0.0f, sum = 0.0f, q_scale = p.scale;
             bool far = false;                            // a row of the warp has a maximum beyond kFar
             bool odd = false;                            // the tail's values have an infinity or NaN
+            bool apart = false;                          // its numbers lie far apart: it is added behind the steps
             if (active) {
                 // the row of queries: [half][row][128 bytes], dims in the order of the codes' bytes
                 uint8_t* const to = shared + t * Shape::kQueryBytes;
-                const T* from = reinterpret_cast<const T*>(p.q) + w.b * p.q_batch + token * p.q_token + q_head * p.q_head;
                 const uint32_t sign = p.negate ? 0x80008000u : 0u;
                 uint32_t raw[D / 2];
 #pragma unroll
                 for (int i = 0; i < D / 2; i += 4) {                     // (all of it requested together)
                     raw[i] = raw[i + 1] = raw[i + 2] = raw[i + 3] = 0;
                     if (row < w.rows && p.q_wide) {
-                        const uint4 four = *reinterpret_cast<const uint4*>(from + 2 * i);
+                        const uint4 four = *reinterpret_cast<const uint4*>(q_row + 2 * i);
                         raw[i] = four.x; raw[i + 1] = four.y; raw[i + 2] = four.z; raw[i + 3] = four.w;
                     } else if (row < w.rows) {
-                        const uint16_t* h = reinterpret_cast<const uint16_t*>(from + 2 * i);
+                        const uint16_t* h = reinterpret_cast<const uint16_t*>(q_row + 2 * i);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) raw[i + e] = h[2 * e] | static_cast<uint32_t>(h[2 * e + 1]) << 16;
                     }
                 }
                 if constexpr (kBf16) {
-                    // by a power of two of the row's own, so that no product is beyond FP32 that the definition has within
+                    // BF16 becomes FP16 by a power of two of the row's own: a number keeps all its bits unless it is 2^-26 of the
+                    // row's largest or less
                     uint32_t largest = 0;
 #pragma unroll
                     for (int i = 0; i < D / 2; ++i) largest = max(largest, max(raw[i] << 16 & 0x7fffffffu, raw[i] & 0x7fff0000u));
@@ -394,7 +461,7 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll
                     for (int i = 0; i < D / 2; ++i) {
                         const float2 f = widen2<T>(raw[i]);
-                        raw[i] = narrow2<T>(f.x * by, f.y * by);
+                        raw[i] = pack_half(f.x * by, f.y * by);
                     }
                 }
 #pragma unroll
@@ -416,24 +483,26 @@ kv_prefill_kernel(const PrefillParams p) {
                 arrive(bars.s_taken[t]);                 // the other tile's scores may come in their place
                 // Of each block: a score's factor, not negative, and the logarithm of its values' scale, which goes into the exponent (and out
                 // of the sum again; BF16: beside it).  Either may be NaN; a row that sees nothing of the block is kept out of that.
-                const float4 k_scale = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][0]);
-                const float4 v_log = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][1]);
-                const float4 v_inverse = *reinterpret_cast<const float4*>(scales[(steps_of_all + step - w.begin) & 3][2]);
-                if (has_tail && step + 1 == w.stop) odd = odd_tail[(steps_of_all + step - w.begin) & 3][w.full % kStepBlocks];
-                float by[kStepBlocks] = {k_scale.x, k_scale.y, k_scale.z, k_scale.w};
-                float value[kStepBlocks] = {v_log.x, v_log.y, v_log.z, v_log.w};
-                float inverse[kStepBlocks] = {v_inverse.x, v_inverse.y, v_inverse.z, v_inverse.w};
+                const float4* const of_blocks = scales[(steps_of_all + step - w.begin) & 3];
+                const unsigned notes = has_tail && step + 1 == w.stop ? tail_notes[(steps_of_all + step - w.begin) & 3][w.full % kStepBlocks] : 0u;
+                odd = (notes & kOddValues) != 0;
+                apart = kBf16 && (notes & kApart) != 0;
                 const bool masked = (step + 1) * kStepTokens - 1 > lowest;
-                const int last = place - step * kStepTokens;             // tokens of the step up to it are seen
-#pragma unroll
-                for (int block = 0; block < kStepBlocks; ++block) {
-                    by[block] *= q_scale;
-                    if (by[block] == 0.0f) by[block] = 0x1p-100f;
+                // Tokens of the step up to this one are seen.  (The step with the block that is being filled goes on behind the last token,
+                // so it is masked.)
+                const int last = (apart ? min(place, w.full * kKvBlock - 1) : place) - step * kStepTokens;
+                auto factors_of = [&](int block, float& by, float& value, float& inverse) {
+                    const float4 of = of_blocks[block];
+                    by = of.x * q_scale;
+                    value = of.y;
+                    inverse = of.z;
+                    if (by == 0.0f) by = 0x1p-100f;
                     if (masked && block * kKvBlock > last) {
-                        by[block] = inverse[block] = 1.0f;
-                        value[block] = 0.0f;
+                        by = 1.0f;
+                        value = 0.0f;
                     }
-                }
+                    if (far) by = 1.0f;
+                };
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < kStepTokens; ++i) {
@@ -449,9 +518,12 @@ kv_prefill_kernel(const PrefillParams p) {
 #pragma unroll 1
                 for (int attempt = 0; attempt < 2; ++attempt) {
                     if (anew) {
-                        float largest[kStepBlocks];
+                        float largest[kStepBlocks], value[kStepBlocks];
+                        far = false;
 #pragma unroll
                         for (int block = 0; block < kStepBlocks; ++block) {
+                            float by, inverse;
+                            factors_of(block, by, value[block], inverse);
                             const float* x = reinterpret_cast<const float*>(score + block * 32);
                             float two[2] = {max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5])};
 #pragma unroll
@@ -459,7 +531,7 @@ kv_prefill_kernel(const PrefillParams p) {
                                 two[0] = max3(two[0], x[i], x[i + 1]);
                                 two[1] = max3(two[1], x[i + 2], x[i + 3]);
                             }
-                            largest[block] = max3(max3(two[0], x[30], x[31]), two[1], two[1]) * by[block];
+                            largest[block] = max3(max3(two[0], x[30], x[31]), two[1], two[1]) * by;
                         }
                         float now = top, shrink = 1.0f;
                         if constexpr (kBf16) {
@@ -502,33 +574,40 @@ kv_prefill_kernel(const PrefillParams p) {
                         }
                         anew = false;
                         far = __any_sync(0xffffffffu, top > kNone && fabsf(top) > kFar);
-                    }
-                    float from = top > kNone ? top : 0.0f;      // (a row that has seen nothing yet: all it meets is masked)
-                    if (far) {
-                        // Product and difference in one rounding would leave the product's own, which for 10^12 is some 10^4: equal
-                        // scores would be beyond or below their maximum.  (The maximum is that of this step, so that there is no
-                        // second attempt.)
+                        if (far) {
+                            // Product and difference in one rounding would leave the product's own, which for 10^12 is some 10^4: equal
+                            // scores would be beyond or below their maximum.  (The maximum is that of this step, so that there is no
+                            // second attempt.)
+                            const float from = top > kNone ? top : 0.0f;
 #pragma unroll
-                        for (int i = 0; i < kStepTokens; ++i) {
-                            score[i] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(score[i]), by[i / kKvBlock]), -from));
+                            for (int block = 0; block < kStepBlocks; ++block) {
+                                float by, value, inverse;
+                                far = false;
+                                factors_of(block, by, value, inverse);
+                                far = true;
+#pragma unroll
+                                for (int i = 0; i < kKvBlock; ++i) {
+                                    score[block * kKvBlock + i] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(score[block * kKvBlock + i]), by), -from));
+                                }
+                            }
                         }
-#pragma unroll
-                        for (int block = 0; block < kStepBlocks; ++block) by[block] = 1.0f;
-                        from = 0.0f;
                     }
+                    const float from = !far && top > kNone ? top : 0.0f;      // (a row that has seen nothing yet: all it meets is masked)
                     step_sum = 0.0f;
                     float largest_sum = 0.0f;
 #pragma unroll
                     for (int block = 0; block < kStepBlocks; ++block) {
                         uint32_t packed[16];
-                        const float rise = value[block] - level + kHeadroom;
+                        float by, value, inverse;
+                        factors_of(block, by, value, inverse);
+                        const float rise = value - level + kHeadroom;
                         const float with = kBf16 ? -from : rise - from;
-                        const float factor = kBf16 ? exp2_fast(rise > 126.0f ? 126.0f : rise) : inverse[block];      // (NaN stays)
+                        const float factor = kBf16 ? exp2_fast(rise > 126.0f ? 126.0f : rise) : inverse;      // (NaN stays)
                         // Where results are FP16 the sum is of the weights as they were rounded, so that what a row's large ones were
                         // off by goes out of its result: root mean square 1.4 times the result's own rounding at most, where it was up to
                         // 1.6 (and 474 us, now 486).  Not of a block whose values are so small that its weights run out of bits.
                         const bool as_rounded = !kBf16 && rise >= kHeadroom - 4.0f;
-                        const uint64_t by2 = pair_of(by[block], by[block]), with2 = pair_of(with, with), factor2 = pair_of(factor, factor);
+                        const uint64_t by2 = pair_of(by, by), with2 = pair_of(with, with), factor2 = pair_of(factor, factor);
                         uint64_t sums[2] = {0, 0};
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
@@ -566,12 +645,18 @@ kv_prefill_kernel(const PrefillParams p) {
             float* part = p.parts + (static_cast<size_t>(blockIdx.x) * kUnitRows + t * kRows + row_in_tile) * (D + 4);
             const bool write = to_part ? active : row < p.tokens * p.group;
             T* out = reinterpret_cast<T*>(p.out) + ((static_cast<size_t>(w.b) * p.tokens + token) * p.q_heads + q_head) * D;
-            const float unit = kBf16 ? exp2_fast(level - kHeadroom) : 1.0f, by = to_part ? unit : sum > 0.0f ? unit / sum : sum;
-            const float shrink = kBf16 && to_part ? kShrink : 1.0f;
             if (active) {
                 wait(bars.o_done[t], steps_done - 1);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if constexpr (kBf16) {
+                    if (apart) {
+                        add_tail<D>(q_row, reinterpret_cast<const T*>(p.cache.k_tail) + (pair * 2 + (w.full & 1)) * kKvBlock * D, v_tail,
+                                    row < w.rows ? min(w.held, place - w.full * kKvBlock + 1) : 0, p.negate ? -p.scale : p.scale, out_at, top, level, sum);
+                    }
+                }
             }
+            const float unit = exp2_fast(level - kHeadroom), by = to_part ? unit : sum > 0.0f ? (kBf16 ? unit / sum : 1.0f / sum) : sum;
+            const float shrink = kBf16 && to_part ? kShrink : 1.0f;
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
                 uint32_t o[32];
@@ -600,11 +685,11 @@ kv_prefill_kernel(const PrefillParams p) {
                     }
                 }
             }
-            if (write && to_part) *reinterpret_cast<float4*>(part + D) = make_float4(top, kBf16 ? 0.0f : level, sum, 0.0f);
+            if (write && to_part) *reinterpret_cast<float2*>(part + D) = make_float2(top, kBf16 ? sum : sum * unit);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // (the next work's first arrival lets O be overwritten)
         }
     } else if (warp < kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDequantRegisters));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PrefillRegisters<T, D>::kDequant));
         // ---------------------------------------------------------------- operands: one block of a step a warp
         const int mine = warp - kSoftmaxWarps, g = lane >> 2, c = lane & 3;
         constexpr int kVectors = D / 16;                 // 16-byte pieces of a block's keys, and values, for a lane
@@ -620,7 +705,10 @@ kv_prefill_kernel(const PrefillParams p) {
         int steps = 0, read = 0;                         // steps of all, this CTA's works one after the other; blocks of codes
         Work w;
         bool asked = false;                              // whether the next step's codes were asked for
-        bool odd_values = false;                         // of the tail, where it is this warp's
+        // of the block that is being filled, where it is this warp's
+        unsigned notes = 0;
+        float k_by = 1.0f, v_by = 1.0f;                  // what its numbers are multiplied with
+        bool v_none = false;                             // all zeros: it counts for no more than a full block of zeros
         for (int n = 0; work_of(p, n, w); ++n) {
             if (w.stop <= w.begin) continue;
             const int pair = w.b * p.cache.kv_heads + w.head;
@@ -637,19 +725,23 @@ kv_prefill_kernel(const PrefillParams p) {
                 ask(1, pair, w.begin * kStepBlocks + mine);
             }
             if (w.held > 0 && w.full % kStepBlocks == mine && w.full / kStepBlocks >= w.begin && w.full / kStepBlocks < w.stop) {
-                // What the numbers of the block that is being filled are multiplied with, and the scale that stands for it.  FP16 keys
-                // stay as they are, BF16 ones stay BF16; values, which become FP16, are brought to the size of codes, so that weights
-                // keep as many bits beside small ones.  Values keep their bits down to 2^-23 of the block's largest (BF16 2^-26), and
-                // below 2^-34 of it count as zero.  (As codes they count as zero below 2^-8 of it; with more room for them weights
-                // would have less, 2^-18 of a row's largest instead of 2^-24.)
+                // What the numbers of the block that is being filled are multiplied with to become FP16, and what is to be noted.  FP16
+                // keys stay as they are; other numbers are brought to the size of codes, so that weights keep as many bits beside small
+                // ones.  They keep their bits down to 2^-23 of the block's largest (BF16 2^-26), and are off by 2^-34 of it below that.
+                // (As codes they count as zero below 2^-8 of it; with more room for them weights would have less.)  BF16 reaches further: where that is more than a 2^-22nd of eight keys' largest, or a 2^-17th
+                // of eight values', which takes one far out that a query may not even see, the block is left to add_tail().
                 const size_t tail = (static_cast<size_t>(pair) * 2 + (w.full & 1)) * kKvBlock * D;
-                float4 factors = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                if (kBf16) factors.x = power_for(finite_top(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane, odd_values), factors.y);
-                const float largest = finite_top(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane, odd_values);
-                factors.z = power_for(largest, factors.w);
-                if (largest == 0.0f) factors.w = 0.0f;       // (it counts for no more than a full block of zeros)
-                if (lane == 0) tail_factors[mine] = factors;
-                __syncwarp();
+                bool odd, unused;
+                float inverse;
+                const float2 values = range_of(reinterpret_cast<const T*>(p.cache.v_tail) + tail, w.held * D, lane, odd);
+                notes = odd ? kOddValues : 0u;
+                v_by = power_for(values.x, inverse);
+                v_none = values.x == 0.0f;
+                if constexpr (kBf16) {
+                    const float2 keys = range_of(reinterpret_cast<const T*>(p.cache.k_tail) + tail, w.held * D, lane, unused);
+                    k_by = power_for(keys.x, inverse);
+                    if (values.y < values.x * 0x1p-17f || keys.y < keys.x * 0x1p-12f) notes |= kApart;
+                }
             }
 #pragma unroll 1
             for (int step = w.begin; step < w.stop; ++step, ++steps) {
@@ -661,30 +753,20 @@ kv_prefill_kernel(const PrefillParams p) {
                 const int next_block = last ? after_block : block + kStepBlocks;
                 const T* k_tail = reinterpret_cast<const T*>(p.cache.k_tail) + (static_cast<size_t>(pair) * 2 + (block & 1)) * kKvBlock * D;
                 const T* v_tail = reinterpret_cast<const T*>(p.cache.v_tail) + (static_cast<size_t>(pair) * 2 + (block & 1)) * kKvBlock * D;
-                float k_scale = 0.0f, v_scale = 0.0f, k_by = 1.0f, v_by = 1.0f;
+                float k_scale = 0.0f, v_scale = 0.0f;
                 if (coded) {
                     k_scale = p.cache.k_scales[static_cast<size_t>(pair) * p.cache.blocks + block];
                     v_scale = p.cache.v_scales[static_cast<size_t>(pair) * p.cache.blocks + block];
                 } else if (tail) {
-                    const float4 factors = tail_factors[mine];
-                    k_by = factors.x;
-                    k_scale = factors.y;
-                    v_by = factors.z;
-                    v_scale = factors.w;
+                    k_scale = inverse_power(k_by);
+                    v_scale = v_none ? 0.0f : inverse_power(v_by);
+                    if (lane == 0) tail_notes[steps & 3][mine] = static_cast<uint8_t>(notes);
                 }
                 auto to_half = [&](uint32_t word, float by) {
                     const float2 f = widen2<T>(word);
                     return pack_half(f.x * by, f.y * by);
                 };
-                auto key_operand = [&](uint32_t word) {
-                    if (!kBf16) return word;
-                    const float2 f = widen2<T>(word);
-                    return narrow2<T>(f.x * k_by, f.y * k_by);
-                };
-                auto key_codes = [&](uint32_t word, uint32_t& even, uint32_t& odd) {
-                    if (kBf16) codes_to_bf16(word, even, odd);
-                    else codes_to_half(word, even, odd);
-                };
+                auto key_to_half = [&](uint32_t word) { return kBf16 ? to_half(word, k_by) : word; };
                 // keys: row of a token, in the order of the columns (token_of)
                 if (coded) wait(bars.codes[mine][0], read);
                 if (steps >= 2) wait(bars.k_empty[stage], steps / 2 - 1);
@@ -702,10 +784,10 @@ kv_prefill_kernel(const PrefillParams p) {
                         for (int i = 0; i < kVectors; ++i) {
                             const uint4 four = *reinterpret_cast<const uint4*>(codes + i * 512 + lane * 16);
                             uint32_t words[8];
-                            key_codes(four.x, words[0], words[1]);
-                            key_codes(four.y, words[2], words[3]);
-                            key_codes(four.z, words[4], words[5]);
-                            key_codes(four.w, words[6], words[7]);
+                            codes_to_half(four.x, words[0], words[1]);
+                            codes_to_half(four.y, words[2], words[3]);
+                            codes_to_half(four.z, words[4], words[5]);
+                            codes_to_half(four.w, words[6], words[7]);
                             store(i, words);
                         }
                     } else {
@@ -717,7 +799,7 @@ kv_prefill_kernel(const PrefillParams p) {
                                 const uint32_t* raw = reinterpret_cast<const uint32_t*>(k_tail + token * D + i % kHalves * 64 + c * 16);
 #pragma unroll
                                 for (int e = 0; e < 8; e += 2) {
-                                    const uint32_t lo = key_operand(raw[e]), hi = key_operand(raw[e + 1]);
+                                    const uint32_t lo = key_to_half(raw[e]), hi = key_to_half(raw[e + 1]);
                                     words[e] = prmt(lo, hi, 0x5410);
                                     words[e + 1] = prmt(lo, hi, 0x7632);
                                 }
@@ -727,11 +809,8 @@ kv_prefill_kernel(const PrefillParams p) {
                     }
                 }
                 if (lane == 0) {
-                    scales[steps & 3][0][mine] = k_scale;
                     const float v_log = !kBf16 && v_scale < 0x1p-40f ? kLightestHalf : __log2f(v_scale);
-                    scales[steps & 3][1][mine] = v_log;
-                    if (!kBf16) scales[steps & 3][2][mine] = exp2_fast(-v_log);
-                    if (tail) odd_tail[steps & 3][mine] = odd_values;
+                    scales[steps & 3][mine] = make_float4(k_scale, v_log, v_scale != v_scale ? 0.0f : exp2_fast(-v_log), 0.0f);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive(bars.k_full[stage]);
@@ -792,11 +871,10 @@ kv_prefill_kernel(const PrefillParams p) {
             for (int which = 0; which < 2; ++which) mbar_wait<false, true>(smem_u32(&bars.codes[mine][which]), read & 1, kKvGaveUp, p.cache.status);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssuerRegisters));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PrefillRegisters<T, D>::kIssuer));
         // ---------------------------------------------------------------- MMAs
         constexpr uint32_t kCommon = (1u << 4) | (static_cast<uint32_t>(kRows >> 4) << 24);      // FP32 sums of FP16, 128 rows, K-major
-        constexpr uint32_t kOfBf16 = kBf16 ? (1u << 7) | (1u << 10) : 0u;                        // both operands
-        constexpr uint32_t kScoreDesc = kCommon | kOfBf16 | (static_cast<uint32_t>(kStepTokens >> 3) << 17);
+        constexpr uint32_t kScoreDesc = kCommon | (static_cast<uint32_t>(kStepTokens >> 3) << 17);
         constexpr uint32_t kOutputDesc = kCommon | (static_cast<uint32_t>(D >> 3) << 17);
         const bool chosen = elect_one();
         int steps = 0, works[2] = {0, 0};                // steps of all, up to this work; works of each tile
@@ -885,43 +963,36 @@ kv_pieces_kernel(const PrefillParams p) {
     const int row = first.first_row + in_unit;
     if (row >= p.tokens * p.group) return;
     constexpr int kDims = D / 32;
-    float top = kNone, level = 0.0f, weight = 0.0f, acc[kDims];
+    float top = kNone, weight = 0.0f, acc[kDims];
 #pragma unroll
     for (int d = 0; d < kDims; ++d) acc[d] = 0.0f;
     if (row < first.rows) {
         for (int begin = 0; begin < p.pieces; begin += BATCH) {
-            float4 state[BATCH];                          // what its numbers are relative to, and its sum
-            float2 numbers[BATCH][kDims / 2];
-            float best = top, of_best = level;
+            float2 state[BATCH], numbers[BATCH][kDims / 2];
+            float best = top;
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
                 const int piece = begin + e;
                 const bool some = piece < p.pieces && static_cast<long long>(first.stop) * piece / p.pieces <
                                                           static_cast<long long>(first.stop) * (piece + 1) / p.pieces;
                 const float* part = p.parts + (static_cast<size_t>(unit * p.pieces + piece) * kUnitRows + in_unit) * (D + 4);
-                state[e] = some ? *reinterpret_cast<const float4*>(part + D) : make_float4(kNone, 0.0f, 0.0f, 0.0f);
+                state[e] = some ? *reinterpret_cast<const float2*>(part + D) : make_float2(kNone, 0.0f);
 #pragma unroll
                 for (int d = 0; d < kDims / 2; ++d) {
                     numbers[e][d] = some ? reinterpret_cast<const float2*>(part + lane * kDims)[d] : make_float2(0.0f, 0.0f);
                 }
             }
 #pragma unroll
-            for (int e = 0; e < BATCH; ++e) {
-                if (state[e].x - best + (state[e].y - of_best) > 0.0f) {
-                    best = state[e].x;
-                    of_best = state[e].y;
-                }
-            }
-            const float mine = exp2_fast(top - best + (level - of_best));
+            for (int e = 0; e < BATCH; ++e) best = fmaxf(best, state[e].x);
+            const float mine = exp2_fast(top - best);
             top = best;
-            level = of_best;
             weight *= mine;
 #pragma unroll
             for (int d = 0; d < kDims; ++d) acc[d] *= mine;
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
-                const float theirs = exp2_fast(state[e].x - best + (state[e].y - of_best));
-                weight = fmaf(state[e].z, theirs, weight);
+                const float theirs = exp2_fast(state[e].x - best);
+                weight = fmaf(state[e].y, theirs, weight);
 #pragma unroll
                 for (int d = 0; d < kDims / 2; ++d) {
                     acc[2 * d] = fmaf(numbers[e][d].x, theirs, acc[2 * d]);

@@ -117,11 +117,12 @@ def _block_tops(v, length):
 
 def _check_seen(cache, k, v, q, length, scale):
     """Attention against its definition, within what the tokens that a query sees allow: a weight (probability times its values' scale)
-    is held in FP16 times 2^10 relative to the largest one seen, M / 127 at most with M the largest p x (largest of the token's block).
-    What is below FP16's normal numbers is off by half a step, 2^-25: times a code of 127 at most that is 2^-35 of M for each token;
-    times a number of the block being filled, held up to 2^10, 2^-25 x 2^-10 x 2^10 / 127 < 2^-31 of it, 31 of them 2^-26; and such a number
-    itself is off by 2^-34 of the block's largest (2^-25 of 2^9), which a query may not see, times its probability.  A sum of rounded
-    weights is off by 2^-31 of itself for each of them at most (their scale is 2^-4 of the largest's or more).  The rest is
+    is held in FP16 times 2^9 (or 2^10) relative to the largest one seen, M / 127 at most with M the largest p x (largest of the token's
+    block).  What is below FP16's normal numbers is off by half a step, 2^-25: times a code of 127 at most that is 2^-34 of M for each
+    token; times a number of the block being filled, held up to 2^10, 2^-25 x 2^-9 x 2^10 / 127 < 2^-30 of it, 31 of them 2^-25; and such a number
+    itself is off by 2^-34 of the block's largest, or (BF16, where those lie further apart it is taken as it is) by 2^-17 of its eight's
+    largest at most, times its probability.  A sum of rounded
+    weights is off by 2^-30 of itself for each of them at most (their scale is 2^-4 of the largest's or more).  The rest is
     kv_oracle.attention_bound's."""
     got = cache.attention(q, _words([length]), softmax_scale=scale)[0].double()
     tokens, q_heads, _ = q.shape[1:]
@@ -136,10 +137,14 @@ def _check_seen(cache, k, v, q, length, scale):
         p = torch.softmax(scores.masked_fill(hidden[:, None, :], float("-inf")), -1)
         most = (p * tops[:, head]).amax(-1, keepdim=True)
         bound = oracle.attention_bound(want[:, rows], weight[:, rows], q.dtype, 0.0)
-        bound = bound + most * (length * 2.0 ** -35 + 2.0 ** -26) + want[:, rows].abs() * length * 2.0 ** -31
+        bound = bound + most * (length * 2.0 ** -34 + 2.0 ** -25) + want[:, rows].abs() * length * 2.0 ** -30
         full = length // 32 * 32
         if full < length:
-            bound = bound + p[..., full:].sum(-1, keepdim=True) * float(v[0, full:length, head].abs().max()) * 2.0 ** -34
+            tails = v[0, full:length, head].double().abs()
+            if q.dtype == torch.float16:
+                bound = bound + p[..., full:].sum(-1, keepdim=True) * float(tails.max()) * 2.0 ** -34
+            else:
+                bound = bound + (p[..., full:] @ tails.unflatten(-1, (-1, 8)).amax(-1).repeat_interleave(8, -1)) * 2.0 ** -17
         off = (got[:, rows] - want[:, rows]).abs()
         assert (off <= bound).all(), (head, float((off / bound).max()))
     cache.check()
@@ -427,3 +432,54 @@ def test_a_cache_far_larger_than_what_it_holds(tokens, q_heads, kv_heads, head_d
         for _ in range(3):
             assert torch.equal(cache.attention(q, _words(lengths)), first)
         cache.check()
+
+
+@pytest.mark.parametrize("length", [50, 90, 95, 33])
+@pytest.mark.parametrize(("tokens", "q_heads", "kv_heads", "head_dim"), [(1, 8, 2, 64), (5, 8, 2, 128), (24, 32, 2, 64), (24, 32, 2, 128)])
+@pytest.mark.parametrize("dims", [slice(None), slice(8, 24)])
+@pytest.mark.parametrize(("k_size", "v_size"), [(1.0, 1e12), (1.0, 3e38), (1e30, 1.0), (1e20, 1e38), (1e-30, 1e-30), (1.0, 1e4)])
+def test_tokens_far_out_in_the_block_being_filled(k_size, v_size, dims, tokens, q_heads, kv_heads, head_dim, length):
+    """BF16, a token some or all of whose key or value is as large (or small) as the type has them, the last but two: in front of it nothing changes, and for
+    those that see it it counts as the definition says."""
+    k, v = (_draw((1, length, kv_heads, head_dim), torch.bfloat16, seed) for seed in (45, 46))
+    top = torch.finfo(torch.bfloat16).max
+    for x, size in ((k, k_size), (v, v_size)):
+        x[:, length - 3, :, dims] = (x[:, length - 3, :, dims].float() * size).clamp(-top, top).to(torch.bfloat16)
+    cache = QuantizedKVCache(1, kv_heads, length + 3, head_dim, dtype=torch.bfloat16)
+    cache.append(k, v, _words([0]))
+    _check_seen(cache, k, v, _draw((1, tokens, q_heads, head_dim), torch.bfloat16, 47), length, head_dim ** -0.5)
+
+
+def test_what_later_tokens_are_does_not_matter_to_a_chunk():
+    """The same result, to a rounding, for queries in front of them, BF16, whatever the keys and values behind are."""
+    for head_dim, length in ((64, 60), (128, 91)):
+        k, v = (_draw((1, length, 2, head_dim), torch.bfloat16, seed) for seed in (48, 49))
+        q = _draw((1, 24, 32, head_dim), torch.bfloat16, 50)
+        outs = []
+        for size in (1.0, 0.0, 1e6, -1e30, 3e38):
+            dirty_k, dirty_v = k.clone(), v.clone()
+            for x in (dirty_k, dirty_v):
+                x[:, length - 2:] = size
+            cache = QuantizedKVCache(1, 2, length, head_dim, dtype=torch.bfloat16)
+            cache.append(dirty_k, dirty_v, _words([0]))
+            got = cache.attention(q, _words([length]))
+            assert got[:, :22].isfinite().all()
+            outs.append(got[:, :22])
+        for out in outs[1:]:
+            # (powers of two alone differ; exponents that they are added to are rounded in FP32, 2^-20 of a weight, and then to FP16)
+            assert ((out.double() - outs[0].double()).abs() <= 2.0 ** -7 * outs[0].double().abs() + 2.0 ** -9).all()
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("scale", [0.125, -0.125, 0.0])
+@pytest.mark.parametrize("large", [60000.0, 300.0, 1.0])
+def test_small_values_beside_large_ones_in_the_block_being_filled(large, scale, strided):
+    """FP16, values 2^14 apart and more, seen and not, by many queries, in whole units and in pieces of one, of either sign of the scale."""
+    for length, tokens, q_heads in ((60, 24, 16), (4000 + 31, 24, 16), (1000 + 15, 150, 16)):
+        k, v = _draw((1, length, 1, 64), torch.float16, 51), _draw((1, length, 1, 64), torch.float16, 52, 0.002)
+        v[:, length - 9] *= large / 0.002 / 4
+        v[:, length - 2, :, 8:16] *= large / 0.002 / 4
+        cache = QuantizedKVCache(1, 1, length + 40, 64)
+        cache.append(k, v, _words([0]))
+        q = _draw((1, tokens, q_heads, 64 + strided), torch.float16, 53)[..., :64]
+        _check_seen(cache, k, v, q, length, scale)
