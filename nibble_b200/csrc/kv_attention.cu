@@ -45,7 +45,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMinRun = 4;                      // blocks that are worth a CTA: one a warp (500 tokens 6.9 us; with eight 8.0)
 constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
-// (weights are held in FP16 times 2^kHeadroom)
+constexpr float kHeadroom = 10.0f;              // weights are held in FP16 times 2^10,
 constexpr float kMaxLag = 3.0f;                 // times 2^3 where the maximum has not been followed yet,
 constexpr float kMaxRise = 2.0f;                // times 2^2 where the values' scale has not: below 65504 in all
 

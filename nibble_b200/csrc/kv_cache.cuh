@@ -30,7 +30,6 @@ constexpr int kKvBlock = 32;           // tokens that share a scale
 constexpr unsigned kKvBadLength = 1;   // status: a length or count outside the cache
 constexpr unsigned kKvGaveUp = 2;      // status: a bounded wait ran out
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHeadroom = 10.0f;           // weights of attention's second product, exp2(score) times the values' scale, are held in FP16 times 2^10
 constexpr float kLightest = -100.0f;         // values' scales below 2^-100 count as that where weights are compared
 constexpr float kShrink = 0x1p-32f;      // BF16: sums of values over tokens are held times this, so that those of its largest are finite
 constexpr float kNone = -3.4028235e38f;      // the maximum of nothing: no score is below it but minus infinity
