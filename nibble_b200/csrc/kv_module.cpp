@@ -133,6 +133,14 @@ bool reachable(const int64_t (&sizes)[4], const int64_t (&strides)[4], int dim, 
     return false;
 }
 
+// Whether two tensors of the same sizes go from number to number by the same strides (those of dimensions with one entry say nothing).
+bool same_strides(const at::Tensor& a, const at::Tensor& b) {
+    for (int64_t d = 0; d < a.dim(); ++d) {
+        if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+    }
+    return true;
+}
+
 // Whether two tensors of the same sizes (four dimensions at most) and 16-bit type may share memory: by their extents, and where those
 // meet and the strides are the same, as of two parts of a fused row, exactly.
 bool may_share(const at::Tensor& a, const at::Tensor& b) {
@@ -144,7 +152,7 @@ bool may_share(const at::Tensor& a, const at::Tensor& b) {
     };
     const auto begin_a = reinterpret_cast<uintptr_t>(a.const_data_ptr()), begin_b = reinterpret_cast<uintptr_t>(b.const_data_ptr());
     if (past(a) <= begin_b || past(b) <= begin_a) return false;
-    if (a.strides() != b.strides() || (begin_a - begin_b) % 2 != 0) return true;
+    if (!same_strides(a, b) || (begin_a - begin_b) % 2 != 0) return true;
     int64_t sizes[4] = {1, 1, 1, 1}, strides[4] = {0, 0, 0, 0};
     int order[4] = {0, 1, 2, 3};
     std::sort(order, order + a.dim(), [&](int x, int y) { return a.stride(x) > a.stride(y); });
@@ -176,12 +184,13 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
     const w4a16_rotary_spec spec = spec_of(inv_freq, x.device(), x.size(-1), scale, interleaved);
     const c10::cuda::CUDAGuard guard(x.device());
     at::Tensor out;
+    bool in_place = false;
     if (given.has_value()) {
         out = *given;
         TORCH_CHECK(out.device() == x.device() && out.scalar_type() == x.scalar_type(), "out must be on the device of x and of its dtype");
         TORCH_CHECK(out.sizes() == x.sizes(), "out must have the shape of x");
         at::assert_no_internal_overlap(out);
-        const bool in_place = out.data_ptr() == x.data_ptr() && out.strides() == x.strides();
+        in_place = out.data_ptr() == x.data_ptr() && same_strides(out, x);
         TORCH_CHECK(in_place || !may_share(out, x), "out must be x itself or share no memory with it");
     } else {
         out = at::detail::empty_cuda(x.sizes(), x.scalar_type(), x.device(), c10::nullopt);
@@ -194,7 +203,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t count) {
         auto stride = [&](int64_t dim) { return dim < missing ? 0 : t.stride(dim - missing); };
         return w4a16_rows{t.data_ptr(), stride(0), stride(1), stride(2)};
     };
-    const w4a16_rows from = rows(x), to = rows(out);
+    const w4a16_rows from = rows(x), to = in_place ? from : rows(out);
     const int64_t* at_positions = words_of(positions, x.device(), size(0) * size(1), "positions");
     if (x.numel() > 0) {
         pybind11::gil_scoped_release unlocked;

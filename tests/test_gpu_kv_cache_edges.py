@@ -336,6 +336,13 @@ def test_turned_into_another_place():
     apply_rotary(one[0:16:2], _words(7), inv_freq, out=one[1:17:2])                # every other head into its neighbour
     assert torch.equal(one[0:16:2], kept[0:16:2]) and torch.equal(one[17:], kept[17:])
     assert torch.equal(one[1:17:2], apply_rotary(kept[0:16:2], _words(7), inv_freq))
+    single = _draw((1, 2, 6 * d), torch.float16, 54)                               # dimensions with one entry, whose strides say nothing
+    spaced = single.as_strided((1, 2, 3, d), (999, 6 * d, d, 1))
+    want = apply_rotary(spaced.contiguous(), places[:1, :2].contiguous(), inv_freq)
+    apply_rotary(spaced, places[:1, :2].contiguous(), inv_freq, out=single.as_strided((1, 2, 3, d), (7, 6 * d, d, 1), 3 * d))
+    assert torch.equal(single[..., 3 * d:].unflatten(-1, (3, d)), want)
+    apply_rotary(spaced, places[:1, :2].contiguous(), inv_freq, out=single.as_strided((1, 2, 3, d), (7, 6 * d, d, 1)))
+    assert torch.equal(spaced, want)
     kept = row.clone()
     for into in (row[..., d:7 * d].unflatten(-1, (6, d)), row[..., 1:6 * d + 1].unflatten(-1, (6, d)), row[..., 5 * d:11 * d].unflatten(-1, (6, d)),
                  row[..., :12 * d].unflatten(-1, (6, 2 * d))[..., :d], row.view(-1).as_strided((2, 3, 6, d), (3 * 20 * d, 20 * d, d, 1), 8),
