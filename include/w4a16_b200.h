@@ -312,11 +312,11 @@ int w4a16_attention_decode_f16(const void* qkv, void* k_cache, void* v_cache, vo
  * So what it holds depends on the tokens alone, not on how many came at a time, and each number is rounded once.  A block with an
  * infinity or NaN gets the scale NaN and reads back as NaN.  The number of tokens held is the caller's to keep (device words, so
  * that a captured graph serves every step); it may be set back, as after refused drafts, to as far as the beginning of the block
- * before the newest one that was reached.
+ * before that of the furthest token that was written.
  *
  * Sizes: head_dim 64 or 128, any max_len >= 1.  `type` says what the numbers outside of the codes are.  Every device word that
- * names a length, start or count outside its range makes the kernel leave that sequence alone (its outputs are zeros), and sets bit 0
- * of *status; bit 1 says that a bounded wait ran out, and that outputs are incomplete.
+ * names a length, start or count outside its range makes the kernel leave that sequence alone (its outputs are zeros, but for queries that
+ * w4a16_kv8_append turns), and sets bit 0 of *status; bit 1 says that a bounded wait ran out, and that outputs are incomplete.
  */
 enum { W4A16_TYPE_F16 = 0, W4A16_TYPE_BF16 = 1 };
 
@@ -366,7 +366,7 @@ int w4a16_kv8_append(const w4a16_kv8_cache* cache, const w4a16_rows* k, const w4
                      const int64_t* counts, const w4a16_rotary_spec* rotary, const w4a16_rows* q, const w4a16_rows* q_out,
                      int32_t q_heads, uint32_t flags, w4a16_stream_t stream);
 
-/* The values held at positions first[b] (NULL: 0) .. first[b] + tokens - 1 of sequences of lengths[b] tokens, zeros behind the
+/* The values held at positions first[b] (0 to max_len; NULL: 0) .. first[b] + tokens - 1 of sequences of lengths[b] tokens, zeros behind the
  * last: k_out, v_out [batch][tokens][kv_heads][head_dim] of the cache's type. */
 int w4a16_kv8_read(const w4a16_kv8_cache* cache, const int64_t* lengths, const int64_t* first, int64_t tokens, void* k_out,
                    void* v_out, uint32_t flags, w4a16_stream_t stream);

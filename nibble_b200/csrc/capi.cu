@@ -574,14 +574,15 @@ static bool fits_queries(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t 
 // once for all of them, or to that with tiles of up to 32 rows (64 at D = 64), where each warp does so for its own and equal runs take
 // ragged lengths evenly.  Measured with FP16, smaller tiles and larger, us (smaller ones have no variant for more than 32 rows at D = 128;
 // one of 64 took 109 instead of 79 for 40 rows of 8 sequences of 8000):
-//     D = 128, 64 heads on 8    8 sequences of 8000:  32 rows 69, 79
+//     D = 128, 64 heads on 8    8 sequences of 8000:  32 rows 69, 78
 //                               1 sequence of 8000:   32 rows 23, 27
-//                               64 sequences of 1000: 24 rows 94, 103; 32 rows 101, 102
-//     D = 64, 32 heads on 4     8 sequences of 8000:  32 rows 28, 40; 64 rows 42, 41; 72 rows 81, 41
-//                               1 sequence of 8000:   64 rows 17, 23; 72 rows 23, 23
-//                               8 ragged up to 2900:  40 rows 19, 24 (BF16)
-//                               32 sequences of 1000: 32 rows 25, 22; 40 rows 34, 22
-//                               64 sequences of 1000: 32 rows 39, 42; 40 rows 56, 42; 64 rows 66, 42
+//                               64 sequences of 1000: 24 rows 94, 98; 32 rows 100, 97
+//     D = 64, 32 heads on 4     8 sequences of 8000:  32 rows 28, 40; 40 rows 43, 40; 64 rows 44, 40; 72 rows 81, 40
+//                               1 sequence of 8000:   40 rows 15, 22; 64 rows 16, 24; 72 rows 23, 24
+//                               8 ragged up to 2900:  40 rows 22, 24 (BF16)
+//                               18 sequences of 1000: 40 rows 24, 21; 64 rows 27, 22
+//                               32 sequences of 1000: 32 rows 24, 21; 40 rows 34, 21
+//                               64 sequences of 1000: 32 rows 40, 41; 40 rows 58, 41; 64 rows 67, 41
 // So from 33 rows on with D = 128, and with D = 64 where there are sequences and heads enough that none has to be cut along its tokens.
 static bool many_queries(const w4a16_kv8_cache* cache, int32_t q_heads, int64_t tokens) {
     const int64_t rows = tokens * (q_heads / cache->kv_heads), pairs = static_cast<int64_t>(cache->batch) * cache->kv_heads;

@@ -19,10 +19,10 @@
 // run has of a sequence and head goes to the workspace, and a second kernel, which starts beside the first, adds those parts up in
 // order and attends over the block that is being filled.
 //
-// Measured (64 query heads on 8, D = 128, in a graph): one token over 65501 29.7 us = 4.5 TB/s, of a measured 6.5 for a copy, of which
+// Measured (64 query heads on 8, D = 128, in a graph): one token over 65501 29.9 us = 4.5 TB/s, of a measured 6.5 for a copy, of which
 // 5 us go by before the first block has arrived and 4 after the last; 48 sequences of up to 8192 tokens 73.0 us = 5.5 TB/s.  Short
-// contexts are latency: 500 tokens of 32 heads on 4, D = 64, 6.9 us, of which two kernels that do nothing would take 4.7.  (A warp that
-// went over a block that is not there while the first lengths are on their way, to have the loop's code at hand, made them 8.0.)
+// contexts are latency: 500 tokens of 32 heads on 4, D = 64, 6.7 us, of which two kernels that do nothing would take 4.7.  (A warp that
+// went over a block that is not there while the first lengths are on their way, to have the loop's code at hand, made 6.9 of it 8.0.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -43,7 +43,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMinRun = 4;                      // blocks that are worth a CTA: one a warp (500 tokens 6.9 us; with eight 8.0)
+constexpr int kMinRun = 4;                      // blocks that are worth a CTA: one a warp (500 tokens took 6.9 us, with eight 8.0)
 constexpr int kUnitCost = 8;                    // what starting and ending a sequence, head and tile costs, in blocks
 constexpr float kHeadroom = 10.0f;              // weights are held in FP16 times 2^10,
 constexpr float kMaxLag = 3.0f;                 // times 2^3 where the maximum has not been followed yet,

@@ -7,8 +7,8 @@
 // and the block that is being filled is held as it came, in 16 bits (the tail).  So a number is rounded once, with the scale of
 // the block it ends up in, and what the cache holds depends on the tokens alone, not on how many came at a time.  (With a scale
 // that grows as tokens arrive, codes already written would be rounded again at every growth.)  The tail has two slots, for
-// blocks of even and of odd index, so that the block before the newest can still be taken back to: the length may fall by up to
-// a block's worth of tokens, as it does when drafted tokens are refused.
+// blocks of even and of odd index, which hold the last token's block and the one before it: the length may fall to the beginning of
+// that, as it does when drafted tokens are refused.
 //
 // A full block lies in the order in which attention's matrix instructions take it, so that a warp's 16-byte reads are
 // contiguous and nothing has to be transposed there:

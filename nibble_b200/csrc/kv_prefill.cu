@@ -17,7 +17,7 @@
 //
 // The tiles share the columns of the scores: a softmax thread takes its row's into registers in one go, and the MMAs of the other
 // tile's scores, which that will want half a round later, follow in their place.  So neither softmax waits for its scores.
-// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 486 us: 0.99 PFLOP/s, of a measured 1.63 for a plain product.
+// 2048 queries of 64 heads on 8 at the end of 8192 tokens, D = 128, take 484 us: 0.99 PFLOP/s, of a measured 1.63 for a plain product.
 // What it was before: 592 with columns for each tile and the probabilities in the scores' place, where a tile's next scores had to
 // wait for its last output, and its softmax for both; 670 with 64 tokens at a time, twice buffered, since MMAs of 64 columns read
 // twice as much shared memory a column; 505 with the maximum of every block sought before its probabilities.  Bounds: on paper MMAs
@@ -605,7 +605,7 @@ kv_prefill_kernel(const PrefillParams p) {
                         const float factor = kBf16 ? exp2_fast(rise > 126.0f ? 126.0f : rise) : inverse;      // (NaN stays)
                         // Where results are FP16 the sum is of the weights as they were rounded, so that what a row's large ones were
                         // off by goes out of its result: root mean square 1.4 times the result's own rounding at most, where it was up to
-                        // 1.6 (and 474 us, now 486).  Not of a block whose values are so small that its weights run out of bits.
+                        // 1.6 (2048 queries at 8192 take 12 us longer for it).  Not of a block whose values are so small that its weights run out of bits.
                         const bool as_rounded = !kBf16 && rise >= kHeadroom - 4.0f;
                         const uint64_t by2 = pair_of(by, by), with2 = pair_of(with, with), factor2 = pair_of(factor, factor);
                         uint64_t sums[2] = {0, 0};

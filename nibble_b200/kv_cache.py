@@ -8,8 +8,9 @@ scale for its keys and one for its values (``scale = max|x| / 127``, ``code = ro
 is being filled is held as it came.  So what the cache holds depends on the tokens alone, not on how many came at a time, and
 each number is rounded once.  A block with an infinity or NaN in it reads back as NaN.
 
-Lengths, starts and counts are int64 tensors on the device, so that a captured CUDA graph serves every step; one that does not fit
-the cache leaves that sequence alone (its outputs are zeros) and is reported by ``check()``.  None of these operators forms
+Lengths, starts and counts are contiguous int64 tensors on the device, so that a captured CUDA graph serves every step; one that does not
+fit the cache leaves that sequence alone (its outputs are zeros, but for queries that ``append`` turns, which are turned all the same) and is
+reported by ``check()``.  None of these operators forms
 gradients: an input that requires one, or carries a forward-mode tangent, is refused.  All of them run on the current stream of the tensors' device.
 """
 from __future__ import annotations
@@ -40,8 +41,9 @@ def apply_rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tenso
     Pair ``j`` of a head at position ``p`` is turned by the angle ``p * inv_freq[j]``; pairs are ``(2j, 2j + 1)`` if
     ``interleaved``, else ``(j, j + rotary_dim / 2)``, with ``rotary_dim = 2 * inv_freq.numel()``; the head's numbers from
     ``rotary_dim`` on stay as they are.  Cosines and sines are multiplied by ``scale``.  Ways of stretching a context are a matter
-    of ``inv_freq`` (FP32) and ``scale``.  Angles are formed in FP64, the rest in FP32, rounded once.  ``positions`` (int64) has the
-    shape of ``x`` without its last two dimensions.  ``out`` may be ``x`` itself, or a tensor that shares no memory with it.
+    of ``inv_freq`` (FP32) and ``scale``.  Angles are formed in FP64, the rest in FP32, rounded once.  ``positions`` (int64, contiguous)
+    has the shape of ``x`` without its last two dimensions.  ``out`` may be ``x`` itself, or a tensor of its shape, with any strides, that
+    shares no memory with it; of one buffer, two parts of the same rows or parts whose extents are apart.  It counts as changed in place.
     """
     return _extension().rotary(x, positions, inv_freq, scale, interleaved, out)
 
@@ -51,7 +53,7 @@ class QuantizedKVCache:
     ``head_dim`` (64 or 128) numbers, which come and are read back as ``dtype`` (FP16 or BF16).
 
     The cache does not count its tokens: every call says how many there are.  The length may be set back, as after refused
-    drafts, as far as the beginning of the block before the newest that was reached; the next ``append`` writes from there.
+    drafts, as far as the beginning of the block before that of the furthest token that was written; the next ``append`` writes from there.
     """
 
     BLOCK = 32          # tokens that share a scale
@@ -81,14 +83,14 @@ class QuantizedKVCache:
         positions ``start[b], start[b] + 1, ...``; of sequence ``b`` the first ``counts[b]`` (default: all).
 
         With ``inv_freq`` the keys are turned to their positions on the way, and so are the queries ``q`` ``[batch, tokens, q_heads,
-        head_dim]``, which are returned: the same bits as ``apply_rotary`` in front, for a few tokens in one launch.
+        head_dim]``, all ``tokens`` of them, which are returned: the same bits as ``apply_rotary`` in front, for a few tokens in one launch.
         """
         return _extension().kv8_append(self.memory, *self._sizes, k, v, start, counts, inv_freq, rope_scale, interleaved, q)
 
     def read(self, lengths: torch.Tensor, first: torch.Tensor | None = None,
              tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """What the cache holds: keys and values ``[batch, tokens, kv_heads, head_dim]`` from position ``first[b]`` (default: 0)
-        on, of sequences of ``lengths[b]`` tokens; zeros behind the last.  ``tokens`` defaults to ``max_len``."""
+        on (up to ``max_len``), of sequences of ``lengths[b]`` tokens; zeros behind the last.  ``tokens`` defaults to ``max_len``."""
         return _extension().kv8_read(self.memory, *self._sizes, lengths, first, self.max_len if tokens is None else tokens)
 
     def attention(self, q: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None,
@@ -98,7 +100,8 @@ class QuantizedKVCache:
         ``lengths[b]`` counts the newest tokens too; query ``i`` of ``counts[b]`` (default: all of ``tokens``) stands at position
         ``lengths[b] - counts[b] + i`` and sees the positions up to its own.  Query heads are a multiple of the cache's, consecutive
         ones sharing a head.  ``softmax_scale`` defaults to ``head_dim ** -0.5``.  Rows behind a sequence's last query, and
-        rows that see nothing, are zeros.
+        rows that see nothing, are zeros.  Scores, sums and results are FP32, probabilities times their values' scale FP16 relative to the
+        largest of them that a row sees.
         """
         return _extension().kv8_attention(self.memory, *self._sizes, q, lengths, counts,
                                           self.head_dim ** -0.5 if softmax_scale is None else softmax_scale)
