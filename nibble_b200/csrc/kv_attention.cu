@@ -4,14 +4,14 @@
 //     out = sum_t p_t v_t / sum_t p_t,   p_t = exp(softmax_scale * q . k_t - max)
 // The queries of all heads that share a key/value head are rows of one problem (row = i * group + head in group).  They are the
 // eight columns of mma.sync m16n8k16, and keys and (transposed) values its sixteen rows: one token of a model with eight query heads
-// for each key/value head fills a tile.  (With the queries as the sixteen rows half of
-// every tile was empty.)  Codes enter the products as exact FP16 integers, made of bytes by XOR-ing them into 1024 + 128 (one LOP3 for two,
-// then 1152 is subtracted); the key's scale multiplies the FP32 score, the value's goes into the probability before that is rounded to
-// FP16.  What is rounded, a probability times the scale of its values, is held relative to the largest of those that the row has seen,
-// times 2^10, whatever the largest probability: FP16 has its eleven bits down to 2^-24 of that.  Where the results are BF16 that is all; where they are FP16 what the rounding left
-// takes part in a second product, so that results are off by their own rounding alone (without it by 1.4 to 1.5 times that, root mean
-// square, and one token over 65501 takes 29.7 us instead of 29.9, 8 sequences of 8000 with 32 rows 60 instead of 69).  Scores, maxima,
-// sums and outputs are FP32.
+// for each key/value head fills a tile.  (With the queries as the sixteen rows half of every tile was empty.)  Codes enter the
+// products as exact FP16 integers, made of bytes by XOR-ing them into 1024 + 128 (one LOP3 for two, then 1152 is subtracted); the key's
+// scale multiplies the FP32 score, the value's goes into the probability before that is rounded to FP16.  What is rounded, a probability
+// times the scale of its values, is held relative to the largest of those that the row has seen, times 2^10, whatever the largest
+// probability: FP16 has its eleven bits down to 2^-24 of that.  Where the results are BF16 that is all; where they are FP16 what the
+// rounding left takes part in a second product, so that results are off by their own rounding alone (without it by 1.4 to 1.5 times
+// that, root mean square, and one token over 65501 takes 29.7 us instead of 29.9, 8 sequences of 8000 with 32 rows 60 instead of 69).
+// Scores, maxima, sums and outputs are FP32.
 //
 // Bound: HBM, one byte a number of the cache.  A warp streams blocks of its own through a ring in shared memory (bulk copies: 4 KB of
 // keys and 4 KB of values at D = 128), keeps its own running maximum, sum and output, and meets the others at the end of a run

@@ -1,8 +1,8 @@
 // Attention of many new tokens (a prompt, or a chunk of one) over the 8-bit cache, on the 5th-generation tensor cores.
 //
 // The same definition as kv_attention.cu, and the same arithmetic: codes are exact FP16 integers in both products, the keys' scales
-// multiply FP32 scores, the values' scales enter the probabilities before those are rounded to FP16 (relative to the largest such weight that the row has seen,
-// times 2^9; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
+// multiply FP32 scores, the values' scales enter the probabilities before those are rounded to FP16 (relative to the largest such weight
+// that the row has seen, times 2^9; here once, without what the rounding leaves), maxima, sums and outputs are FP32.
 //
 // A unit of work is 256 rows (row = query * group + head in group) of one sequence and key/value head, as two tiles A and B of 128,
 // against its visible tokens in steps of 128 (four blocks).  Roles of a CTA's sixteen warps, one CTA per SM:
@@ -287,6 +287,10 @@ __device__ __forceinline__ float2 range_of(const T* numbers, int count, int lane
     }
     return make_float2(top, least);
 }
+
+// The inverse of a power of two.
+__device__ __forceinline__ float inverse_power(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
+
 // Adds the block that is being filled, of BF16 numbers that lie far apart, to a row's results: all in FP32 from the numbers as they came, a
 // thread for its row, as the kernel for few rows does.  `top`, `level` and `sum` are the row's, its numbers lie in TMEM; by a whole warp.
 template <int D>
@@ -341,9 +345,6 @@ __device__ __forceinline__ void add_tail(const __nv_bfloat16* q, const __nv_bflo
     top = now;
     level = kHeadroom + 32.0f;                           // TMEM holds sums times kShrink
 }
-
-// The inverse of a power of two.
-__device__ __forceinline__ float inverse_power(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
@@ -605,7 +606,8 @@ kv_prefill_kernel(const PrefillParams p) {
                         const float factor = kBf16 ? exp2_fast(rise > 126.0f ? 126.0f : rise) : inverse;      // (NaN stays)
                         // Where results are FP16 the sum is of the weights as they were rounded, so that what a row's large ones were
                         // off by goes out of its result: root mean square 1.4 times the result's own rounding at most, where it was up to
-                        // 1.6 (2048 queries at 8192 take 12 us longer for it).  Not of a block whose values are so small that its weights run out of bits.
+                        // 1.6 (2048 queries at 8192 take 12 us longer for it).  Not of a block whose values are so small that its weights
+                        // run out of bits.
                         const bool as_rounded = !kBf16 && rise >= kHeadroom - 4.0f;
                         const uint64_t by2 = pair_of(by, by), with2 = pair_of(with, with), factor2 = pair_of(factor, factor);
                         uint64_t sums[2] = {0, 0};
@@ -634,6 +636,7 @@ kv_prefill_kernel(const PrefillParams p) {
                     }
                     anew = __any_sync(0xffffffffu, largest_sum > kLargestSum);
                     if (!anew) break;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");      // (these weights are written over)
                 }
                 sum += step_sum;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
